@@ -54,6 +54,14 @@ typedef enum rk_dtype {
   RK_DTYPE_BF16 = 1
 } rk_dtype;
 
+/* Element types of an 8-bit K/V cache: E4M3 has 4 exponent and 3 mantissa bits (largest value
+ * 448, no infinities), INT8 holds -127..127.  A stored value stands for itself times the fp32
+ * scale of its block and head. */
+typedef enum rk_cache_dtype {
+  RK_CACHE_E4M3 = 0,
+  RK_CACHE_INT8 = 1
+} rk_cache_dtype;
+
 /* GEMM variants (the `variant` launch parameter of the dispatch manifest). */
 enum {
   RK_GEMM_AUTO = 0,        /* pick from shape, alignment and device */
@@ -420,6 +428,119 @@ RK_API rk_status rk_sdpa(const void* query, const void* key, const void* value, 
                          int64_t batch, int64_t query_heads, int64_t kv_heads,
                          int64_t sequence, int64_t head_dim, int is_causal, float scale,
                          rk_dtype dt, rk_stream_t stream);
+
+/*
+ * Rotary positions of queries and keys.  The first `rotary_dim` elements of each head are
+ * rotary_dim / 2 pairs -- (i, i + rotary_dim / 2), or (2i, 2i + 1) with `interleaved` -- and
+ * pair i of a token at position p is turned by the angle p * frequencies[i]:
+ *   (a, b) -> amplitude * (a cos - b sin, b cos + a sin);
+ * the rest of the head is copied.  `inverse` turns by the negative angle: applied to the
+ * gradients of the outputs it gives those of the inputs.  query: [tokens, query_heads,
+ * head_dim], key: [tokens, kv_heads, head_dim], read in place with the given strides between
+ * tokens and heads (in elements; the elements of a head are adjacent), so parts of a joint
+ * projection need no copy; query_out, key_out: dense, overlapping no input.  positions: [tokens] int32 or
+ * int64 (index_bits), any sign; frequencies: [rotary_dim / 2] fp64, radians per position.
+ * Angles are formed and reduced in fp64, so they are as exact at position 2^30 as at 1; the
+ * turn is fp32 and each output is rounded once.  rotary_dim even, 2 <= rotary_dim <= head_dim
+ * <= 1024; query_heads, kv_heads <= 32767.  tokens == 0: nothing to do.  No counterpart in
+ * the reference.
+ */
+RK_API rk_status rk_rotary_embedding(const void* query, const void* key, const void* positions,
+                                     const double* frequencies, void* query_out, void* key_out,
+                                     int64_t tokens, int64_t query_heads, int64_t kv_heads,
+                                     int64_t head_dim, int64_t rotary_dim,
+                                     int64_t query_token_stride, int64_t query_head_stride,
+                                     int64_t key_token_stride, int64_t key_head_stride,
+                                     int interleaved, int inverse, float amplitude, rk_dtype dt,
+                                     int index_bits, rk_stream_t stream);
+
+/*
+ * Block tables and slot map of one step of a paged K/V cache, from the requests' lengths.
+ * Request b holds context_lengths[b] tokens, in the blocks of row b of block_tables, and
+ * gets new_lengths[b] more (0: none).  Written:
+ *   block_tables    entries [ceil(has / block_size), ceil((has + gets) / block_size)) of each
+ *                   row, taken from free_blocks in request order; no other entry;
+ *   slot_mapping    [tokens] int64: block * block_size + offset of every new token, the
+ *                   requests' tokens one after the other; -1 behind the last;
+ *   positions       [tokens]: its position in its request; 0 behind the last;
+ *   lengths_out     [batch]: has + gets, at most max_blocks * block_size; may be
+ *                   context_lengths only if it is not read again by this step;
+ *   blocks_used     [1]: entries of free_blocks that the step needs.
+ * All index arrays but slot_mapping are int32 or int64 (index_bits).  Where free_blocks is too
+ * short, entries and slots that miss a block are -1; tokens past the end of their table row
+ * and those of an entry below 0 have slot -1; a negative length counts as 0.  Each of these,
+ * and more tokens than `tokens`, makes the next rk_device_status() report
+ * RK_ERR_INVALID_ARGUMENT (blocks_used > free_count says that the list was too short).
+ * batch, max_blocks, block_size >= 1; tokens, free_count >= 0; max_blocks * block_size <
+ * 2^31.  No counterpart in the reference.
+ */
+RK_API rk_status rk_paged_slots(void* block_tables, const void* context_lengths,
+                                const void* new_lengths, const void* free_blocks,
+                                int64_t* slot_mapping, void* positions, void* lengths_out,
+                                void* blocks_used, int64_t batch, int64_t max_blocks,
+                                int64_t block_size, int64_t free_count, int64_t tokens,
+                                int index_bits, rk_stream_t stream);
+
+/*
+ * Appends new keys and values to a paged cache in 8 bits.  key, value: [tokens, kv_heads,
+ * head_dim] of dtype `dt`, with strides between tokens and heads (in elements, multiples of
+ * 8; 16-byte aligned); key_cache, value_cache: [num_blocks, block_size, kv_heads, head_dim]
+ * of type `cache`; key_scales, value_scales: [num_blocks, kv_heads] fp32; slot_mapping:
+ * [tokens] int32 or int64 (index_bits), token t's place block * block_size + offset; a
+ * negative slot skips the token.  Caches and scales are updated in place.  For each cache,
+ * block and head that gets rows:
+ *   need  = the least power of two (at least 2^-126) with max |row| <= LARGEST * need,
+ *           LARGEST = 448 (E4M3) or 127 (INT8), over the finite elements of the new rows;
+ *   scale = need if the call writes the block's first slot, else max(old scale, need);
+ *   new rows are stored as round(x / scale), nearest even, saturating (NaN: NaN in E4M3, 0
+ *   in INT8); where the scale grew, the block's other rows below the last new one become
+ *   round(stored * old / scale).  Rows behind the last new one stay as they are.
+ * The tokens of one block are adjacent in slot_mapping and their slots ascend, as
+ * rk_paged_slots lays them out; a later run of tokens for a block that the call has already
+ * written is skipped, and it and slots >= num_blocks * block_size make the next
+ * rk_device_status() report RK_ERR_INVALID_ARGUMENT.  head_dim 64, 128 or 256; 1 <=
+ * block_size <= 1024; tokens < 2^30.  workspace: rk_paged_cache_append_8bit_workspace_size()
+ * bytes, uninitialised.  No counterpart in the reference.
+ */
+RK_API rk_status rk_paged_cache_append_8bit(const void* key, const void* value, void* key_cache,
+                                            void* value_cache, float* key_scales,
+                                            float* value_scales, const void* slot_mapping,
+                                            int64_t tokens, int64_t kv_heads, int64_t head_dim,
+                                            int64_t num_blocks, int64_t block_size,
+                                            int64_t key_token_stride, int64_t key_head_stride,
+                                            int64_t value_token_stride, int64_t value_head_stride,
+                                            rk_dtype dt, rk_cache_dtype cache, int index_bits,
+                                            void* workspace, size_t workspace_bytes,
+                                            rk_stream_t stream);
+
+/* Workspace bytes of rk_paged_cache_append_8bit (0 for few tokens). */
+RK_API rk_status rk_paged_cache_append_8bit_workspace_size(int64_t tokens, int64_t num_blocks,
+                                                           size_t* bytes);
+
+/*
+ * rk_paged_attention_decode over a cache in 8 bits with a scale per block and head:
+ *   out[b,h,:] = softmax_t(scale * query[b,h,:] . K[b,t,:]) @ V[b,t,:],  t < context_lengths[b],
+ * K[b,t] = key_scales[block, g] * key_cache[block, t % block_size, g], V alike, with block =
+ * block_tables[b, t / block_size] and g the KV head of h.  Shapes, index types, empty
+ * sequences (NaN), clamped lengths and block-table entries out of range (skipped and
+ * reported) as there; any query_heads / kv_heads and any block_size.  Scales are finite and
+ * >= 0.  The caches are 16-byte aligned, the query 8-byte.  fp32 scores, softmax and sums;
+ * the weights of V are rounded to fp16 (relative to the largest of the head), the output
+ * once.  workspace: rk_paged_attention_decode_8bit_workspace_size() bytes, uninitialised, its
+ * size independent of batch and lengths; calls that may overlap need one each.  No
+ * counterpart in the reference.
+ */
+RK_API rk_status rk_paged_attention_decode_8bit(
+    const void* query, const void* key_cache, const void* value_cache, const float* key_scales,
+    const float* value_scales, const void* block_tables, const void* context_lengths, void* out,
+    int64_t batch, int64_t query_heads, int64_t kv_heads, int64_t head_dim, int64_t num_blocks,
+    int64_t block_size, int64_t max_blocks_per_sequence, float scale, rk_dtype dt,
+    rk_cache_dtype cache, int index_bits, void* workspace, size_t workspace_bytes,
+    rk_stream_t stream);
+
+/* Workspace bytes of rk_paged_attention_decode_8bit on the current device. */
+RK_API rk_status rk_paged_attention_decode_8bit_workspace_size(int64_t query_heads, int64_t kv_heads,
+                                                               int64_t head_dim, size_t* bytes);
 
 /* Static description of a status code; never NULL. */
 RK_API const char* rk_status_string(rk_status status);

@@ -1,0 +1,178 @@
+// paged_slots.cu -- block tables and slot maps of one step, from the requests' lengths.
+//
+// Request b holds h_b tokens and gets n_b more.  Its blocks grow from ceil(h_b / block_size)
+// to ceil((h_b + n_b) / block_size); the new ones come from the list of free blocks in request
+// order, so request b takes the list from the exclusive sum of those differences on, and
+// its tokens take the output from the exclusive sum of n on.  Both sums are a scan over the
+// requests.
+//
+// One launch, no workspace: every CTA repeats the whole scan (a few KB from L2) and then
+// handles its own stretch of tokens and its own share of the table rows, so no CTA waits for
+// another.  New entries are taken from the free list by both the CTA that writes them and
+// those that need them; entries of blocks that a request had are only read.
+//
+// What bounds it: launch and memory latency (two dependent loads) for a decode step, the
+// bytes of the slot map and positions for a prefill.
+#include <cuda_runtime.h>
+
+#include "rk_device.cuh"
+#include "rk_internal.h"
+
+namespace rk {
+namespace {
+
+constexpr int THREADS = 256;
+constexpr int TOKENS_PER_CTA = 512;
+
+template <typename Index>
+struct SlotParams {
+  Index* tables;
+  const Index* has;
+  const Index* gets;
+  const Index* free_blocks;
+  int64_t* slots;
+  Index* positions;
+  Index* lengths;
+  Index* used;
+  int64_t batch, max_blocks, block_size, free_count, tokens;
+};
+
+// Inclusive sums over the CTA of two values, in thread order.
+__device__ __forceinline__ void scan2(int64_t& a, int64_t& b, int64_t (*warp_sums)[2]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t x = __shfl_up_sync(0xffffffffu, a, o), y = __shfl_up_sync(0xffffffffu, b, o);
+    if (lane >= o) {
+      a += x;
+      b += y;
+    }
+  }
+  if (lane == 31) {
+    warp_sums[warp][0] = a;
+    warp_sums[warp][1] = b;
+  }
+  __syncthreads();
+  for (int w = 0; w < warp; ++w) {
+    a += warp_sums[w][0];
+    b += warp_sums[w][1];
+  }
+}
+
+template <typename Index>
+__global__ void __launch_bounds__(THREADS) paged_slots_kernel(SlotParams<Index> p, KernelCtl ctl) {
+  __shared__ int64_t warp_sums[THREADS / 32][2];
+  __shared__ int64_t s_end[THREADS];    // tokens of the requests up to and with this one
+  __shared__ int64_t s_has[THREADS];    // tokens that the request had
+  __shared__ int64_t s_first[THREADS];  // its first entry of the free list
+  __shared__ int64_t s_old[THREADS], s_want[THREADS];  // its blocks before and after
+  pdl_begin();
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * TOKENS_PER_CTA;
+  const int64_t t1 = min(t0 + TOKENS_PER_CTA, p.tokens);
+  const int64_t room = p.max_blocks * p.block_size;
+  int64_t token_base = 0, free_base = 0;  // sums over the requests of earlier rounds
+  bool bad = false;
+  for (int64_t base = 0; base < p.batch; base += THREADS) {
+    const int64_t r = base + threadIdx.x;
+    int64_t has = 0, gets = 0;
+    if (r < p.batch) {
+      has = static_cast<int64_t>(p.has[r]);
+      gets = static_cast<int64_t>(p.gets[r]);
+      bad = bad || has < 0 || gets < 0 || has > room || gets > room || has + gets > room;
+      has = min(max(has, int64_t{0}), room);
+      gets = max(gets, int64_t{0});
+    }
+    const int64_t end = min(has + min(gets, room), room);
+    gets = min(gets, p.tokens);  // a larger count overruns the token buffer in any case
+    const int64_t old = (has + p.block_size - 1) / p.block_size;
+    const int64_t want = (end + p.block_size - 1) / p.block_size;
+    int64_t tokens = gets, blocks = want - old;
+    scan2(tokens, blocks, warp_sums);
+    s_end[threadIdx.x] = token_base + tokens;
+    s_has[threadIdx.x] = has;
+    s_first[threadIdx.x] = free_base + blocks - (want - old);
+    s_old[threadIdx.x] = old;
+    s_want[threadIdx.x] = want;
+    __syncthreads();
+    const int n = static_cast<int>(min(static_cast<int64_t>(THREADS), p.batch - base));
+    if (blockIdx.x == 0 && r < p.batch) p.lengths[r] = static_cast<Index>(end);
+    // Table rows: a warp per request of this CTA's share.
+    for (int i = blockIdx.x + gridDim.x * (threadIdx.x >> 5); i < n; i += gridDim.x * (THREADS / 32)) {
+      for (int64_t j = s_old[i] + (threadIdx.x & 31); j < s_want[i]; j += 32) {
+        const int64_t at = s_first[i] + j - s_old[i];
+        if (at >= p.free_count) bad = true;
+        p.tables[(base + i) * p.max_blocks + j] = at < p.free_count ? p.free_blocks[at] : static_cast<Index>(-1);
+      }
+    }
+    // Tokens of these requests that fall into this CTA's stretch.
+    const int64_t from = max(t0, token_base), to = min(t1, s_end[n - 1]);
+    for (int64_t t = from + threadIdx.x; t < to; t += THREADS) {
+      int lo = 0, hi = n - 1;  // the first request whose end is behind t
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (s_end[mid] > t) hi = mid;
+        else lo = mid + 1;
+      }
+      const int64_t before = lo == 0 ? token_base : s_end[lo - 1];
+      const int64_t position = s_has[lo] + t - before;
+      const int64_t j = position / p.block_size;
+      int64_t block = -1;
+      if (j < s_old[lo]) {
+        block = static_cast<int64_t>(p.tables[(base + lo) * p.max_blocks + j]);
+      } else if (j < s_want[lo]) {
+        const int64_t at = s_first[lo] + j - s_old[lo];
+        if (at < p.free_count) block = static_cast<int64_t>(p.free_blocks[at]);
+      }
+      bad = bad || block < 0;
+      p.slots[t] = block < 0 ? -1 : block * p.block_size + position - j * p.block_size;
+      p.positions[t] = static_cast<Index>(position);
+    }
+    token_base = s_end[THREADS - 1];  // threads past the batch add nothing
+    free_base = s_first[THREADS - 1] + s_want[THREADS - 1] - s_old[THREADS - 1];
+    __syncthreads();  // the arrays are written again
+  }
+  for (int64_t t = max(t0, token_base) + threadIdx.x; t < t1; t += THREADS) {
+    p.slots[t] = -1;
+    p.positions[t] = 0;
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    p.used[0] = static_cast<Index>(free_base);
+    bad = bad || token_base > p.tokens;
+  }
+  if (bad) atomicOr(ctl.status, RK_DEV_ERR_BAD_INDEX);
+}
+
+template <typename Index>
+cudaError_t launch(const PagedSlotsArgs& a, const KernelCtl& ctl, cudaStream_t s) {
+  SlotParams<Index> p{};
+  p.tables = static_cast<Index*>(a.block_tables);
+  p.has = static_cast<const Index*>(a.context_lengths);
+  p.gets = static_cast<const Index*>(a.new_lengths);
+  p.free_blocks = static_cast<const Index*>(a.free_blocks);
+  p.slots = a.slot_mapping;
+  p.positions = static_cast<Index*>(a.positions);
+  p.lengths = static_cast<Index*>(a.lengths_out);
+  p.used = static_cast<Index*>(a.blocks_used);
+  p.batch = a.batch;
+  p.max_blocks = a.max_blocks;
+  p.block_size = a.block_size;
+  p.free_count = a.free_count;
+  p.tokens = a.tokens;
+  const int64_t ctas = (a.tokens + TOKENS_PER_CTA - 1) / TOKENS_PER_CTA;
+  return launch_kernel(paged_slots_kernel<Index>, dim3(static_cast<unsigned>(ctas < 1 ? 1 : ctas)), dim3(THREADS), 0,
+                       s, 0, p, ctl);
+}
+
+}  // namespace
+
+rk_status paged_slots_launch(const PagedSlotsArgs& a, cudaStream_t s) {
+  LaunchCtl lc;
+  const rk_status st = launch_ctl(&lc);
+  if (st != RK_OK) return st;
+  const KernelCtl ctl{lc.status, lc.timeout_ns, 0};
+  const cudaError_t e = a.index_bits == 32 ? launch<int32_t>(a, ctl, s) : launch<int64_t>(a, ctl, s);
+  note_launch("paged_slots_kernel");
+  return cuda_status(e);
+}
+
+}  // namespace rk

@@ -421,6 +421,195 @@ rk_status rk_sdpa(const void* query, const void* key, const void* value, void* o
                      is_causal != 0, scale, dt, reinterpret_cast<cudaStream_t>(stream));
 }
 
+rk_status rk_rotary_embedding(const void* query, const void* key, const void* positions,
+                              const double* frequencies, void* query_out, void* key_out,
+                              int64_t tokens, int64_t query_heads, int64_t kv_heads,
+                              int64_t head_dim, int64_t rotary_dim, int64_t query_token_stride,
+                              int64_t query_head_stride, int64_t key_token_stride,
+                              int64_t key_head_stride, int interleaved, int inverse,
+                              float amplitude, rk_dtype dt, int index_bits, rk_stream_t stream) {
+  if (!valid_dtype(dt) || tokens < 0 || query_heads < 1 || kv_heads < 1 || head_dim < 2 ||
+      rotary_dim < 2 || rotary_dim % 2 != 0 || rotary_dim > head_dim ||
+      (index_bits != 32 && index_bits != 64) || !(amplitude >= -3.4e38f && amplitude <= 3.4e38f) ||
+      query_token_stride < 0 || query_head_stride < 0 || key_token_stride < 0 || key_head_stride < 0)
+    return RK_ERR_INVALID_ARGUMENT;
+  if (head_dim > 1024 || query_heads > 32767 || kv_heads > 32767 || tokens > INT32_MAX) return RK_ERR_UNSUPPORTED;
+  if (tokens == 0) return RK_OK;
+  if (query == nullptr || key == nullptr || positions == nullptr || frequencies == nullptr ||
+      query_out == nullptr || key_out == nullptr)
+    return RK_ERR_INVALID_ARGUMENT;
+  if (current_device_info() == nullptr) return RK_ERR_NO_DEVICE;
+  RotaryArgs a{};
+  a.query = query;
+  a.key = key;
+  a.positions = positions;
+  a.frequencies = frequencies;
+  a.query_out = query_out;
+  a.key_out = key_out;
+  a.tokens = tokens;
+  a.query_heads = query_heads;
+  a.kv_heads = kv_heads;
+  a.head_dim = head_dim;
+  a.rotary_dim = rotary_dim;
+  a.query_token_stride = query_token_stride;
+  a.query_head_stride = query_head_stride;
+  a.key_token_stride = key_token_stride;
+  a.key_head_stride = key_head_stride;
+  a.amplitude = amplitude;
+  a.interleaved = interleaved != 0;
+  a.inverse = inverse != 0;
+  a.dt = dt;
+  a.index_bits = index_bits;
+  return rotary_launch(a, reinterpret_cast<cudaStream_t>(stream));
+}
+
+rk_status rk_paged_slots(void* block_tables, const void* context_lengths, const void* new_lengths,
+                         const void* free_blocks, int64_t* slot_mapping, void* positions,
+                         void* lengths_out, void* blocks_used, int64_t batch, int64_t max_blocks,
+                         int64_t block_size, int64_t free_count, int64_t tokens, int index_bits,
+                         rk_stream_t stream) {
+  if (batch < 1 || max_blocks < 1 || block_size < 1 || free_count < 0 || tokens < 0 ||
+      (index_bits != 32 && index_bits != 64))
+    return RK_ERR_INVALID_ARGUMENT;
+  if (block_tables == nullptr || context_lengths == nullptr || new_lengths == nullptr ||
+      lengths_out == nullptr || blocks_used == nullptr || (free_count > 0 && free_blocks == nullptr) ||
+      (tokens > 0 && (slot_mapping == nullptr || positions == nullptr)))
+    return RK_ERR_INVALID_ARGUMENT;
+  if (max_blocks > INT32_MAX || block_size > INT32_MAX || max_blocks * block_size > INT32_MAX ||
+      batch > INT32_MAX || tokens > INT32_MAX)
+    return RK_ERR_UNSUPPORTED;
+  if (current_device_info() == nullptr) return RK_ERR_NO_DEVICE;
+  PagedSlotsArgs a{};
+  a.block_tables = block_tables;
+  a.context_lengths = context_lengths;
+  a.new_lengths = new_lengths;
+  a.free_blocks = free_blocks;
+  a.slot_mapping = slot_mapping;
+  a.positions = positions;
+  a.lengths_out = lengths_out;
+  a.blocks_used = blocks_used;
+  a.batch = batch;
+  a.max_blocks = max_blocks;
+  a.block_size = block_size;
+  a.free_count = free_count;
+  a.tokens = tokens;
+  a.index_bits = index_bits;
+  return paged_slots_launch(a, reinterpret_cast<cudaStream_t>(stream));
+}
+
+static bool valid_cache(rk_cache_dtype c) { return c == RK_CACHE_E4M3 || c == RK_CACHE_INT8; }
+static bool valid_head_dim(int64_t d) { return d == 64 || d == 128 || d == 256; }
+
+rk_status rk_paged_cache_append_8bit_workspace_size(int64_t tokens, int64_t num_blocks, size_t* bytes) {
+  if (bytes == nullptr) return RK_ERR_INVALID_ARGUMENT;
+  *bytes = 0;
+  if (tokens < 0 || num_blocks < 1) return RK_ERR_INVALID_ARGUMENT;
+  *bytes = paged_append8_workspace_bytes(tokens, num_blocks);
+  return RK_OK;
+}
+
+rk_status rk_paged_cache_append_8bit(const void* key, const void* value, void* key_cache,
+                                     void* value_cache, float* key_scales, float* value_scales,
+                                     const void* slot_mapping, int64_t tokens, int64_t kv_heads,
+                                     int64_t head_dim, int64_t num_blocks, int64_t block_size,
+                                     int64_t key_token_stride, int64_t key_head_stride,
+                                     int64_t value_token_stride, int64_t value_head_stride,
+                                     rk_dtype dt, rk_cache_dtype cache, int index_bits,
+                                     void* workspace, size_t workspace_bytes, rk_stream_t stream) {
+  if (!valid_dtype(dt) || !valid_cache(cache) || tokens < 0 || kv_heads < 1 || num_blocks < 1 ||
+      block_size < 1 || !valid_head_dim(head_dim) || (index_bits != 32 && index_bits != 64) ||
+      key_token_stride < 0 || key_head_stride < 0 || value_token_stride < 0 || value_head_stride < 0)
+    return RK_ERR_INVALID_ARGUMENT;
+  if (block_size > 1024 || num_blocks > INT32_MAX || kv_heads > 65535 || tokens >= (int64_t{1} << 30))
+    return RK_ERR_UNSUPPORTED;
+  if (tokens == 0) return RK_OK;
+  if (key == nullptr || value == nullptr || key_cache == nullptr || value_cache == nullptr ||
+      key_scales == nullptr || value_scales == nullptr || slot_mapping == nullptr)
+    return RK_ERR_INVALID_ARGUMENT;
+  if (!aligned16(key) || !aligned16(value) || !aligned16(key_cache) || !aligned16(value_cache) ||
+      key_token_stride % 8 != 0 || key_head_stride % 8 != 0 || value_token_stride % 8 != 0 ||
+      value_head_stride % 8 != 0)
+    return RK_ERR_UNSUPPORTED;
+  if (current_device_info() == nullptr) return RK_ERR_NO_DEVICE;
+  PagedAppend8Args a{};
+  a.key = key;
+  a.value = value;
+  a.slot_mapping = slot_mapping;
+  a.key_cache = key_cache;
+  a.value_cache = value_cache;
+  a.key_scales = key_scales;
+  a.value_scales = value_scales;
+  a.tokens = tokens;
+  a.kv_heads = kv_heads;
+  a.head_dim = head_dim;
+  a.num_blocks = num_blocks;
+  a.block_size = block_size;
+  a.key_token_stride = key_token_stride;
+  a.key_head_stride = key_head_stride;
+  a.value_token_stride = value_token_stride;
+  a.value_head_stride = value_head_stride;
+  a.dt = dt;
+  a.cache = cache;
+  a.index_bits = index_bits;
+  return paged_append8_launch(a, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
+}
+
+rk_status rk_paged_attention_decode_8bit_workspace_size(int64_t query_heads, int64_t kv_heads,
+                                                        int64_t head_dim, size_t* bytes) {
+  if (bytes == nullptr) return RK_ERR_INVALID_ARGUMENT;
+  *bytes = 0;
+  if (query_heads < 1 || kv_heads < 1 || query_heads % kv_heads != 0 || !valid_head_dim(head_dim))
+    return RK_ERR_INVALID_ARGUMENT;
+  if (current_device_info() == nullptr) return RK_ERR_NO_DEVICE;
+  *bytes = paged_attention8_workspace_bytes(query_heads, kv_heads, head_dim);
+  return RK_OK;
+}
+
+rk_status rk_paged_attention_decode_8bit(
+    const void* query, const void* key_cache, const void* value_cache, const float* key_scales,
+    const float* value_scales, const void* block_tables, const void* context_lengths, void* out,
+    int64_t batch, int64_t query_heads, int64_t kv_heads, int64_t head_dim, int64_t num_blocks,
+    int64_t block_size, int64_t max_blocks, float scale, rk_dtype dt, rk_cache_dtype cache,
+    int index_bits, void* workspace, size_t workspace_bytes, rk_stream_t stream) {
+  if (batch < 1 || query_heads < 1 || kv_heads < 1 || query_heads % kv_heads != 0 || num_blocks < 1 ||
+      block_size < 1 || max_blocks < 1 || !valid_dtype(dt) || !valid_cache(cache) ||
+      !valid_head_dim(head_dim) || (index_bits != 32 && index_bits != 64) ||
+      !(scale > 0.0f && scale <= 3.4e38f))
+    return RK_ERR_INVALID_ARGUMENT;
+  if (query == nullptr || key_cache == nullptr || value_cache == nullptr || key_scales == nullptr ||
+      value_scales == nullptr || block_tables == nullptr || context_lengths == nullptr || out == nullptr)
+    return RK_ERR_INVALID_ARGUMENT;
+  if ((reinterpret_cast<uintptr_t>(query) & 7u) != 0 || (reinterpret_cast<uintptr_t>(out) & 3u) != 0 ||
+      !aligned16(key_cache) || !aligned16(value_cache))
+    return RK_ERR_UNSUPPORTED;
+  // Positions of a unit's last tile stay below 2^31.
+  if (num_blocks > INT32_MAX || block_size > INT32_MAX || max_blocks > INT32_MAX ||
+      max_blocks * block_size > INT32_MAX - 64 || batch > INT32_MAX || batch * query_heads > INT32_MAX)
+    return RK_ERR_UNSUPPORTED;
+  if (current_device_info() == nullptr) return RK_ERR_NO_DEVICE;
+  PagedAttention8Args a{};
+  a.query = query;
+  a.key_cache = key_cache;
+  a.value_cache = value_cache;
+  a.block_tables = block_tables;
+  a.context_lengths = context_lengths;
+  a.key_scales = key_scales;
+  a.value_scales = value_scales;
+  a.out = out;
+  a.batch = batch;
+  a.hq = query_heads;
+  a.hkv = kv_heads;
+  a.head_dim = head_dim;
+  a.num_blocks = num_blocks;
+  a.block_size = block_size;
+  a.max_blocks = max_blocks;
+  a.scale = scale;
+  a.dt = dt;
+  a.cache = cache;
+  a.index_bits = index_bits;
+  return paged_attention8_launch(a, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
+}
+
 void rk_paged_attention_set_path(int path) { paged_attention_set_path(path); }
 
 void rk_norm_backward_set_ctas_per_sm(int ctas_per_sm) {

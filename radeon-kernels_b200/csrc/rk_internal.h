@@ -149,6 +149,59 @@ rk_status sdpa_launch(const void* q, const void* k, const void* v, void* out, in
                       int64_t Hq, int64_t Hkv, int64_t S, int64_t D, bool causal, float scale,
                       rk_dtype dt, cudaStream_t s);
 
+// Rotary positions (rotary.cu).  Strides in elements; the outputs are dense.
+struct RotaryArgs {
+  const void *query, *key, *positions;
+  const double* frequencies;
+  void *query_out, *key_out;
+  int64_t tokens, query_heads, kv_heads, head_dim, rotary_dim;
+  int64_t query_token_stride, query_head_stride, key_token_stride, key_head_stride;
+  float amplitude;
+  bool interleaved, inverse;
+  rk_dtype dt;
+  int index_bits;
+};
+rk_status rotary_launch(const RotaryArgs& a, cudaStream_t s);
+
+// Block tables and slot maps of one step (paged_slots.cu).
+struct PagedSlotsArgs {
+  void* block_tables;
+  const void *context_lengths, *new_lengths, *free_blocks;
+  int64_t* slot_mapping;
+  void *positions, *lengths_out, *blocks_used;
+  int64_t batch, max_blocks, block_size, free_count, tokens;
+  int index_bits;
+};
+rk_status paged_slots_launch(const PagedSlotsArgs& a, cudaStream_t s);
+
+// The paged K/V cache in 8 bits: append (paged_append8.cu) and decode attention
+// (paged_attention8.cu).
+struct PagedAppend8Args {
+  const void *key, *value, *slot_mapping;
+  void *key_cache, *value_cache;
+  float *key_scales, *value_scales;
+  int64_t tokens, kv_heads, head_dim, num_blocks, block_size;
+  int64_t key_token_stride, key_head_stride, value_token_stride, value_head_stride;
+  rk_dtype dt;
+  rk_cache_dtype cache;
+  int index_bits;
+};
+size_t paged_append8_workspace_bytes(int64_t tokens, int64_t num_blocks);
+rk_status paged_append8_launch(const PagedAppend8Args& a, void* workspace, size_t workspace_bytes, cudaStream_t s);
+
+struct PagedAttention8Args {
+  const void *query, *key_cache, *value_cache, *block_tables, *context_lengths;
+  const float *key_scales, *value_scales;
+  void* out;
+  int64_t batch, hq, hkv, head_dim, num_blocks, block_size, max_blocks;
+  float scale;
+  rk_dtype dt;
+  rk_cache_dtype cache;
+  int index_bits;
+};
+size_t paged_attention8_workspace_bytes(int64_t hq, int64_t hkv, int64_t head_dim);
+rk_status paged_attention8_launch(const PagedAttention8Args& a, void* workspace, size_t workspace_bytes, cudaStream_t s);
+
 rk_status gather_column_blocks_launch(const void* blocks, void* out, int64_t G, int64_t M,
                                       int64_t N, rk_dtype dt, cudaStream_t s);
 

@@ -410,6 +410,177 @@ at::Tensor sdpa(const at::Tensor& query, const at::Tensor& key, const at::Tensor
   return out;
 }
 
+// Index tensors of one call: int32 or int64, CUDA, contiguous.
+int index_bits_of(const at::Tensor& t, const char* name, int64_t rank) {
+  TORCH_CHECK(t.is_cuda() && t.dim() == rank && t.is_contiguous(), name, " must be a contiguous CUDA tensor of rank ",
+              rank);
+  TORCH_CHECK(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, name, " must use torch.int32 or torch.int64");
+  return t.scalar_type() == at::kInt ? 32 : 64;
+}
+
+// [tokens, heads, head_dim] rows as the kernels read them in place: adjacent elements, any
+// stride between tokens and heads; a dense copy where the last dimension is strided.
+at::Tensor strided_rows(const at::Tensor& t, const char* name) {
+  TORCH_CHECK(t.is_cuda() && t.dim() == 3, name, " must be a CUDA tensor of rank 3");
+  dtype_of(t, name);
+  return t.size(2) <= 1 || t.stride(2) == 1 ? t : t.contiguous();
+}
+
+bool aligned(const at::Tensor& t, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % bytes == 0; }
+
+// The same for kernels that read 16-byte vectors only: also a copy of misaligned rows.
+at::Tensor vector_rows(const at::Tensor& t, const char* name) {
+  const at::Tensor rows = strided_rows(t, name);
+  if (aligned(rows, 16) && rows.stride(0) % 8 == 0 && rows.stride(1) % 8 == 0) return rows;
+  return rows.clone(at::MemoryFormat::Contiguous);
+}
+
+// Rotary positions (rk_rotary_embedding): new dense [query_out, key_out].
+std::vector<at::Tensor> rotary_embedding(const at::Tensor& query_in, const at::Tensor& key_in,
+                                         const at::Tensor& positions_in, const at::Tensor& frequencies_in,
+                                         bool interleaved, double amplitude, bool inverse) {
+  TORCH_CHECK(query_in.is_cuda(), "query must be a CUDA tensor");
+  c10::cuda::CUDAGuard guard(query_in.device());
+  const at::Tensor query = strided_rows(query_in, "query"), key = strided_rows(key_in, "key");
+  const at::Tensor positions = positions_in.contiguous(), frequencies = frequencies_in.contiguous();
+  const int bits = index_bits_of(positions, "positions", 1);
+  TORCH_CHECK(frequencies.is_cuda() && frequencies.dim() == 1 && frequencies.is_contiguous() &&
+                  frequencies.scalar_type() == at::kDouble,
+              "frequencies must be a contiguous CUDA float64 tensor of rank 1");
+  TORCH_CHECK(query.scalar_type() == key.scalar_type(), "query and key must share a dtype");
+  TORCH_CHECK(query.device() == key.device() && query.device() == positions.device() &&
+                  query.device() == frequencies.device(),
+              "all inputs must use the query's device");
+  TORCH_CHECK(key.size(0) == query.size(0) && key.size(2) == query.size(2),
+              "query and key must share tokens and head_dim");
+  TORCH_CHECK(positions.size(0) == query.size(0), "positions must hold one position per token");
+  auto query_out = at::empty(query.sizes(), query.options());
+  auto key_out = at::empty(key.sizes(), key.options());
+  check_status(rk_rotary_embedding(query.data_ptr(), key.data_ptr(), positions.data_ptr(),
+                                   frequencies.data_ptr<double>(), query_out.data_ptr(), key_out.data_ptr(),
+                                   query.size(0), query.size(1), key.size(1), query.size(2), 2 * frequencies.size(0),
+                                   query.stride(0), query.stride(1), key.stride(0), key.stride(1), interleaved ? 1 : 0,
+                                   inverse ? 1 : 0, static_cast<float>(amplitude), dtype_of(query, "query"), bits,
+                                   current_stream(query)),
+               "rk_rotary_embedding");
+  return {query_out, key_out};
+}
+
+// Slot map of one step (rk_paged_slots): block_tables in place, new [slot_mapping, positions,
+// lengths, blocks_used].
+std::vector<at::Tensor> paged_slots(at::Tensor block_tables, const at::Tensor& context_lengths,
+                                    const at::Tensor& new_lengths, const at::Tensor& free_blocks, int64_t num_tokens,
+                                    int64_t block_size) {
+  const int bits = index_bits_of(block_tables, "block_tables", 2);
+  for (const auto& [t, name] : {std::pair<const at::Tensor*, const char*>{&context_lengths, "context_lengths"},
+                                {&new_lengths, "new_lengths"}, {&free_blocks, "free_blocks"}}) {
+    TORCH_CHECK(index_bits_of(*t, name, 1) == bits, "index tensors must share int32 or int64");
+    TORCH_CHECK(t->device() == block_tables.device(), "all inputs must use the device of block_tables");
+  }
+  TORCH_CHECK(context_lengths.size(0) == block_tables.size(0) && new_lengths.size(0) == block_tables.size(0),
+              "lengths must hold one entry per row of block_tables");
+  TORCH_CHECK(num_tokens >= 0, "num_tokens must not be negative");
+  c10::cuda::CUDAGuard guard(block_tables.device());
+  auto slots = at::empty({num_tokens}, block_tables.options().dtype(at::kLong));
+  auto positions = at::empty({num_tokens}, block_tables.options());
+  auto lengths = at::empty({block_tables.size(0)}, block_tables.options());
+  auto used = at::empty({1}, block_tables.options());
+  check_status(rk_paged_slots(block_tables.data_ptr(), context_lengths.data_ptr(), new_lengths.data_ptr(),
+                              free_blocks.data_ptr(), slots.data_ptr<int64_t>(), positions.data_ptr(),
+                              lengths.data_ptr(), used.data_ptr(), block_tables.size(0), block_tables.size(1),
+                              block_size, free_blocks.size(0), num_tokens, bits, current_stream(block_tables)),
+               "rk_paged_slots");
+  return {slots, positions, lengths, used};
+}
+
+rk_cache_dtype cache_dtype_of(const at::Tensor& t, const char* name) {
+  if (t.scalar_type() == at::kFloat8_e4m3fn) return RK_CACHE_E4M3;
+  if (t.scalar_type() == at::kChar) return RK_CACHE_INT8;
+  TORCH_CHECK(false, name, " must use torch.float8_e4m3fn or torch.int8");
+}
+
+// The caches and scales of an 8-bit cache, on `device`.
+void check_cache8(const at::Tensor& key_cache, const at::Tensor& value_cache, const at::Tensor& key_scales,
+                  const at::Tensor& value_scales, const at::Device& device) {
+  for (const auto& [t, name] : {std::pair<const at::Tensor*, const char*>{&key_cache, "key_cache"},
+                                {&value_cache, "value_cache"}}) {
+    TORCH_CHECK(t->is_cuda() && t->dim() == 4 && t->is_contiguous() && t->device() == device, name,
+                " must be a contiguous CUDA tensor of rank 4 on the device of the call");
+    TORCH_CHECK(cache_dtype_of(*t, name) == cache_dtype_of(key_cache, "key_cache"), "caches must share a dtype");
+    TORCH_CHECK(aligned(*t, 16), name, " must start on a 16-byte boundary");
+  }
+  TORCH_CHECK(key_cache.sizes() == value_cache.sizes(), "K/V cache shapes must match");
+  for (const auto& [t, name] : {std::pair<const at::Tensor*, const char*>{&key_scales, "key_scales"},
+                                {&value_scales, "value_scales"}}) {
+    TORCH_CHECK(t->is_cuda() && t->dim() == 2 && t->is_contiguous() && t->device() == device &&
+                    t->scalar_type() == at::kFloat && t->size(0) == key_cache.size(0) && t->size(1) == key_cache.size(2),
+                name, " must be a contiguous CUDA float32 tensor [num_blocks, kv_heads] on the device of the call");
+  }
+}
+
+// Append to an 8-bit cache (rk_paged_cache_append_8bit), in place: [key_cache, value_cache, key_scales,
+// value_scales].
+std::vector<at::Tensor> paged_cache_append_8bit(const at::Tensor& key_in, const at::Tensor& value_in,
+                                                at::Tensor key_cache, at::Tensor value_cache, at::Tensor key_scales,
+                                                at::Tensor value_scales, const at::Tensor& slot_mapping) {
+  TORCH_CHECK(key_in.is_cuda(), "key must be a CUDA tensor");
+  c10::cuda::CUDAGuard guard(key_in.device());
+  const at::Tensor key = vector_rows(key_in, "key"), value = vector_rows(value_in, "value");
+  TORCH_CHECK(key.scalar_type() == value.scalar_type(), "key and value must share a dtype");
+  TORCH_CHECK(key.sizes() == value.sizes() && key.device() == value.device(),
+              "key and value must share shape and device");
+  check_cache8(key_cache, value_cache, key_scales, value_scales, key.device());
+  const int bits = index_bits_of(slot_mapping, "slot_mapping", 1);
+  TORCH_CHECK(slot_mapping.device() == key.device() && slot_mapping.size(0) == key.size(0),
+              "slot_mapping must hold one slot per token, on the device of key");
+  TORCH_CHECK(key_cache.size(2) == key.size(1) && key_cache.size(3) == key.size(2),
+              "key and cache must share heads and head_dim");
+  size_t ws_bytes = 0;
+  check_status(rk_paged_cache_append_8bit_workspace_size(key.size(0), key_cache.size(0), &ws_bytes),
+               "rk_paged_cache_append_8bit_workspace_size");
+  at::Tensor ws;
+  if (ws_bytes > 0) ws = at::empty({static_cast<int64_t>(ws_bytes)}, key.options().dtype(at::kByte));
+  check_status(rk_paged_cache_append_8bit(
+                   key.data_ptr(), value.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
+                   key_scales.data_ptr<float>(), value_scales.data_ptr<float>(), slot_mapping.data_ptr(), key.size(0),
+                   key.size(1), key.size(2), key_cache.size(0), key_cache.size(1), key.stride(0), key.stride(1),
+                   value.stride(0), value.stride(1), dtype_of(key, "key"), cache_dtype_of(key_cache, "key_cache"), bits,
+                   ws_bytes > 0 ? ws.data_ptr() : nullptr, ws_bytes, current_stream(key)),
+               "rk_paged_cache_append_8bit");
+  return {key_cache, value_cache, key_scales, value_scales};
+}
+
+// Decode attention over an 8-bit cache (rk_paged_attention_decode_8bit) -> new output.
+at::Tensor paged_attention_decode_8bit(const at::Tensor& query_in, const at::Tensor& key_cache,
+                                       const at::Tensor& value_cache, const at::Tensor& key_scales,
+                                       const at::Tensor& value_scales, const at::Tensor& block_tables,
+                                       const at::Tensor& context_lengths, double scale) {
+  check_rows(query_in, "query", 3);
+  c10::cuda::CUDAGuard guard(query_in.device());
+  const at::Tensor query = aligned(query_in, 8) ? query_in : query_in.clone();
+  check_cache8(key_cache, value_cache, key_scales, value_scales, query.device());
+  const int bits = index_bits_of(block_tables, "block_tables", 2);
+  TORCH_CHECK(index_bits_of(context_lengths, "context_lengths", 1) == bits, "index tensors must share int32 or int64");
+  TORCH_CHECK(block_tables.device() == query.device() && context_lengths.device() == query.device(),
+              "all inputs must use the query's device");
+  TORCH_CHECK(block_tables.size(0) == query.size(0) && context_lengths.size(0) == query.size(0),
+              "index tensors must have one row per sequence");
+  TORCH_CHECK(key_cache.size(3) == query.size(2), "query and cache head dimensions must match");
+  auto out = at::empty_like(query);
+  size_t ws_bytes = 0;
+  check_status(rk_paged_attention_decode_8bit_workspace_size(query.size(1), key_cache.size(2), query.size(2), &ws_bytes),
+               "rk_paged_attention_decode_8bit_workspace_size");
+  auto ws = at::empty({static_cast<int64_t>(ws_bytes)}, query.options().dtype(at::kByte));
+  check_status(rk_paged_attention_decode_8bit(
+                   query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), key_scales.data_ptr<float>(),
+                   value_scales.data_ptr<float>(), block_tables.data_ptr(), context_lengths.data_ptr(), out.data_ptr(),
+                   query.size(0), query.size(1), key_cache.size(2), query.size(2), key_cache.size(0), key_cache.size(1),
+                   block_tables.size(1), static_cast<float>(scale), dtype_of(query, "query"),
+                   cache_dtype_of(key_cache, "key_cache"), bits, ws.data_ptr(), ws_bytes, current_stream(query)),
+               "rk_paged_attention_decode_8bit");
+  return out;
+}
+
 // ------------------------------------------------------------------ backward passes
 std::vector<at::Tensor> silu_mul_backward(const at::Tensor& grad, const at::Tensor& gate,
                                           const at::Tensor& up) {
@@ -555,6 +726,21 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("ctl_ptrs"), py::arg("rank"), py::arg("timeout_ns") = 0);
   m.def("paged_attention_decode", &paged_attention_decode, "decode attention over a paged K/V cache",
         py::arg("query"), py::arg("key_cache"), py::arg("value_cache"), py::arg("block_tables"),
+        py::arg("context_lengths"), py::arg("scale"));
+  m.def("rotary_embedding", &rotary_embedding, "rotary positions -> [query_out, key_out]", py::arg("query"),
+        py::arg("key"), py::arg("positions"), py::arg("frequencies"), py::arg("interleaved"), py::arg("amplitude"),
+        py::arg("inverse") = false);
+  m.def("paged_slots", &paged_slots,
+        "block tables (in place) and slot map of one step -> [slot_mapping, positions, lengths, blocks_used]",
+        py::arg("block_tables"), py::arg("context_lengths"), py::arg("new_lengths"), py::arg("free_blocks"),
+        py::arg("num_tokens"), py::arg("block_size"));
+  m.def("paged_cache_append_8bit", &paged_cache_append_8bit,
+        "append keys and values to an 8-bit paged cache, in place", py::arg("key"), py::arg("value"),
+        py::arg("key_cache"), py::arg("value_cache"), py::arg("key_scales"), py::arg("value_scales"),
+        py::arg("slot_mapping"));
+  m.def("paged_attention_decode_8bit", &paged_attention_decode_8bit,
+        "decode attention over an 8-bit paged K/V cache", py::arg("query"), py::arg("key_cache"),
+        py::arg("value_cache"), py::arg("key_scales"), py::arg("value_scales"), py::arg("block_tables"),
         py::arg("context_lengths"), py::arg("scale"));
   m.def("gemm_swiglu", &gemm_swiglu, "silu(a @ b[:, :N]) * (a @ b[:, N:])", py::arg("a"),
         py::arg("b"), py::arg("variant") = 0);

@@ -39,6 +39,9 @@ RK_ERR_TOO_LARGE = 6
 # rk_dtype
 RK_DTYPE_FP16 = 0
 RK_DTYPE_BF16 = 1
+# rk_cache_dtype
+RK_CACHE_E4M3 = 0
+RK_CACHE_INT8 = 1
 # variants
 GEMM_VARIANTS = {"auto": 0, "simt": 1, "tc_1sm": 2, "tc_2sm": 3}
 GEMV_VARIANTS = {"auto": 0, "scalar": 1, "stream": 2, "tc": 3}
@@ -79,6 +82,20 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.rk_gemv_allgather_ctl_bytes.restype = cint
     lib.rk_sdpa.argtypes = [vp] * 4 + [i64] * 5 + [cint, ctypes.c_float, cint, vp]
     lib.rk_sdpa.restype = cint
+    size_out = ctypes.POINTER(ctypes.c_size_t)
+    lib.rk_rotary_embedding.argtypes = [vp] * 6 + [i64] * 9 + [cint, cint, ctypes.c_float, cint, cint, vp]
+    lib.rk_rotary_embedding.restype = cint
+    lib.rk_paged_slots.argtypes = [vp] * 8 + [i64] * 5 + [cint, vp]
+    lib.rk_paged_slots.restype = cint
+    lib.rk_paged_cache_append_8bit.argtypes = [vp] * 7 + [i64] * 9 + [cint, cint, cint, vp, ctypes.c_size_t, vp]
+    lib.rk_paged_cache_append_8bit.restype = cint
+    lib.rk_paged_cache_append_8bit_workspace_size.argtypes = [i64, i64, size_out]
+    lib.rk_paged_cache_append_8bit_workspace_size.restype = cint
+    lib.rk_paged_attention_decode_8bit.argtypes = (
+        [vp] * 8 + [i64] * 7 + [ctypes.c_float, cint, cint, cint, vp, ctypes.c_size_t, vp])
+    lib.rk_paged_attention_decode_8bit.restype = cint
+    lib.rk_paged_attention_decode_8bit_workspace_size.argtypes = [i64, i64, i64, size_out]
+    lib.rk_paged_attention_decode_8bit_workspace_size.restype = cint
     lib.rk_silu_mul_backward.argtypes = [vp] * 5 + [i64, i64, cint, vp]
     lib.rk_silu_mul_backward.restype = cint
     lib.rk_rms_norm_backward_workspace_size.argtypes = [i64, i64, ctypes.POINTER(ctypes.c_size_t)]

@@ -13,6 +13,7 @@ served it, or the fallback with the winner's failure reason, or "none".
 
 from __future__ import annotations
 
+import weakref
 from pathlib import Path
 from threading import Lock
 from typing import Any, Callable, Iterable, Mapping
@@ -33,7 +34,19 @@ from radeon_kernels.runtime.registry import DispatchRegistry
 from radeon_kernels.runtime.resources import builtin_dispatch_registry
 
 FALLBACK_PROVIDER = "cuda"
+POSITIONAL_CALLS = 8192  # kinds of call that a runtime keeps ready
 WINNER_FAILURES = (PackResolutionError, ArtifactError, native.NativeProviderError, RuntimeError, TypeError, ValueError)
+
+
+# Every runtime's loaders, for loaded_modules(); a loader that is gone takes its entry along.
+_LOADERS: weakref.WeakSet[Any] = weakref.WeakSet()
+
+
+def loaded_modules() -> list[Any]:
+    """The pack modules that a runtime of this process has loaded and that keep a status word."""
+
+    modules = {id(m): m for loader in list(_LOADERS) for m in getattr(loader, "modules", ())}
+    return [m for m in modules.values() if hasattr(m, "device_status")]
 
 
 class OperatorDispatchError(RadeonKernelsError):
@@ -102,6 +115,7 @@ class DispatchingRuntime:
         with self._lock:
             if root not in self._loaders:
                 self._loaders[root] = self._loader_factory(root)
+                _LOADERS.add(self._loaders[root])
             return self._loaders[root]
 
     @staticmethod
@@ -112,8 +126,12 @@ class DispatchingRuntime:
         """Run a cached winner for ``key`` (operator-specific positional key), or None."""
 
         cached = self._fast_positional.get(key)
-        if cached is None:
-            return None
+        return None if cached is None else self.fast_run(cached, arguments)
+
+    def fast_find(self, key: tuple) -> tuple[Any, Any, dict[str, Any]] | None:
+        return self._fast_positional.get(key)
+
+    def fast_run(self, cached: tuple[Any, Any, dict[str, Any]], arguments: tuple[Any, ...]) -> Any:
         entry, launch, record = cached
         result = entry(*arguments, **launch)
         if result is None:
@@ -126,6 +144,9 @@ class DispatchingRuntime:
 
         cached = self._fast.get(signature_key)
         if cached is not None:
+            if len(self._fast_positional) >= POSITIONAL_CALLS:
+                # Step sizes of a server never stop changing: start over rather than grow.
+                self._fast_positional.clear()
             self._fast_positional[key] = cached
 
     def fast_lookup(self, key: tuple) -> tuple[Any, Any, dict[str, Any]] | None:

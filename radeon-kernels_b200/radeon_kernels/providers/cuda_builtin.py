@@ -27,6 +27,10 @@ SELECTED_ADD_RMS_NORM = "cuda/add_rms_norm"
 SELECTED_GEMM_SWIGLU = "cuda/gemm_swiglu"
 SELECTED_PAGED_ATTENTION = "cuda/paged_attention_decode"
 SELECTED_SDPA = "cuda/sdpa"
+SELECTED_ROTARY = "cuda/rotary_embedding"
+SELECTED_PAGED_SLOTS = "cuda/paged_slots"
+SELECTED_PAGED_APPEND_8BIT = "cuda/paged_cache_append_8bit"
+SELECTED_PAGED_ATTENTION_8BIT = "cuda/paged_attention_decode_8bit"
 
 
 def _contiguous(tensor: Any) -> Any:
@@ -279,3 +283,68 @@ def sdpa(torch_module: Any, query: Any, key: Any, value: Any, is_causal: bool, s
     """rk_sdpa (inference only; the front-end rejects autograd and non-contiguous inputs)."""
 
     return _native.extension().sdpa(query, key, value, is_causal, scale)
+
+
+# ------------------------------------------------- rotary positions and the 8-bit cache
+_ROTARY_FUNCTION: Any = None
+
+
+def _rotary_function() -> Any:
+    global _ROTARY_FUNCTION
+    if _ROTARY_FUNCTION is None:
+        import torch
+
+        class _RotaryFunction(torch.autograd.Function):
+            """A rotation is linear in queries and keys: its gradient is the inverse rotation,
+            which is this function again (so gradients of gradients work too)."""
+
+            @staticmethod
+            def forward(ctx: Any, query: Any, key: Any, positions: Any, frequencies: Any, interleaved: bool,
+                        amplitude: float, inverse: bool) -> Any:
+                ctx.save_for_backward(positions, frequencies)
+                ctx.how = (interleaved, amplitude, inverse)
+                return tuple(
+                    _native.extension().rotary_embedding(query, key, positions, frequencies, interleaved, amplitude, inverse)
+                )
+
+            @staticmethod
+            def backward(ctx: Any, grad_query: Any, grad_key: Any) -> Any:
+                interleaved, amplitude, inverse = ctx.how
+                out = _rotate(torch, grad_query, grad_key, *ctx.saved_tensors, interleaved, amplitude, not inverse)
+                return (*out, None, None, None, None, None)
+
+        _ROTARY_FUNCTION = _RotaryFunction
+    return _ROTARY_FUNCTION
+
+
+def _rotate(torch_module: Any, query: Any, key: Any, positions: Any, frequencies: Any, interleaved: bool,
+            amplitude: float, inverse: bool) -> Any:
+    if _needs_grad(torch_module, query, key):
+        return _rotary_function().apply(query, key, positions, frequencies, interleaved, amplitude, inverse)
+    return _native.extension().rotary_embedding(query, key, positions, frequencies, interleaved, amplitude, inverse)
+
+
+def rotary_embedding(torch_module: Any, query: Any, key: Any, positions: Any, frequencies: Any, interleaved: bool,
+                     amplitude: float) -> Any:
+    """rk_rotary_embedding, with the inverse rotation as its gradient."""
+
+    return _rotate(torch_module, query, key, positions, frequencies, interleaved, amplitude, False)
+
+
+def paged_slots(torch_module: Any, block_tables: Any, context_lengths: Any, new_lengths: Any, free_blocks: Any,
+                num_tokens: int, block_size: int) -> Any:
+    """rk_paged_slots (block_tables in place)."""
+
+    return _native.extension().paged_slots(block_tables, context_lengths, new_lengths, free_blocks, num_tokens, block_size)
+
+
+def paged_cache_append_8bit(torch_module: Any, *arguments: Any) -> Any:
+    """rk_paged_cache_append_8bit (in place, inference only; the front-end rejects autograd inputs)."""
+
+    return _native.extension().paged_cache_append_8bit(*arguments)
+
+
+def paged_attention_decode_8bit(torch_module: Any, *arguments: Any) -> Any:
+    """rk_paged_attention_decode_8bit (inference only; the front-end rejects autograd inputs)."""
+
+    return _native.extension().paged_attention_decode_8bit(*arguments)

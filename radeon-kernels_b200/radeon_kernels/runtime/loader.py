@@ -85,6 +85,11 @@ class PrecompiledArtifactLoader:
     def root(self) -> Path:
         return self._root
 
+    @property
+    def modules(self) -> tuple[ModuleType, ...]:
+        with self._lock:
+            return tuple(self._modules.values())
+
     def resolve_and_verify(self, artifact: ArtifactSpec) -> Path:
         path = (self._root / artifact.artifact).resolve()
         if not path.is_relative_to(self._root):

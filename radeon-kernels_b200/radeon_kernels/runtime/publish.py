@@ -46,6 +46,10 @@ ENTRYPOINTS = {
     ("gemm_swiglu", "1.0"): ("gemm_swiglu", "rk-sm100a-gemm_swiglu"),
     ("paged_attention_decode", "1.0"): ("paged_attention_decode", "rk-sm100a-paged_attention_decode"),
     ("sdpa", "1.0"): ("sdpa", "rk-sm100a-sdpa"),
+    ("rotary_embedding", "1.0"): ("rotary_embedding", "rk-sm100a-rotary_embedding"),
+    ("paged_slots", "1.0"): ("paged_slots", "rk-sm100a-paged_slots"),
+    ("paged_cache_append_8bit", "1.0"): ("paged_cache_append_8bit", "rk-sm100a-paged_cache_append_8bit"),
+    ("paged_attention_decode_8bit", "1.0"): ("paged_attention_decode_8bit", "rk-sm100a-paged_attention_decode_8bit"),
 }
 
 
