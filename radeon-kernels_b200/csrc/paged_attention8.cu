@@ -49,24 +49,44 @@ namespace pa8 {
 
 constexpr int WARPS = 4;
 constexpr int THREADS = WARPS * 32;
-constexpr int TILE = 16;             // positions of a warp's tile
-constexpr int UNIT = WARPS * TILE;   // positions of a unit
 constexpr int STAGES = 3;
 constexpr int MAX_CTAS_PER_SM = 4;   // sizes the workspace
+constexpr int RANGE_COST = 2;        // what starting and ending a range costs, in units
 constexpr float SLACK = 8.0f;        // a running maximum is raised when it is passed by 2^SLACK
+constexpr float NONE = -3.402823466e38f;  // a maximum before any score: finite, so that -inf - NONE = -inf
 
-// Shared-memory layout.  A row of K or V is D bytes; the pads make the 128-bit (V at D 64:
-// 64-bit) reads of the MMA operands free of bank conflicts.
+// Positions of a unit, which is one tile of a warp.
+__host__ __device__ constexpr int unit_of(int head_dim) { return head_dim == 256 ? 16 : 32; }
+
+// Shared memory of a tile.  The 16-byte chunks of a row are exchanged by its number (chunk ^
+// row % 8), so that the 128-bit reads of the MMA operands touch every bank once; at D 64,
+// where 64-bit reads of V pair with 64-byte rows, V's rows are padded instead.
 template <int D>
 struct Layout {
-  static constexpr int K_STRIDE = D == 64 ? 64 : D + 16;
-  static constexpr int V_STRIDE = D + 16;
-  static constexpr int K_BYTES = TILE * K_STRIDE;
-  static constexpr int V_BYTES = TILE * V_STRIDE;
-  static constexpr int SCALES = K_BYTES + V_BYTES;       // 16 of K, 16 of V
-  static constexpr int MASK = SCALES + 2 * TILE * 4;     // which rows hold a position
+  static constexpr int TILE = unit_of(D);
+  static constexpr int V_STRIDE = D == 64 ? 80 : D;
+  static constexpr int K_BYTES = TILE * D;
+  static constexpr int SCALES = K_BYTES + TILE * V_STRIDE;  // of K, then of V
+  static constexpr int MASK = SCALES + 2 * TILE * 4;        // which rows hold a position
   static constexpr int STAGE = MASK + 16;
   static constexpr int RING = WARPS * STAGES * STAGE;
+  static __device__ __forceinline__ int k_at(int row, int chunk) {
+    return row * D + (D == 64 ? chunk : chunk ^ (row & 7)) * 16;
+  }
+  static __device__ __forceinline__ int v_at(int row, int chunk) {
+    return K_BYTES + row * V_STRIDE + (D == 64 ? chunk : chunk ^ (row & 7)) * 16;
+  }
+};
+
+// A part in the workspace: per head the unnormalised sum, then m, mo and l.
+__host__ __device__ constexpr int part_stride(int head_dim) { return head_dim + 4; }
+
+// What a warp leaves in the workspace about the range that it begins and others end.
+struct Shared {
+  int row;    // first row of the output
+  int heads;  // rows; 0: no such range
+  int last;   // the warp that ends it
+  int slot;   // which of the first warp's two parts; the others' is part 0
 };
 
 struct Params {
@@ -78,40 +98,48 @@ struct Params {
   const void* tables;
   const void* lens;
   void* out;
-  float* part;  // [CTA][2][heads of a tile][D + 3 (rounded up)]: see part_floats
+  float* part;     // [warp][2][heads of a tile][part_stride]
+  Shared* shared;  // [warp]
   int batch, hq, hkv, group, head_groups, tile_heads;
   int num_blocks, block_size, block_shift, max_blocks;
   int index_bits, bf16;
   float scale_log2;
 };
 
-__host__ __device__ constexpr int part_stride(int head_dim) { return head_dim + 4; }  // sum, then m, mo, l
-
-__device__ __forceinline__ int64_t index_at(const void* p, int bits, int64_t i) {
-  return bits == 32 ? static_cast<int64_t>(__ldg(static_cast<const int32_t*>(p) + i))
-                    : static_cast<int64_t>(__ldg(static_cast<const long long*>(p) + i));
+// An index as loaded: nothing waits for the load until value_of.
+struct Raw {
+  uint32_t lo, hi;
+};
+__device__ __forceinline__ Raw load_raw(const void* p, int bits, int64_t i) {
+  Raw r{0, 0};
+  if (bits == 32) {
+    r.lo = __ldg(static_cast<const uint32_t*>(p) + i);
+  } else {
+    const uint2 v = __ldg(static_cast<const uint2*>(p) + i);
+    r.lo = v.x;
+    r.hi = v.y;
+  }
+  return r;
+}
+__device__ __forceinline__ int64_t value_of(Raw r, int bits) {
+  return bits == 32 ? static_cast<int64_t>(static_cast<int32_t>(r.lo))
+                    : static_cast<int64_t>(static_cast<uint64_t>(r.hi) << 32 | r.lo);
 }
 
-__device__ __forceinline__ int context_of(const Params& p, int b) {
-  const int64_t n = index_at(p.lens, p.index_bits, b);
+__device__ __forceinline__ int context_of(const Params& p, Raw raw) {
+  const int64_t n = value_of(raw, p.index_bits);
   const int64_t room = static_cast<int64_t>(p.max_blocks) * p.block_size;  // below 2^31
   return static_cast<int>(n < 0 ? 0 : (n > room ? room : n));
 }
 
-// Units of one (sequence, head tile); an empty sequence has one, which writes its NaN.
-__device__ __forceinline__ int units_of(int context) { return context <= UNIT ? 1 : (context + UNIT - 1) / UNIT; }
+__device__ __forceinline__ int context_of(const Params& p, int b) {
+  return context_of(p, load_raw(p.lens, p.index_bits, b));
+}
 
-// Sum of v over the CTA, in every thread.
-__device__ __forceinline__ int64_t cta_sum(int64_t v, int64_t* scratch) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-  __syncthreads();
-  int64_t total = 0;
-#pragma unroll
-  for (int w = 0; w < WARPS; ++w) total += scratch[w];
-  return total;
+// Units of one (sequence, head tile); an empty sequence has one, which writes its NaN.
+template <int D>
+__device__ __forceinline__ int units_of(int context) {
+  return context <= unit_of(D) ? 1 : (context + unit_of(D) - 1) / unit_of(D);
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
@@ -126,34 +154,14 @@ __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-  uint4 r;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a) : "memory");
-  return r;
+template <typename T>
+__device__ __forceinline__ T at_smem(const uint8_t* smem, int offset) {
+  return *reinterpret_cast<const T*>(smem + offset);
 }
-__device__ __forceinline__ uint2 lds64(uint32_t a) {
-  uint2 r;
-  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(a) : "memory");
-  return r;
-}
-__device__ __forceinline__ float lds_f32(uint32_t a) {
-  float r;
-  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(r) : "r"(a) : "memory");
-  return r;
-}
-__device__ __forceinline__ uint32_t lds_u32(uint32_t a) {
-  uint32_t r;
-  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r) : "r"(a) : "memory");
-  return r;
-}
-__device__ __forceinline__ void sts_u32(uint32_t a, uint32_t v) {
-  asm volatile("st.shared.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
-}
-
 // D[16 x 8] += A[16 x 16] B[16 x 8], f16 operands, fp32 accumulators.
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -161,7 +169,7 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
 // Transposes an 8 x 8 matrix of 16-bit values held across the warp.
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
 __device__ __forceinline__ float lg2_approx(float x) {
@@ -176,163 +184,262 @@ __device__ __forceinline__ int k_chunk(int c, int i) {
   return D == 64 ? c : 2 * c + (i & 1) + 8 * (i >> 1);
 }
 
-// Which dimension an accumulator stands for: MMA tile mt, lane row g, half e.
-template <int D>
-__device__ __forceinline__ int o_dim(int mt, int g, int e) {
-  return D == 64 ? 8 * g + 2 * mt + e : (mt >> 3) * 128 + 16 * g + 2 * (mt & 7) + e;
-}
-
-// A walk over units: sequence b, head tile h, unit c of its `units`.
+// A place in the row of all units: sequence b, head tile h, unit c of its `units`; `left` units
+// of this warp's share from here on.  Every range is followed by RANGE_COST places that hold
+// no unit, so that shares with many short ranges hold fewer units.  The next sequence's
+// length is loaded a sequence ahead.
 struct Walk {
-  int b, h, c, units, context;
+  int b, h, c, units, left, context;
+  Raw next;
 };
 
-__device__ __forceinline__ void walk_on(const Params& p, Walk& w, int tiles) {
-  if (++w.c < w.units) return;
+// To the first unit of the next (sequence, head tile).  Past the last sequence the walk holds
+// some valid length and is not used (left <= 0).
+template <int D>
+__device__ __forceinline__ void next_range(const Params& p, Walk& w, int tiles) {
+  w.left -= w.units + RANGE_COST - w.c;
   w.c = 0;
   if (++w.h < tiles) return;
   w.h = 0;
-  if (++w.b < p.batch) {
-    w.context = context_of(p, w.b);
-    w.units = units_of(w.context);
+  ++w.b;
+  w.context = context_of(p, w.next);
+  w.units = units_of<D>(w.context);
+  w.next = load_raw(p.lens, p.index_bits, min(w.b + 1, p.batch - 1));
+}
+
+template <int D>
+__device__ __forceinline__ void next_unit(const Params& p, Walk& w, int tiles) {
+  ++w.c;
+  --w.left;
+  if (w.c == w.units) next_range<D>(p, w, tiles);
+}
+
+// N (a multiple of 4) neighbouring elements of an output row times f.
+template <int N>
+__device__ __forceinline__ void write_out(const Params& p, int64_t element, const float* v, float f) {
+  uint32_t w[N / 2];
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i)
+    w[i] = p.bf16 ? Pack2<__nv_bfloat16>::from_floats(v[2 * i] * f, v[2 * i + 1] * f)
+                  : Pack2<__half>::from_floats(v[2 * i] * f, v[2 * i + 1] * f);
+  uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + element);
+  if (N % 8 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 8; ++i)
+      reinterpret_cast<uint4*>(out)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) reinterpret_cast<uint2*>(out)[i] = make_uint2(w[2 * i], w[2 * i + 1]);
   }
 }
 
-// The CTA that holds unit u when CTA w holds [floor(w * total / ctas), ...).
-__device__ __forceinline__ int64_t owner_of(int64_t u, int64_t total, int64_t ctas) {
-  return ((u + 1) * ctas - 1) / total;
+// What brings the sums to the output: the weights' sum, and from the one maximum to the
+// other.  Without a position it is 1 / 0, and the sums 0.
+__device__ __forceinline__ float last_factor(float m, float mo, float l) { return ex2_approx(mo - m) / l; }
+
+// First place of warp w's share.  The division is 32 bits wide where it can be.
+__device__ __forceinline__ int64_t share_of(uint32_t w, int64_t total, int64_t warps) {
+  const uint64_t product = static_cast<uint64_t>(w) * static_cast<uint64_t>(total);
+  if (product >> 32 == 0) return static_cast<uint32_t>(product) / static_cast<uint32_t>(warps);
+  return static_cast<int64_t>(product / static_cast<uint64_t>(warps));
+}
+
+// The warp whose share holds place u: the largest w with floor(w * total / warps) <= u.
+__device__ __forceinline__ int owner_of(int64_t u, int64_t total, int64_t warps) {
+  return static_cast<int>(((u + 1) * warps - 1) / total);
 }
 
 template <typename C, int D, int NT>
-__global__ void __launch_bounds__(THREADS) paged_attention8_kernel(Params p, KernelCtl ctl) {
+__global__ void __launch_bounds__(THREADS, 2) paged_attention8_kernel(Params p, KernelCtl ctl) {
   using L = Layout<D>;
+  constexpr int TILE = L::TILE, SUB = TILE / 16;  // MMA tiles of 16 positions
   constexpr int KC = D / 64;   // 16-byte chunks of a K row per lane
   constexpr int MT = D / 16;   // MMA tiles of 16 dimensions
   constexpr int HEADS = 8 * NT;
-  constexpr int O_STRIDE = D + 4;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ int64_t s_scratch[WARPS];
-  __shared__ int s_at[3];
-  __shared__ float s_stats[WARPS][HEADS][3];
-  float* s_out = reinterpret_cast<float*>(smem + L::RING);  // [warp][head][O_STRIDE]
 
   pdl_begin();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, c4 = lane & 3;
   const int tiles = p.hkv * p.head_groups;
+  const int me = static_cast<int>(blockIdx.x) * WARPS + warp;
+  Shared shared{0, 0, 0, 0};
 
-  // ---- this CTA's units
-  int64_t total = 0;
-  for (int base = 0; base < p.batch; base += THREADS) {
-    const int b = base + threadIdx.x;
-    total += cta_sum(b < p.batch ? units_of(context_of(p, b)) : 0, s_scratch);
-  }
-  total *= tiles;
-  const int64_t ctas = min(static_cast<int64_t>(gridDim.x), total);  // each has a unit at least
-  if (blockIdx.x >= ctas) return;
-  const int64_t u0 = blockIdx.x * total / ctas, u1 = (blockIdx.x + 1) * total / ctas;
+  // ---- this warp's share, found 128 sequences at a time (four neighbours to a lane, so that
+  // the loads of a round are in flight together).
+  Walk run{};
+  int64_t place0, total = 0, warps;  // of this warp's range: the place of its first unit
   {
-    // The sequence that holds unit u0: sums over 32 sequences at a time, by every warp alike.
-    int64_t before = 0;  // units (of one head tile) of earlier sequences
-    const int64_t want = u0;
-    for (int base = 0; base < p.batch; base += 32) {
-      const int b = base + lane;
-      const int mine = b < p.batch ? units_of(context_of(p, b)) : 0;
+    constexpr int ROUND = 128;
+    int unit[4];
+    auto load_round = [&](int base) -> int {  // the units of a lane's four sequences
+      Raw raw[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) raw[i] = load_raw(p.lens, p.index_bits, min(base + 4 * lane + i, p.batch - 1));
+      int sum = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        unit[i] = base + 4 * lane + i < p.batch ? units_of<D>(context_of(p, raw[i])) + RANGE_COST : 0;
+        sum += unit[i];
+      }
+      return sum;
+    };
+    int mine = 0;
+    for (int base = 0; base < p.batch; base += ROUND) {
+      mine = load_round(base);
+      int64_t sum = mine;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      total += sum;
+    }
+    total *= tiles;
+    warps = min(static_cast<int64_t>(gridDim.x) * WARPS, total);
+    if (me >= warps) {
+      if (lane == 0) p.shared[me] = shared;
+      return;
+    }
+    const int64_t u0 = share_of(me, total, warps);
+    run.left = static_cast<int>(share_of(me + 1, total, warps) - u0);
+    // The sequence that holds place u0.
+    int64_t before = 0;  // places, of one head tile, of earlier rounds
+    for (int base = 0; base < p.batch; base += ROUND) {
+      if (p.batch > ROUND) mine = load_round(base);
       int64_t upto = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += x;
       }
-      const uint32_t past = __ballot_sync(0xffffffffu, (before + upto) * tiles > want);
+      const uint32_t past = __ballot_sync(0xffffffffu, (before + upto) * tiles > u0);
       if (past != 0) {
         const int at = __ffs(past) - 1;
-        const int64_t prior = __shfl_sync(0xffffffffu, before + upto - mine, at);
-        const int units = __shfl_sync(0xffffffffu, mine, at);
-        if (threadIdx.x == 0) {
-          const int64_t in = want - prior * tiles;
-          s_at[0] = base + at;
-          s_at[1] = static_cast<int>(in / units);
-          s_at[2] = static_cast<int>(in % units);
+        int64_t prior = __shfl_sync(0xffffffffu, before + upto - mine, at);
+        int b = base + 4 * at, units = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int n = __shfl_sync(0xffffffffu, unit[i], at);
+          if (units == 0) {
+            if ((prior + n) * tiles > u0) {
+              units = n;
+            } else {
+              prior += n;
+              ++b;
+            }
+          }
         }
+        const uint32_t in = static_cast<uint32_t>(u0 - prior * tiles);  // below tiles * units, which the host checked
+        run.b = b;
+        run.h = static_cast<int>(in / static_cast<uint32_t>(units));
+        run.c = static_cast<int>(in - static_cast<uint32_t>(run.h) * units);
+        run.units = units - RANGE_COST;
+        place0 = u0 - run.c;
         break;
       }
       before += __shfl_sync(0xffffffffu, upto, 31);
     }
   }
-  __syncthreads();
-  Walk run{s_at[0], s_at[1], s_at[2], 0, context_of(p, s_at[0])};
-  run.units = units_of(run.context);
-  Walk load = run;
+  run.context = context_of(p, run.b);
+  run.next = load_raw(p.lens, p.index_bits, min(run.b + 1, p.batch - 1));
 
-  const uint32_t ring = smem_u32(smem) + warp * (STAGES * L::STAGE);
-  const int64_t slot_bytes = static_cast<int64_t>(p.hkv) * D;
-
-  // Block of the row that this lane (lane % 16) looks up for the tile of `w`; -1: no position.
-  auto look_up = [&](const Walk& w) -> int {
-    const int t = w.c * UNIT + warp * TILE + (lane & 15);
-    if (t >= w.context) return -1;
-    const int j = p.block_shift >= 0 ? t >> p.block_shift : t / p.block_size;
-    const int64_t blk = index_at(p.tables, p.index_bits, static_cast<int64_t>(w.b) * p.max_blocks + j);
-    if (blk < 0 || blk >= p.num_blocks) {
-      if (lane < 16) atomicOr(ctl.status, RK_DEV_ERR_BAD_INDEX);
-      return -1;
-    }
-    return static_cast<int>(blk);
-  };
-  auto issue = [&](const Walk& w, int blk, int stage) {
-    const uint32_t base = ring + stage * L::STAGE;
-    const int kvh = w.h / p.head_groups;
-    const int t = w.c * UNIT + warp * TILE + (lane & 15);
-    const int off = p.block_shift >= 0 ? t & (p.block_size - 1) : t % p.block_size;
-    const int64_t slot = blk < 0 ? 0 : static_cast<int64_t>(blk) * p.block_size + off;
-    const uint32_t mask = __ballot_sync(0xffffffffu, blk >= 0) & 0xFFFFu;
-    if (lane == 0) sts_u32(base + L::MASK, mask);
-    const int64_t sc = static_cast<int64_t>(blk < 0 ? 0 : blk) * p.hkv + kvh;
-    cp_async4(base + L::SCALES + lane * 4, (lane < 16 ? p.ks : p.vs) + sc, blk < 0 ? 0u : 4u);
-    constexpr int CHUNKS = D / 16, PER = 32 / CHUNKS;  // chunks of a row, rows side by side
-    const int r0 = lane / CHUNKS, ch = lane - r0 * CHUNKS;
-#pragma unroll
-    for (int i = 0; i < TILE / PER; ++i) {
-      const int r = r0 + i * PER;
-      const int64_t row_slot = __shfl_sync(0xffffffffu, slot, r);
-      const uint32_t bytes = (mask >> r) & 1u ? 16u : 0u;
-      const int64_t from = row_slot * slot_bytes + kvh * D + ch * 16;
-      cp_async16(base + r * L::K_STRIDE + ch * 16, p.k + from, bytes);
-      cp_async16(base + L::K_BYTES + r * L::V_STRIDE + ch * 16, p.v + from, bytes);
-    }
-  };
-
-  int64_t loaded = u0;
-  int blk = look_up(load);
-#pragma unroll
-  for (int s = 0; s < STAGES - 1; ++s) {
-    if (loaded < u1) {
-      issue(load, blk, s);
-      walk_on(p, load, tiles);
-      if (++loaded < u1) blk = look_up(load);
-    }
-    cp_async_commit();
+  if (run.c >= run.units) {  // the share starts behind a range
+    place0 += run.units + RANGE_COST;
+    next_range<D>(p, run, tiles);
   }
 
-  uint32_t qf[NT][4 * KC][2];
-  float factor[NT][2];
-  float o[NT][MT][4];
-  float m[NT][2], mo[NT][2], l[NT][2];
-  int64_t range0 = u0;  // first unit of the current range that this CTA holds
-  bool fresh = true;
-  int stage = 0;
+  // ---- this warp's ring; `load` runs ahead of `run`.
+  Walk load = run;
+  const int ring = warp * (STAGES * L::STAGE);
+  const uint32_t smem_base = smem_u32(smem);
+  const int64_t slot_bytes = static_cast<int64_t>(p.hkv) * D;
+  constexpr int CHUNKS = D / 16, PER = 32 / CHUNKS;  // chunks of a row, rows side by side
+  const int r0 = lane / CHUNKS, ch = lane - r0 * CHUNKS;
+  const int64_t lane_bytes = r0 * slot_bytes + ch * 16, step_bytes = PER * slot_bytes, to_v = p.v - p.k;
 
-  for (int64_t u = u0; u < u1; ++u) {
-    const int kvh = run.h / p.head_groups, hg = run.h - kvh * p.head_groups;
+  // The table entry of the row that this lane (lane % TILE) looks up for the tile of `w`.
+  auto look_up = [&](const Walk& w) -> Raw {
+    const int t = w.c * TILE + (lane & (TILE - 1));
+    const int j = p.block_shift >= 0 ? t >> p.block_shift : t / p.block_size;
+    return t < w.context ? load_raw(p.tables, p.index_bits, static_cast<int64_t>(w.b) * p.max_blocks + j) : Raw{0, 0};
+  };
+  auto issue = [&](const Walk& w, Raw entry, int stage) {
+    const int offset = ring + stage * L::STAGE;
+    const uint32_t base = smem_base + offset;
+    const int kvh = p.head_groups == 1 ? w.h : w.h / p.head_groups;
+    const int t = w.c * TILE + (lane & (TILE - 1));
+    const int off = p.block_shift >= 0 ? t & (p.block_size - 1) : t % p.block_size;
+    const int64_t value = value_of(entry, p.index_bits);
+    const bool in = t < w.context, found = value >= 0 && value < p.num_blocks;
+    if (in && !found && lane < TILE) atomicOr(ctl.status, RK_DEV_ERR_BAD_INDEX);
+    const int blk = in && found ? static_cast<int>(value) : -1;
+    const uint32_t mask = __ballot_sync(0xffffffffu, blk >= 0);
+    if (lane == 0)
+      *reinterpret_cast<uint32_t*>(smem + offset + L::MASK) = TILE == 32 ? mask : mask & 0xFFFFu;
+    const int64_t scale_at = static_cast<int64_t>(blk < 0 ? 0 : blk) * p.hkv + kvh;
+    const uint32_t scale_bytes = blk < 0 ? 0u : 4u;
+    if (TILE == 32) {
+      cp_async4(base + L::SCALES + lane * 4, p.ks + scale_at, scale_bytes);
+      cp_async4(base + L::SCALES + 128 + lane * 4, p.vs + scale_at, scale_bytes);
+    } else {
+      cp_async4(base + L::SCALES + lane * 4, (lane < 16 ? p.ks : p.vs) + scale_at, scale_bytes);
+    }
+    // Bytes from the start of a cache to this lane's row.
+    const int64_t row_bytes = (static_cast<int64_t>(blk < 0 ? 0 : blk) * p.block_size + (blk < 0 ? 0 : off)) * slot_bytes;
+    const int head_bytes = kvh * D;
+    if (mask == 0xFFFFFFFFu && p.block_size % 16 == 0) {
+      // Full tiles whose 16 positions lie side by side.
+#pragma unroll
+      for (int sub = 0; sub < SUB; ++sub) {
+        const uint8_t* from = p.k + __shfl_sync(0xffffffffu, row_bytes, 16 * sub) + head_bytes + lane_bytes;
+#pragma unroll
+        for (int i = 0; i < 16 / PER; ++i) {
+          const int r = 16 * sub + i * PER + r0;
+          cp_async16(base + L::k_at(r, ch), from, 16);
+          cp_async16(base + L::v_at(r, ch), from + to_v, 16);
+          from += step_bytes;
+        }
+      }
+    } else {
+#pragma unroll 4
+      for (int i = 0; i < TILE / PER; ++i) {
+        const int r = i * PER + r0;
+        const uint8_t* from = p.k + __shfl_sync(0xffffffffu, row_bytes, r) + head_bytes + ch * 16;
+        const uint32_t bytes = (mask >> r) & 1u ? 16u : 0u;  // rows without a position: zeros
+        cp_async16(base + L::k_at(r, ch), from, bytes);
+        cp_async16(base + L::v_at(r, ch), from + to_v, bytes);
+      }
+    }
+  };
+
+  Raw entry{0, 0};
+  if (load.left > 0) entry = look_up(load);
+  auto load_next = [&](int stage) {  // always a group, so that the groups count the tiles
+    if (load.left > 0) {
+      issue(load, entry, stage);
+      next_unit<D>(p, load, tiles);
+      if (load.left > 0) entry = look_up(load);
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < STAGES; ++s) load_next(s);
+
+  int stage = 0;
+  int slot = 0;  // of this warp's next part
+  while (run.left > 0) {
+    const int length = min(run.units - run.c, run.left);  // units of the range that this warp holds
+    const int kvh = p.head_groups == 1 ? run.h : run.h / p.head_groups, hg = run.h - kvh * p.head_groups;
     const int head0 = kvh * p.group + hg * HEADS;
     const int nheads = min(HEADS, p.group - hg * HEADS);
-    if (fresh) {
+    const int64_t row0 = static_cast<int64_t>(run.b) * p.hq + head0;
+    uint32_t qf[NT][4 * KC][2];
+      float factor[NT][2];
+      float o[NT][MT][4];
+      float m[NT][2], mo[NT][2], l[NT][2];
       // Queries of the head tile: lane (g, c4) holds head g's dimensions of its K chunks.
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const bool live = nt * 8 + g < nheads;
-        const int64_t row = (static_cast<int64_t>(run.b) * p.hq + head0 + nt * 8 + g) * D;
+        const int64_t row = (row0 + nt * 8 + g) * D;
         float f[4 * KC][4];
         float amax = 0.f;
 #pragma unroll
@@ -365,7 +472,7 @@ __global__ void __launch_bounds__(THREADS) paged_attention8_kernel(Params p, Ker
         factor[nt][1] = __shfl_sync(0xffffffffu, up, 8 * c4 + 4);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          m[nt][i] = mo[nt][i] = -INFINITY;
+          m[nt][i] = mo[nt][i] = NONE;
           l[nt][i] = 0.f;
         }
 #pragma unroll
@@ -373,261 +480,266 @@ __global__ void __launch_bounds__(THREADS) paged_attention8_kernel(Params p, Ker
 #pragma unroll
           for (int i = 0; i < 4; ++i) o[nt][mt][i] = 0.f;
       }
-      fresh = false;
-    }
 
-    cp_async_wait<STAGES - 2>();
-    __syncwarp();
-    {
-      const int next = stage + STAGES - 1 >= STAGES ? stage - 1 : stage + STAGES - 1;
-      if (loaded < u1) {
-        issue(load, blk, next);
-        walk_on(p, load, tiles);
-        if (++loaded < u1) blk = look_up(load);
-      }
-      cp_async_commit();
-    }
-    const uint32_t base = ring + stage * L::STAGE;
-    stage = stage + 1 == STAGES ? 0 : stage + 1;
-    const uint32_t mask = lds_u32(base + L::MASK);
-    if (mask != 0) {
-      float s[NT][4];
+      for (int step = 0; step < length; ++step) {
+        cp_async_wait<STAGES - 1>();
+        __syncwarp();
+        const uint8_t* tile = smem + ring + stage * L::STAGE;
+        const uint32_t mask = at_smem<uint32_t>(tile, L::MASK);
+        if (mask != 0) {
+          float s[NT][SUB][4], s2[NT][SUB][4];  // two chains of products: half the latency
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[nt][i] = 0.f;
+            for (int t = 0; t < SUB; ++t)
 #pragma unroll
-      for (int i = 0; i < KC; ++i) {
-        const uint32_t at = base + k_chunk<D>(c4, i) * 16;
-        const uint4 ka = lds128(at + g * L::K_STRIDE), kb = lds128(at + (g + 8) * L::K_STRIDE);
-        const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+              for (int i = 0; i < 4; ++i) s[nt][t][i] = s2[nt][t][i] = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          uint32_t a0, a1, a2, a3;
-          C::halves(wa[j], a0, a2);
-          C::halves(wb[j], a1, a3);
+          for (int i = 0; i < KC; ++i) {
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma16816(s[nt], a0, a1, a2, a3, qf[nt][4 * i + j][0], qf[nt][4 * i + j][1]);
-        }
-      }
-      // Rows g and g + 8 of the tile.
-      const float ks0 = lds_f32(base + L::SCALES + g * 4), ks1 = lds_f32(base + L::SCALES + (g + 8) * 4);
-      const float lv0 = lg2_approx(lds_f32(base + L::SCALES + 64 + g * 4));
-      const float lv1 = lg2_approx(lds_f32(base + L::SCALES + 64 + (g + 8) * 4));
-      const bool in0 = (mask >> g) & 1u, in1 = (mask >> (g + 8)) & 1u;
-      bool raise = false;
-      float w[NT][4];
+            for (int t = 0; t < SUB; ++t) {
+              const uint4 ka = at_smem<uint4>(tile, L::k_at(16 * t + g, k_chunk<D>(c4, i)));
+              const uint4 kb = at_smem<uint4>(tile, L::k_at(16 * t + g + 8, k_chunk<D>(c4, i)));
+              const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
+              for (int j = 0; j < 4; ++j) {
+                uint32_t a0, a1, a2, a3;
+                C::halves(wa[j], a0, a2);
+                C::halves(wb[j], a1, a3);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const bool in = i < 2 ? in0 : in1;
-          s[nt][i] = in ? s[nt][i] * ((i < 2 ? ks0 : ks1) * factor[nt][i & 1]) : -INFINITY;
-          w[nt][i] = in ? s[nt][i] + (i < 2 ? lv0 : lv1) : -INFINITY;
-          raise = raise || s[nt][i] > m[nt][i & 1] + SLACK || w[nt][i] > mo[nt][i & 1] + SLACK;
-        }
-      }
-      if (__any_sync(0xffffffffu, raise)) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            float a = fmax3(m[nt][i], s[nt][i], s[nt][i + 2]), b = fmax3(mo[nt][i], w[nt][i], w[nt][i + 2]);
-#pragma unroll
-            for (int x = 4; x < 32; x <<= 1) {
-              a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, x));
-              b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, x));
+                for (int nt = 0; nt < NT; ++nt)
+                  mma16816((j & 1) ? s2[nt][t] : s[nt][t], a0, a1, a2, a3, qf[nt][4 * i + j][0], qf[nt][4 * i + j][1]);
+              }
             }
-            // A maximum of -inf has nothing behind it to scale.
-            const float down_l = m[nt][i] == -INFINITY ? 0.f : ex2_approx(m[nt][i] - a);
-            const float down_o = mo[nt][i] == -INFINITY ? 0.f : ex2_approx(mo[nt][i] - b);
-            m[nt][i] = a;
-            mo[nt][i] = b;
-            l[nt][i] *= down_l;
+          }
+          // Rows g and g + 8 of each 16.
+          bool raise = false;
+          float w[NT][SUB][4];
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-              o[nt][mt][i] *= down_o;
-              o[nt][mt][i + 2] *= down_o;
+          for (int t = 0; t < SUB; ++t) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const int row = 16 * t + 8 * r + g;
+              const float ks = at_smem<float>(tile, L::SCALES + row * 4);
+              const float lv = lg2_approx(at_smem<float>(tile, L::SCALES + (TILE + row) * 4));
+              const bool in = (mask >> row) & 1u;
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                  float& x = s[nt][t][2 * r + i];
+                  x = in ? (x + s2[nt][t][2 * r + i]) * (ks * factor[nt][i]) : -INFINITY;
+                  w[nt][t][2 * r + i] = in ? x + lv : -INFINITY;
+                  raise = raise || x > m[nt][i] + SLACK || w[nt][t][2 * r + i] > mo[nt][i] + SLACK;
+                }
+              }
+            }
+          }
+          if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                float a = m[nt][i], b = mo[nt][i];
+#pragma unroll
+                for (int t = 0; t < SUB; ++t) {
+                  a = fmax3(a, s[nt][t][i], s[nt][t][i + 2]);
+                  b = fmax3(b, w[nt][t][i], w[nt][t][i + 2]);
+                }
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) {
+                  a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, x));
+                  b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, x));
+                }
+                const float down_l = ex2_approx(m[nt][i] - a), down_o = ex2_approx(mo[nt][i] - b);
+                m[nt][i] = a;
+                mo[nt][i] = b;
+                l[nt][i] *= down_l;
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                  o[nt][mt][i] *= down_o;
+                  o[nt][mt][i + 2] *= down_o;
+                }
+              }
+            }
+          }
+          uint32_t pf[NT][SUB][2];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int t = 0; t < SUB; ++t) {
+              float e[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                l[nt][i & 1] += ex2_approx(s[nt][t][i] - m[nt][i & 1]);
+                e[i] = ex2_approx(w[nt][t][i] - mo[nt][i & 1]);
+              }
+              pf[nt][t][0] = transpose8x8(Pack2<__half>::from_floats(e[0], e[1]));
+              pf[nt][t][1] = transpose8x8(Pack2<__half>::from_floats(e[2], e[3]));
+            }
+          }
+          // V^T: a lane's 16 (D 64: 8) bytes of positions 2 c4, 2 c4 + 1, and those + 8, byte by
+          // byte side by side, are two rows of the operand.
+#pragma unroll
+          for (int t = 0; t < SUB; ++t) {
+            const int row = 16 * t + 2 * c4;
+            if (D == 64) {
+              const int at = L::K_BYTES + g * 8;
+              const uint2 va = at_smem<uint2>(tile, at + row * L::V_STRIDE), vb = at_smem<uint2>(tile, at + (row + 1) * L::V_STRIDE);
+              const uint2 vc = at_smem<uint2>(tile, at + (row + 8) * L::V_STRIDE), vd = at_smem<uint2>(tile, at + (row + 9) * L::V_STRIDE);
+              const uint32_t w0[2] = {va.x, va.y}, w1[2] = {vb.x, vb.y}, w2[2] = {vc.x, vc.y}, w3[2] = {vd.x, vd.y};
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                  const uint32_t pick = x == 0 ? 0x5140u : 0x7362u;
+                  uint32_t a0, a1, a2, a3;
+                  C::halves(__byte_perm(w0[j], w1[j], pick), a0, a1);
+                  C::halves(__byte_perm(w2[j], w3[j], pick), a2, a3);
+#pragma unroll
+                  for (int nt = 0; nt < NT; ++nt)
+                    mma16816(o[nt][(2 * j + x) % MT], a0, a1, a2, a3, pf[nt][t][0], pf[nt][t][1]);
+                }
+              }
+            } else {
+#pragma unroll
+              for (int h = 0; h < D / 128; ++h) {
+                const uint4 va = at_smem<uint4>(tile, L::v_at(row, g + 8 * h)), vb = at_smem<uint4>(tile, L::v_at(row + 1, g + 8 * h));
+                const uint4 vc = at_smem<uint4>(tile, L::v_at(row + 8, g + 8 * h)), vd = at_smem<uint4>(tile, L::v_at(row + 9, g + 8 * h));
+                const uint32_t w0[4] = {va.x, va.y, va.z, va.w}, w1[4] = {vb.x, vb.y, vb.z, vb.w};
+                const uint32_t w2[4] = {vc.x, vc.y, vc.z, vc.w}, w3[4] = {vd.x, vd.y, vd.z, vd.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+#pragma unroll
+                  for (int x = 0; x < 2; ++x) {
+                    const uint32_t pick = x == 0 ? 0x5140u : 0x7362u;
+                    uint32_t a0, a1, a2, a3;
+                    C::halves(__byte_perm(w0[j], w1[j], pick), a0, a1);
+                    C::halves(__byte_perm(w2[j], w3[j], pick), a2, a3);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+                      mma16816(o[nt][(8 * h + 2 * j + x) % MT], a0, a1, a2, a3, pf[nt][t][0], pf[nt][t][1]);
+                  }
+                }
+              }
             }
           }
         }
+        __syncwarp();  // the tile is read
+        load_next(stage);
+        stage = stage + 1 == STAGES ? 0 : stage + 1;
       }
-      uint32_t pf[NT][2];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float e[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          // Against a maximum of -inf every weight is 0 (2^-inf), not 2^(inf - inf).
-          const float ms = m[nt][i & 1] == -INFINITY ? 0.f : m[nt][i & 1];
-          const float mw = mo[nt][i & 1] == -INFINITY ? 0.f : mo[nt][i & 1];
-          l[nt][i & 1] += ex2_approx(s[nt][i] - ms);
-          e[i] = ex2_approx(w[nt][i] - mw);
-        }
-        pf[nt][0] = transpose8x8(Pack2<__half>::from_floats(e[0], e[1]));
-        pf[nt][1] = transpose8x8(Pack2<__half>::from_floats(e[2], e[3]));
-      }
-      // V^T: a lane's 16 (D 64: 8) bytes of positions 2 c4, 2 c4 + 1, and those + 8, byte by
-      // byte side by side, are two rows of the operand.
-      const uint32_t vb = base + L::K_BYTES;
-      if (D == 64) {
-        const uint2 va = lds64(vb + (2 * c4) * L::V_STRIDE + g * 8), vc = lds64(vb + (2 * c4 + 1) * L::V_STRIDE + g * 8);
-        const uint2 vd = lds64(vb + (2 * c4 + 8) * L::V_STRIDE + g * 8), ve = lds64(vb + (2 * c4 + 9) * L::V_STRIDE + g * 8);
-        const uint32_t w0[2] = {va.x, va.y}, w1[2] = {vc.x, vc.y}, w2[2] = {vd.x, vd.y}, w3[2] = {ve.x, ve.y};
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const uint32_t pick = x == 0 ? 0x5140u : 0x7362u;
-            uint32_t a0, a1, a2, a3;
-            C::halves(__byte_perm(w0[j], w1[j], pick), a0, a1);
-            C::halves(__byte_perm(w2[j], w3[j], pick), a2, a3);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma16816(o[nt][2 * j + x], a0, a1, a2, a3, pf[nt][0], pf[nt][1]);
-          }
-        }
-      } else {
-#pragma unroll
-        for (int h = 0; h < D / 128; ++h) {
-          const uint32_t at = vb + g * 16 + h * 128;
-          const uint4 va = lds128(at + (2 * c4) * L::V_STRIDE), vc = lds128(at + (2 * c4 + 1) * L::V_STRIDE);
-          const uint4 vd = lds128(at + (2 * c4 + 8) * L::V_STRIDE), ve = lds128(at + (2 * c4 + 9) * L::V_STRIDE);
-          const uint32_t w0[4] = {va.x, va.y, va.z, va.w}, w1[4] = {vc.x, vc.y, vc.z, vc.w};
-          const uint32_t w2[4] = {vd.x, vd.y, vd.z, vd.w}, w3[4] = {ve.x, ve.y, ve.z, ve.w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              const uint32_t pick = x == 0 ? 0x5140u : 0x7362u;
-              uint32_t a0, a1, a2, a3;
-              C::halves(__byte_perm(w0[j], w1[j], pick), a0, a1);
-              C::halves(__byte_perm(w2[j], w3[j], pick), a2, a3);
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-                mma16816(o[nt][8 * h + 2 * j + x], a0, a1, a2, a3, pf[nt][0], pf[nt][1]);
-            }
-          }
-        }
-      }
-    }
-    __syncwarp();  // the stage is read before it is filled again
 
-    if (run.c + 1 == run.units || u + 1 == u1) {
-      // End of a range: join the warps.  Accumulator (mt, g, e) of a head lies at
-      // [16 mt + 2 g + e], which keeps the stores free of bank conflicts.
+      // The end of a range.  A lane holds 16 (D 64: 8) neighbouring dimensions of two heads.
+      const bool whole = length == run.units;
+      if (!whole && run.c == 0) {
+        shared.row = static_cast<int>(row0);
+        shared.heads = nheads;
+        shared.last = owner_of(place0 + run.units - 1, total, warps);
+        shared.slot = slot;
+      }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) l[nt][i] += __shfl_xor_sync(0xffffffffu, l[nt][i], x);
-          if (g == 0) {
-            float* st = s_stats[warp][nt * 8 + 2 * c4 + i];
-            st[0] = m[nt][i];
-            st[1] = mo[nt][i];
-            st[2] = l[nt][i];
-          }
+          const int h = nt * 8 + 2 * c4 + i;
+          constexpr int N = D == 64 ? 8 : 16;
+          if (h < nheads) {
+            float* part = p.part + ((static_cast<int64_t>(me) * 2 + slot) * HEADS + h) * part_stride(D);
+            const float f = last_factor(m[nt][i], mo[nt][i], l[nt][i]);
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
-            *reinterpret_cast<float2*>(s_out + (warp * HEADS + nt * 8 + 2 * c4 + i) * O_STRIDE + 16 * mt + 2 * g) =
-                make_float2(o[nt][mt][i], o[nt][mt][i + 2]);
-        }
-      __syncthreads();
-      const bool whole = run.c + 1 == run.units && u + 1 - range0 == run.units;
-      const int slot = range0 == u0 ? 0 : 1;
-      for (int idx = threadIdx.x; idx < nheads * (D / 2); idx += THREADS) {
-        const int h = idx / (D / 2), at = (idx - h * (D / 2)) * 2;
-        float am = -INFINITY, ao = -INFINITY;
+            for (int k = 0; k < MT * 2 / N; ++k) {
+              float v[N];
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
-          am = fmaxf(am, s_stats[w][h][0]);
-          ao = fmaxf(ao, s_stats[w][h][1]);
-        }
-        float sum = 0.f, x = 0.f, y = 0.f;
+              for (int j = 0; j < N / 2; ++j) {
+                v[2 * j] = o[nt][k * (N / 2) + j][i];
+                v[2 * j + 1] = o[nt][k * (N / 2) + j][i + 2];
+              }
+              const int d = N * g + 128 * k;
+              if (whole) {
+                write_out<N>(p, (row0 + h) * D + d, v, f);
+              } else {
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
-          const float wm = s_stats[w][h][0], wo = s_stats[w][h][1];
-          // A warp without a maximum has sums of 0, or NaN from NaN scores, which stay.
-          sum += s_stats[w][h][2] * (wm == -INFINITY ? 1.f : ex2_approx(wm - am));
-          const float f = wo == -INFINITY ? 1.f : ex2_approx(wo - ao);
-          const float2 v = *reinterpret_cast<const float2*>(s_out + (w * HEADS + h) * O_STRIDE + at);
-          x = fmaf(v.x, f, x);
-          y = fmaf(v.y, f, y);
-        }
-        if (whole) {
-          const float f = (ao == -INFINITY || am == -INFINITY ? 1.f : ex2_approx(ao - am)) / sum;
-          const int d = o_dim<D>(at >> 4, (at & 15) >> 1, 0);
-          const int64_t row = (static_cast<int64_t>(run.b) * p.hq + head0 + h) * D + d;
-          static_cast<uint32_t*>(p.out)[row >> 1] =
-              p.bf16 ? Pack2<__nv_bfloat16>::from_floats(x * f, y * f) : Pack2<__half>::from_floats(x * f, y * f);
-        } else {
-          float* part = p.part + ((static_cast<int64_t>(blockIdx.x) * 2 + slot) * HEADS + h) * part_stride(D);
-          *reinterpret_cast<float2*>(part + at) = make_float2(x, y);
-          if (at == 0) {
-            part[D] = am;
-            part[D + 1] = ao;
-            part[D + 2] = sum;
+                for (int j = 0; j < N / 4; ++j)
+                  reinterpret_cast<float4*>(part + d)[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+              }
+            }
+            if (!whole && g == 0) *reinterpret_cast<float4*>(part + D) = make_float4(m[nt][i], mo[nt][i], l[nt][i], 0.f);
           }
         }
-      }
-      __syncthreads();
-      range0 = u + 1;
-      fresh = true;
-    }
-    walk_on(p, run, tiles);
+      slot = 1;
+    place0 += run.units + RANGE_COST;
+    next_range<D>(p, run, tiles);
   }
+  if (lane == 0) p.shared[me] = shared;
 }
 
-// Joins the parts of the ranges that several CTAs shared.  One CTA per (sequence, head tile).
+// Joins the parts of the ranges that several warps of the attention shared.  One CTA for the
+// range that warp blockIdx.x began (most began none), a warp for each head.
+constexpr int JOIN_THREADS = 256;
+
 template <int D>
-__global__ void __launch_bounds__(THREADS) paged_attention8_join_kernel(Params p, int64_t grid) {
-  __shared__ int64_t s_scratch[WARPS];
+__global__ void __launch_bounds__(JOIN_THREADS) paged_attention8_join_kernel(Params p) {
+  constexpr int V = D / 32;                // neighbouring dimensions of a lane
+  constexpr int AHEAD = D == 256 ? 8 : 16;  // parts whose loads are in flight together
   pdl_begin();
-  const int tiles = p.hkv * p.head_groups;
-  const int b = blockIdx.x / tiles, tile = blockIdx.x - b * tiles;
-  int64_t total = 0, before = 0;
-  for (int base = 0; base < p.batch; base += THREADS) {
-    const int i = base + threadIdx.x;
-    const int64_t units = i < p.batch ? units_of(context_of(p, i)) : 0;
-    total += units;
-    if (i < b) before += units;
-  }
-  total = cta_sum(total, s_scratch) * tiles;
-  before = cta_sum(before, s_scratch) * tiles;
-  const int64_t ctas = min(grid, total);
-  const int64_t units = units_of(context_of(p, b));
-  const int64_t first = before + tile * units;
-  const int64_t w0 = owner_of(first, total, ctas), w1 = owner_of(first + units - 1, total, ctas);
-  if (w0 == w1) return;  // written by its one CTA
-  const int slot0 = w0 * total / ctas == first ? 0 : 1;
-  const int kvh = tile / p.head_groups, hg = tile - kvh * p.head_groups;
-  const int nheads = min(p.tile_heads, p.group - hg * p.tile_heads);
-  const int64_t head0 = static_cast<int64_t>(b) * p.hq + kvh * p.group + hg * p.tile_heads;
-  const int64_t step = static_cast<int64_t>(2) * p.tile_heads * part_stride(D);  // from CTA to CTA
-  for (int idx = threadIdx.x; idx < nheads * (D / 2); idx += THREADS) {
-    const int h = idx / (D / 2), at = (idx - h * (D / 2)) * 2;
-    const float* head = p.part + w0 * step + (static_cast<int64_t>(slot0) * p.tile_heads + h) * part_stride(D);
-    const float* rest = p.part + (w0 + 1) * step + static_cast<int64_t>(h) * part_stride(D);
-    const int n = static_cast<int>(w1 - w0);
-    float am = head[D], ao = head[D + 1];
-    for (int i = 0; i < n; ++i) {
-      am = fmaxf(am, rest[i * step + D]);
-      ao = fmaxf(ao, rest[i * step + D + 1]);
+  const int4 raw = __ldg(reinterpret_cast<const int4*>(p.shared) + blockIdx.x);
+  const Shared shared{raw.x, raw.y, raw.z, raw.w};
+  const int lane = threadIdx.x & 31;
+  const int64_t step = static_cast<int64_t>(2) * p.tile_heads * part_stride(D);  // from warp to warp
+  const int n = shared.last - static_cast<int>(blockIdx.x) + 1;
+  for (int h = threadIdx.x >> 5; h < shared.heads; h += JOIN_THREADS / 32) {
+    const float* part0 = p.part + blockIdx.x * step + static_cast<int64_t>(h) * part_stride(D);
+    const int64_t shift0 = static_cast<int64_t>(shared.slot) * p.tile_heads * part_stride(D);
+    float m = NONE, mo = NONE, l = 0.f, v[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = 0.f;
+    for (int i0 = 0; i0 < n; i0 += AHEAD) {
+      float x[AHEAD][V];
+      float4 st[AHEAD];
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        const float* part = part0 + min(i0 + i, n - 1) * step + (i0 + i == 0 ? shift0 : 0);
+#pragma unroll
+        for (int j = 0; j < V; j += 2) {
+          const float2 y = *reinterpret_cast<const float2*>(part + V * lane + j);
+          x[i][j] = y.x;
+          x[i][j + 1] = y.y;
+        }
+        st[i] = *reinterpret_cast<const float4*>(part + D);
+      }
+      float bm = m, bo = mo;
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        bm = fmaxf(bm, st[i].x);  // a part that is loaded twice changes no maximum
+        bo = fmaxf(bo, st[i].y);
+      }
+      l *= ex2_approx(m - bm);
+      const float fo = ex2_approx(mo - bo);
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] *= fo;
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        if (i0 + i < n) {
+          l = fmaf(st[i].z, ex2_approx(st[i].x - bm), l);
+          const float f = ex2_approx(st[i].y - bo);
+#pragma unroll
+          for (int j = 0; j < V; ++j) v[j] = fmaf(x[i][j], f, v[j]);
+        }
+      }
+      m = bm;
+      mo = bo;
     }
-    float sum = 0.f, x = 0.f, y = 0.f;
-    for (int i = -1; i < n; ++i) {
-      const float* part = i < 0 ? head : rest + i * step;
-      const float wm = part[D], wo = part[D + 1];
-      sum += part[D + 2] * (wm == -INFINITY ? 1.f : ex2_approx(wm - am));
-      const float f = wo == -INFINITY ? 1.f : ex2_approx(wo - ao);
-      const float2 v = *reinterpret_cast<const float2*>(part + at);
-      x = fmaf(v.x, f, x);
-      y = fmaf(v.y, f, y);
+    const float f = last_factor(m, mo, l);
+    const int64_t element = (static_cast<int64_t>(shared.row) + h) * D + V * lane;
+    if (V >= 4) {
+      write_out<V < 4 ? 4 : V>(p, element, v, f);
+    } else {
+      static_cast<uint32_t*>(p.out)[element >> 1] = p.bf16 ? Pack2<__nv_bfloat16>::from_floats(v[0] * f, v[1] * f)
+                                                           : Pack2<__half>::from_floats(v[0] * f, v[1] * f);
     }
-    const float f = (ao == -INFINITY || am == -INFINITY ? 1.f : ex2_approx(ao - am)) / sum;
-    const int d = o_dim<D>(at >> 4, (at & 15) >> 1, 0);
-    static_cast<uint32_t*>(p.out)[((head0 + h) * D + d) >> 1] =
-        p.bf16 ? Pack2<__nv_bfloat16>::from_floats(x * f, y * f) : Pack2<__half>::from_floats(x * f, y * f);
   }
 }
 
@@ -646,7 +758,7 @@ Plan plan(int64_t hq, int64_t hkv, int64_t head_dim) {
 
 template <typename C, int D, int NT>
 rk_status launch(const Params& p, const KernelCtl& ctl, cudaStream_t s) {
-  constexpr size_t SMEM = Layout<D>::RING + static_cast<size_t>(WARPS) * 8 * NT * (D + 4) * sizeof(float);
+  constexpr size_t SMEM = Layout<D>::RING;
   auto kernel = paged_attention8_kernel<C, D, NT>;
   static std::atomic<int> residents[64];  // CTAs per SM, by device; 0: not asked yet
   int dev = 0;
@@ -661,13 +773,20 @@ rk_status launch(const Params& p, const KernelCtl& ctl, cudaStream_t s) {
     residents[dev & 63].store(resident, std::memory_order_relaxed);
   }
   const int64_t ranges = static_cast<int64_t>(p.batch) * p.hkv * p.head_groups;
-  const int64_t per_range = (static_cast<int64_t>(p.max_blocks) * p.block_size + UNIT - 1) / UNIT;
+  const int64_t per_range = (static_cast<int64_t>(p.max_blocks) * p.block_size + unit_of(D) - 1) / unit_of(D);
+  // A warp counts its places, and a sequence's over its heads, in 32 bits.
+  if (static_cast<int64_t>(p.hkv) * p.head_groups > INT32_MAX / (per_range + RANGE_COST) ||
+      ranges > (int64_t{1} << 38) / (per_range + RANGE_COST))
+    return RK_ERR_UNSUPPORTED;
   int64_t ctas = static_cast<int64_t>(device_sm_count()) * (resident < MAX_CTAS_PER_SM ? resident : MAX_CTAS_PER_SM);
-  if (ranges <= ctas && ranges * per_range < ctas) ctas = ranges * per_range;
+  // Not more warps than units; RANGE_COST places of a range hold none.
+  if (ranges <= ctas * WARPS && ranges * (per_range + RANGE_COST) < ctas * WARPS)
+    ctas = (ranges * (per_range + RANGE_COST) + WARPS - 1) / WARPS;
   e = launch_kernel(kernel, dim3(static_cast<unsigned>(ctas)), dim3(THREADS), SMEM, s, 0, p, ctl);
   note_launch("paged_attention8_kernel");
   if (e == cudaSuccess && per_range > 1) {
-    e = launch_kernel(paged_attention8_join_kernel<D>, dim3(static_cast<unsigned>(ranges)), dim3(THREADS), 0, s, 0, p, ctas);
+    e = launch_kernel(paged_attention8_join_kernel<D>, dim3(static_cast<unsigned>(ctas * WARPS)), dim3(JOIN_THREADS), 0, s,
+                      0, p);
     note_launch("paged_attention8_join_kernel");
   }
   return cuda_status(e);
@@ -686,8 +805,8 @@ rk_status launch_d(const Params& p, int64_t head_dim, int nt, const KernelCtl& c
 
 size_t paged_attention8_workspace_bytes(int64_t hq, int64_t hkv, int64_t head_dim) {
   const pa8::Plan pl = pa8::plan(hq, hkv, head_dim);
-  return static_cast<size_t>(device_sm_count()) * pa8::MAX_CTAS_PER_SM * 2 * 8 * pl.nt *
-         pa8::part_stride(static_cast<int>(head_dim)) * sizeof(float);
+  const size_t warps = static_cast<size_t>(device_sm_count()) * pa8::MAX_CTAS_PER_SM * pa8::WARPS;
+  return warps * (sizeof(pa8::Shared) + 2 * 8 * pl.nt * pa8::part_stride(static_cast<int>(head_dim)) * sizeof(float));
 }
 
 rk_status paged_attention8_launch(const PagedAttention8Args& a, void* workspace, size_t workspace_bytes, cudaStream_t s) {
@@ -707,7 +826,8 @@ rk_status paged_attention8_launch(const PagedAttention8Args& a, void* workspace,
   p.tables = a.block_tables;
   p.lens = a.context_lengths;
   p.out = a.out;
-  p.part = static_cast<float*>(workspace);
+  p.shared = static_cast<pa8::Shared*>(workspace);
+  p.part = reinterpret_cast<float*>(p.shared + device_sm_count() * pa8::MAX_CTAS_PER_SM * pa8::WARPS);
   p.batch = static_cast<int>(a.batch);
   p.hq = static_cast<int>(a.hq);
   p.hkv = static_cast<int>(a.hkv);
