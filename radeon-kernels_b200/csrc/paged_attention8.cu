@@ -81,12 +81,14 @@ struct Layout {
 // A part in the workspace: per head the unnormalised sum, then m, mo and l.
 __host__ __device__ constexpr int part_stride(int head_dim) { return head_dim + 4; }
 
-// What a warp leaves in the workspace about the range that it begins and others end.
+// What a warp leaves in the workspace about its parts.  Part 1 of a warp begins a range that
+// later CTAs end (row, heads and last describe it); part 0 continues one that an earlier CTA
+// began.  Parts of one CTA's warps are joined before, into the first of them.
 struct Shared {
-  int row;    // first row of the output
-  int heads;  // rows; 0: no such range
-  int last;   // the warp that ends it
-  int slot;   // which of the first warp's two parts; the others' is part 0
+  int row;    // of the range that part 1 begins: its first row of the output,
+  int heads;  // its rows (0: there is no part 1),
+  int last;   // and the warp that ends it
+  int kept;   // whether part 0 stands for itself
 };
 
 struct Params {
@@ -178,6 +180,13 @@ __device__ __forceinline__ float lg2_approx(float x) {
   return y;
 }
 
+// A warp's last range, of which it holds a part in shared memory.
+struct Last {
+  int64_t place;  // of the range's first unit; -1: the warp has no such part
+  int row, heads, last;
+  int begins, ends;  // whether the part holds the range's first and last unit
+};
+
 // The chunk (16 bytes of a row) that lane column c reads as its i-th of K.
 template <int D>
 __device__ __forceinline__ int k_chunk(int c, int i) {
@@ -233,6 +242,16 @@ __device__ __forceinline__ void write_out(const Params& p, int64_t element, cons
   }
 }
 
+template <int V>
+__device__ __forceinline__ void write_lane(const Params& p, int64_t element, const float* v, float f) {
+  if constexpr (V % 4 == 0) {
+    write_out<V>(p, element, v, f);
+  } else {
+    static_cast<uint32_t*>(p.out)[element >> 1] = p.bf16 ? Pack2<__nv_bfloat16>::from_floats(v[0] * f, v[1] * f)
+                                                         : Pack2<__half>::from_floats(v[0] * f, v[1] * f);
+  }
+}
+
 // What brings the sums to the output: the weights' sum, and from the one maximum to the
 // other.  Without a position it is 1 / 0, and the sums 0.
 __device__ __forceinline__ float last_factor(float m, float mo, float l) { return ex2_approx(mo - m) / l; }
@@ -256,7 +275,9 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attention8_kernel(Params p, 
   constexpr int KC = D / 64;   // 16-byte chunks of a K row per lane
   constexpr int MT = D / 16;   // MMA tiles of 16 dimensions
   constexpr int HEADS = 8 * NT;
+  static_assert(HEADS * part_stride(D) * 4 <= STAGES * L::STAGE, "a warp's sums fit its ring");
   extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ Last s_last[WARPS];
 
   pdl_begin();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -294,12 +315,9 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attention8_kernel(Params p, 
     }
     total *= tiles;
     warps = min(static_cast<int64_t>(gridDim.x) * WARPS, total);
-    if (me >= warps) {
-      if (lane == 0) p.shared[me] = shared;
-      return;
-    }
-    const int64_t u0 = share_of(me, total, warps);
-    run.left = static_cast<int>(share_of(me + 1, total, warps) - u0);
+    const bool idle = me >= warps;  // fewer places than warps
+    const int64_t u0 = share_of(idle ? 0 : me, total, warps);
+    run.left = idle ? 0 : static_cast<int>(share_of(me + 1, total, warps) - u0);
     // The sequence that holds place u0.
     int64_t before = 0;  // places, of one head tile, of earlier rounds
     for (int base = 0; base < p.batch; base += ROUND) {
@@ -424,7 +442,8 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attention8_kernel(Params p, 
   for (int s = 0; s < STAGES; ++s) load_next(s);
 
   int stage = 0;
-  int slot = 0;  // of this warp's next part
+  Last mine{-1, 0, 0, 0, 0, 0};
+  float* const sums = reinterpret_cast<float*>(smem + ring);  // for the last range's part: no tile is left then
   while (run.left > 0) {
     const int length = min(run.units - run.c, run.left);  // units of the range that this warp holds
     const int kvh = p.head_groups == 1 ? run.h : run.h / p.head_groups, hg = run.h - kvh * p.head_groups;
@@ -632,11 +651,20 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attention8_kernel(Params p, 
 
       // The end of a range.  A lane holds 16 (D 64: 8) neighbouring dimensions of two heads.
       const bool whole = length == run.units;
-      if (!whole && run.c == 0) {
-        shared.row = static_cast<int>(row0);
-        shared.heads = nheads;
-        shared.last = owner_of(place0 + run.units - 1, total, warps);
-        shared.slot = slot;
+      const bool final = run.left <= run.units + RANGE_COST - run.c;  // no other range follows
+      float* part = sums;
+      if (!whole) {
+        if (final) {
+          mine.place = place0;
+          mine.row = static_cast<int>(row0);
+          mine.heads = nheads;
+          mine.last = owner_of(place0 + run.units - 1, total, warps);
+          mine.begins = run.c == 0;
+          mine.ends = run.c + length == run.units;
+        } else {
+          part = p.part + static_cast<int64_t>(me) * 2 * HEADS * part_stride(D);  // part 0: it ends its range
+          shared.kept = 1;
+        }
       }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -647,7 +675,7 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attention8_kernel(Params p, 
           const int h = nt * 8 + 2 * c4 + i;
           constexpr int N = D == 64 ? 8 : 16;
           if (h < nheads) {
-            float* part = p.part + ((static_cast<int64_t>(me) * 2 + slot) * HEADS + h) * part_stride(D);
+            float* row = part + h * part_stride(D);
             const float f = last_factor(m[nt][i], mo[nt][i], l[nt][i]);
 #pragma unroll
             for (int k = 0; k < MT * 2 / N; ++k) {
@@ -663,82 +691,148 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attention8_kernel(Params p, 
               } else {
 #pragma unroll
                 for (int j = 0; j < N / 4; ++j)
-                  reinterpret_cast<float4*>(part + d)[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                  reinterpret_cast<float4*>(row + d)[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
               }
             }
-            if (!whole && g == 0) *reinterpret_cast<float4*>(part + D) = make_float4(m[nt][i], mo[nt][i], l[nt][i], 0.f);
+            if (!whole && g == 0) *reinterpret_cast<float4*>(row + D) = make_float4(m[nt][i], mo[nt][i], l[nt][i], 0.f);
           }
         }
-      slot = 1;
     place0 += run.units + RANGE_COST;
     next_range<D>(p, run, tiles);
+  }
+
+  // ---- the warps' last ranges: neighbours that hold parts of one range join them.
+  if (lane == 0) s_last[warp] = mine;
+  __syncthreads();
+  for (int w = 0; w < WARPS;) {
+    const Last first = s_last[w];
+    int end = w + 1;  // behind the warps that share it
+    if (first.place < 0) {
+      ++w;
+      continue;
+    }
+    while (end < WARPS && s_last[end].place == first.place) ++end;
+    const bool whole = first.begins && s_last[end - 1].ends;
+    for (int h = warp; h < first.heads; h += WARPS) {
+      constexpr int V = D / 32;  // neighbouring dimensions of a lane
+      float m = NONE, mo = NONE, l = 0.f, v[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] = 0.f;
+      const auto row = [&](int i) {
+        return reinterpret_cast<const float*>(smem + i * (STAGES * L::STAGE)) + h * part_stride(D);
+      };
+      for (int i = w; i < end; ++i) {
+        m = fmaxf(m, row(i)[D]);
+        mo = fmaxf(mo, row(i)[D + 1]);
+      }
+      for (int i = w; i < end; ++i) {
+        l = fmaf(row(i)[D + 2], ex2_approx(row(i)[D] - m), l);
+        const float f = ex2_approx(row(i)[D + 1] - mo);
+#pragma unroll
+        for (int j = 0; j < V; j += 2) {
+          const float2 x = *reinterpret_cast<const float2*>(row(i) + V * lane + j);
+          v[j] = fmaf(x.x, f, v[j]);
+          v[j + 1] = fmaf(x.y, f, v[j + 1]);
+        }
+      }
+      if (whole) {
+        write_lane<V>(p, (static_cast<int64_t>(first.row) + h) * D + V * lane, v, last_factor(m, mo, l));
+      } else {
+        float* part = p.part + ((static_cast<int64_t>(me - warp + w) * 2 + (first.begins ? 1 : 0)) * HEADS + h) * part_stride(D);
+#pragma unroll
+        for (int j = 0; j < V; j += 2) *reinterpret_cast<float2*>(part + V * lane + j) = make_float2(v[j], v[j + 1]);
+        if (lane == 0) *reinterpret_cast<float4*>(part + D) = make_float4(m, mo, l, 0.f);
+      }
+    }
+    if (warp == w && !whole) {
+      if (first.begins) {
+        shared.row = first.row;
+        shared.heads = first.heads;
+        shared.last = first.last;
+      } else {
+        shared.kept = 1;
+      }
+    }
+    w = end;
   }
   if (lane == 0) p.shared[me] = shared;
 }
 
-// Joins the parts of the ranges that several warps of the attention shared.  One CTA for the
-// range that warp blockIdx.x began (most began none), a warp for each head.
+// Joins the parts of the ranges that several CTAs of the attention shared.  One CTA for those
+// that CTA blockIdx.x began, a warp for each head; the parts in order of their CTAs.
 constexpr int JOIN_THREADS = 256;
 
 template <int D>
-__global__ void __launch_bounds__(JOIN_THREADS) paged_attention8_join_kernel(Params p) {
-  constexpr int V = D / 32;                // neighbouring dimensions of a lane
-  constexpr int AHEAD = D == 256 ? 8 : 16;  // parts whose loads are in flight together
+__global__ void __launch_bounds__(JOIN_THREADS, 4) paged_attention8_join_kernel(Params p) {
+  constexpr int V = D / 32;              // neighbouring dimensions of a lane
+  constexpr int AHEAD = D == 256 ? 4 : 8;  // parts whose sums are loaded together
   pdl_begin();
-  const int4 raw = __ldg(reinterpret_cast<const int4*>(p.shared) + blockIdx.x);
-  const Shared shared{raw.x, raw.y, raw.z, raw.w};
   const int lane = threadIdx.x & 31;
-  const int64_t step = static_cast<int64_t>(2) * p.tile_heads * part_stride(D);  // from warp to warp
-  const int n = shared.last - static_cast<int>(blockIdx.x) + 1;
-  for (int h = threadIdx.x >> 5; h < shared.heads; h += JOIN_THREADS / 32) {
-    const float* part0 = p.part + blockIdx.x * step + static_cast<int64_t>(h) * part_stride(D);
-    const int64_t shift0 = static_cast<int64_t>(shared.slot) * p.tile_heads * part_stride(D);
-    float m = NONE, mo = NONE, l = 0.f, v[V];
+  const int4* const all = reinterpret_cast<const int4*>(p.shared);
+  const int64_t part_floats = static_cast<int64_t>(p.tile_heads) * part_stride(D);
+  int4 info[WARPS];
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = 0.f;
-    for (int i0 = 0; i0 < n; i0 += AHEAD) {
-      float x[AHEAD][V];
-      float4 st[AHEAD];
+  for (int w = 0; w < WARPS; ++w) info[w] = __ldg(all + blockIdx.x * WARPS + w);
 #pragma unroll
-      for (int i = 0; i < AHEAD; ++i) {
-        const float* part = part0 + min(i0 + i, n - 1) * step + (i0 + i == 0 ? shift0 : 0);
+  for (int w = 0; w < WARPS; ++w) {
+    const Shared shared{info[w].x, info[w].y, info[w].z, info[w].w};
+    if (shared.heads == 0) continue;
+    // The part that begins the range, one of each later CTA's first warp, and one of the
+    // warp that ends it where that is no CTA's first and did not join its neighbours.
+    const int ctas = shared.last / WARPS - static_cast<int>(blockIdx.x);
+    const int n = 1 + ctas + (shared.last % WARPS != 0 && __ldg(all + shared.last).w != 0 ? 1 : 0);
+    const float* const first = p.part + (static_cast<int64_t>(blockIdx.x) * WARPS + w) * 2 * part_floats + part_floats;
+    for (int h = threadIdx.x >> 5; h < shared.heads; h += JOIN_THREADS / 32) {
+      const auto row = [&](int i) -> const float* {
+        if (i == 0) return first + h * part_stride(D);
+        const int64_t from = i <= ctas ? (static_cast<int64_t>(blockIdx.x) + i) * WARPS : shared.last;
+        return p.part + from * 2 * part_floats + h * part_stride(D);
+      };
+      float m = NONE, mo = NONE, l = 0.f, v[V];
 #pragma unroll
-        for (int j = 0; j < V; j += 2) {
-          const float2 y = *reinterpret_cast<const float2*>(part + V * lane + j);
-          x[i][j] = y.x;
-          x[i][j + 1] = y.y;
+      for (int j = 0; j < V; ++j) v[j] = 0.f;
+      for (int i0 = 0; i0 < n; i0 += 32) {  // a lane for the statistics of each of 32 parts
+        const int count = min(32, n - i0);
+        float4 st = make_float4(NONE, NONE, 0.f, 0.f);
+        if (lane < count) st = *reinterpret_cast<const float4*>(row(i0 + lane) + D);
+        float bm = fmaxf(m, st.x), bo = fmaxf(mo, st.y);
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) {
+          bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, x));
+          bo = fmaxf(bo, __shfl_xor_sync(0xffffffffu, bo, x));
         }
-        st[i] = *reinterpret_cast<const float4*>(part + D);
-      }
-      float bm = m, bo = mo;
+        float dl = st.z * ex2_approx(st.x - bm);
 #pragma unroll
-      for (int i = 0; i < AHEAD; ++i) {
-        bm = fmaxf(bm, st[i].x);  // a part that is loaded twice changes no maximum
-        bo = fmaxf(bo, st[i].y);
-      }
-      l *= ex2_approx(m - bm);
-      const float fo = ex2_approx(mo - bo);
+        for (int x = 16; x > 0; x >>= 1) dl += __shfl_xor_sync(0xffffffffu, dl, x);
+        l = fmaf(l, ex2_approx(m - bm), dl);
+        const float fo = ex2_approx(mo - bo), fi = ex2_approx(st.y - bo);
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[j] *= fo;
+        for (int j = 0; j < V; ++j) v[j] *= fo;
+        m = bm;
+        mo = bo;
+        for (int j0 = 0; j0 < count; j0 += AHEAD) {
+          float x[AHEAD][V];
 #pragma unroll
-      for (int i = 0; i < AHEAD; ++i) {
-        if (i0 + i < n) {
-          l = fmaf(st[i].z, ex2_approx(st[i].x - bm), l);
-          const float f = ex2_approx(st[i].y - bo);
+          for (int j = 0; j < AHEAD; ++j) {
+            const float* from = row(i0 + min(j0 + j, count - 1)) + V * lane;
 #pragma unroll
-          for (int j = 0; j < V; ++j) v[j] = fmaf(x[i][j], f, v[j]);
+            for (int k = 0; k < V; k += 2) {
+              const float2 y = *reinterpret_cast<const float2*>(from + k);
+              x[j][k] = y.x;
+              x[j][k + 1] = y.y;
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < AHEAD; ++j) {
+            const float f = __shfl_sync(0xffffffffu, fi, (j0 + j) & 31);
+            if (j0 + j < count) {
+#pragma unroll
+              for (int k = 0; k < V; ++k) v[k] = fmaf(x[j][k], f, v[k]);
+            }
+          }
         }
       }
-      m = bm;
-      mo = bo;
-    }
-    const float f = last_factor(m, mo, l);
-    const int64_t element = (static_cast<int64_t>(shared.row) + h) * D + V * lane;
-    if (V >= 4) {
-      write_out<V < 4 ? 4 : V>(p, element, v, f);
-    } else {
-      static_cast<uint32_t*>(p.out)[element >> 1] = p.bf16 ? Pack2<__nv_bfloat16>::from_floats(v[0] * f, v[1] * f)
-                                                           : Pack2<__half>::from_floats(v[0] * f, v[1] * f);
+      write_lane<V>(p, (static_cast<int64_t>(shared.row) + h) * D + V * lane, v, last_factor(m, mo, l));
     }
   }
 }
@@ -785,8 +879,7 @@ rk_status launch(const Params& p, const KernelCtl& ctl, cudaStream_t s) {
   e = launch_kernel(kernel, dim3(static_cast<unsigned>(ctas)), dim3(THREADS), SMEM, s, 0, p, ctl);
   note_launch("paged_attention8_kernel");
   if (e == cudaSuccess && per_range > 1) {
-    e = launch_kernel(paged_attention8_join_kernel<D>, dim3(static_cast<unsigned>(ctas * WARPS)), dim3(JOIN_THREADS), 0, s,
-                      0, p);
+    e = launch_kernel(paged_attention8_join_kernel<D>, dim3(static_cast<unsigned>(ctas)), dim3(JOIN_THREADS), 0, s, 0, p);
     note_launch("paged_attention8_join_kernel");
   }
   return cuda_status(e);
