@@ -39,6 +39,7 @@
 #include <cuda_runtime.h>
 
 #include <atomic>
+#include <chrono>
 
 #include "rk_cache8.cuh"
 #include "rk_device.cuh"
@@ -81,16 +82,6 @@ struct Layout {
 // A part in the workspace: per head the unnormalised sum, then m, mo and l.
 __host__ __device__ constexpr int part_stride(int head_dim) { return head_dim + 4; }
 
-// What a warp leaves in the workspace about its parts.  Part 1 of a warp begins a range that
-// later CTAs end (row, heads and last describe it); part 0 continues one that an earlier CTA
-// began.  Parts of one CTA's warps are joined before, into the first of them.
-struct Shared {
-  int row;    // of the range that part 1 begins: its first row of the output,
-  int heads;  // its rows (0: there is no part 1),
-  int last;   // and the warp that ends it
-  int kept;   // whether part 0 stands for itself
-};
-
 struct Params {
   const void* q;
   const uint8_t* k;
@@ -100,13 +91,24 @@ struct Params {
   const void* tables;
   const void* lens;
   void* out;
-  float* part;     // [warp][2][heads of a tile][part_stride]
-  Shared* shared;  // [warp]
+  float* part;      // [warp][2][heads of a tile][part_stride]: part 0 continues a range, part 1 begins one
+  uint64_t* arrivals;  // [warp]: `tag` plus the parts written of the range that the warp begins; or anything
+  uint64_t tag;        // of this launch; its low 16 bits are 0, the others not all
   int batch, hq, hkv, group, head_groups, tile_heads;
-  int num_blocks, block_size, block_shift, max_blocks;
+  int num_blocks, block_size, max_blocks;
+  uint32_t block_multiplier;  // t / block_size = t * block_multiplier >> block_shift for t < 2^31
+  int block_shift;
   int index_bits, bf16;
   float scale_log2;
 };
+
+// A launch constant, hidden from the compiler, which would otherwise keep a copy of every loop for
+// each value of each flag: 75 KB of code at head_dim 128 instead of KBYTES, and the time to
+// fetch it, in every launch.
+__device__ __forceinline__ int flag_of(int v) {
+  asm volatile("" : "+r"(v));
+  return v;
+}
 
 // An index as loaded: nothing waits for the load until value_of.
 struct Raw {
@@ -114,7 +116,7 @@ struct Raw {
 };
 __device__ __forceinline__ Raw load_raw(const void* p, int bits, int64_t i) {
   Raw r{0, 0};
-  if (bits == 32) {
+  if (flag_of(bits) == 32) {
     r.lo = __ldg(static_cast<const uint32_t*>(p) + i);
   } else {
     const uint2 v = __ldg(static_cast<const uint2*>(p) + i);
@@ -124,7 +126,7 @@ __device__ __forceinline__ Raw load_raw(const void* p, int bits, int64_t i) {
   return r;
 }
 __device__ __forceinline__ int64_t value_of(Raw r, int bits) {
-  return bits == 32 ? static_cast<int64_t>(static_cast<int32_t>(r.lo))
+  return flag_of(bits) == 32 ? static_cast<int64_t>(static_cast<int32_t>(r.lo))
                     : static_cast<int64_t>(static_cast<uint64_t>(r.hi) << 32 | r.lo);
 }
 
@@ -136,6 +138,12 @@ __device__ __forceinline__ int context_of(const Params& p, Raw raw) {
 
 __device__ __forceinline__ int context_of(const Params& p, int b) {
   return context_of(p, load_raw(p.lens, p.index_bits, b));
+}
+
+// The block of position t, by a multiplication (the host's multiplier is 2^block_shift /
+// block_size, rounded up; with 31 bits more than block_size's that is exact below 2^31).
+__device__ __forceinline__ int block_of(const Params& p, int t) {
+  return static_cast<int>(static_cast<uint64_t>(static_cast<uint32_t>(t)) * p.block_multiplier >> p.block_shift);
 }
 
 // Units of one (sequence, head tile); an empty sequence has one, which writes its NaN.
@@ -180,12 +188,36 @@ __device__ __forceinline__ float lg2_approx(float x) {
   return y;
 }
 
-// A warp's last range, of which it holds a part in shared memory.
-struct Last {
-  int64_t place;  // of the range's first unit; -1: the warp has no such part
-  int row, heads, last;
+// A range of which a warp holds a part.
+struct Piece {
+  uint32_t place;  // of the range's first unit
+  int row, heads, units;  // heads 0: there is none
   int begins, ends;  // whether the part holds the range's first and last unit
 };
+
+// Adds `parts` to the arrivals of a range and returns whether that makes `all`.  A word that does not
+// carry the launch's tag counts as none; the last to arrive leaves 0, so that the next launch
+// of a captured graph, whose tag is the same, starts anew.  The word was seen as `seen`: once
+// tagged it stays so until the last arrival, so an addition is enough (tens of CTAs can come
+// at once, and exchanges would repeat); the first to come to an untagged word tags it.
+// Nothing waits for another CTA.
+__device__ __forceinline__ bool arrive(uint64_t* word, uint64_t seen, uint64_t tag, int parts, int all) {
+  auto* const at = reinterpret_cast<unsigned long long*>(word);
+  uint64_t before = tag;
+  for (;;) {
+    if ((seen & ~uint64_t{0xFFFF}) == tag) {
+      before = atomicAdd(at, static_cast<unsigned long long>(parts));
+      break;
+    }
+    const uint64_t found = atomicCAS(at, seen, tag + parts);
+    if (found == seen) break;
+    seen = found;
+  }
+  const bool last = static_cast<int>(before & 0xFFFF) + parts == all;
+  if (last) *word = 0;
+  return last;
+}
+__device__ __forceinline__ void fence_gpu() { asm volatile("fence.acq_rel.gpu;" ::: "memory"); }
 
 // The chunk (16 bytes of a row) that lane column c reads as its i-th of K.
 template <int D>
@@ -193,22 +225,25 @@ __device__ __forceinline__ int k_chunk(int c, int i) {
   return D == 64 ? c : 2 * c + (i & 1) + 8 * (i >> 1);
 }
 
-// A place in the row of all units: sequence b, head tile h, unit c of its `units`; `left` units
+// A place in the row of all units: sequence b, KV head h and its group hg of query heads (a
+// head tile), unit c of its `units`; `left` units
 // of this warp's share from here on.  Every range is followed by RANGE_COST places that hold
 // no unit, so that shares with many short ranges hold fewer units.  The next sequence's
 // length is loaded a sequence ahead.
 struct Walk {
-  int b, h, c, units, left, context;
+  int b, h, hg, c, units, left, context;
   Raw next;
 };
 
 // To the first unit of the next (sequence, head tile).  Past the last sequence the walk holds
 // some valid length and is not used (left <= 0).
 template <int D>
-__device__ __forceinline__ void next_range(const Params& p, Walk& w, int tiles) {
+__device__ __forceinline__ void next_range(const Params& p, Walk& w) {
   w.left -= w.units + RANGE_COST - w.c;
   w.c = 0;
-  if (++w.h < tiles) return;
+  if (++w.hg < p.head_groups) return;
+  w.hg = 0;
+  if (++w.h < p.hkv) return;
   w.h = 0;
   ++w.b;
   w.context = context_of(p, w.next);
@@ -217,19 +252,20 @@ __device__ __forceinline__ void next_range(const Params& p, Walk& w, int tiles) 
 }
 
 template <int D>
-__device__ __forceinline__ void next_unit(const Params& p, Walk& w, int tiles) {
+__device__ __forceinline__ void next_unit(const Params& p, Walk& w) {
   ++w.c;
   --w.left;
-  if (w.c == w.units) next_range<D>(p, w, tiles);
+  if (w.c == w.units) next_range<D>(p, w);
 }
 
 // N (a multiple of 4) neighbouring elements of an output row times f.
 template <int N>
 __device__ __forceinline__ void write_out(const Params& p, int64_t element, const float* v, float f) {
   uint32_t w[N / 2];
+  const int bf16 = flag_of(p.bf16);
 #pragma unroll
   for (int i = 0; i < N / 2; ++i)
-    w[i] = p.bf16 ? Pack2<__nv_bfloat16>::from_floats(v[2 * i] * f, v[2 * i + 1] * f)
+    w[i] = bf16 ? Pack2<__nv_bfloat16>::from_floats(v[2 * i] * f, v[2 * i + 1] * f)
                   : Pack2<__half>::from_floats(v[2 * i] * f, v[2 * i + 1] * f);
   uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + element);
   if (N % 8 == 0) {
@@ -242,30 +278,141 @@ __device__ __forceinline__ void write_out(const Params& p, int64_t element, cons
   }
 }
 
-template <int V>
-__device__ __forceinline__ void write_lane(const Params& p, int64_t element, const float* v, float f) {
-  if constexpr (V % 4 == 0) {
-    write_out<V>(p, element, v, f);
-  } else {
-    static_cast<uint32_t*>(p.out)[element >> 1] = p.bf16 ? Pack2<__nv_bfloat16>::from_floats(v[0] * f, v[1] * f)
-                                                         : Pack2<__half>::from_floats(v[0] * f, v[1] * f);
-  }
-}
-
 // What brings the sums to the output: the weights' sum, and from the one maximum to the
 // other.  Without a position it is 1 / 0, and the sums 0.
 __device__ __forceinline__ float last_factor(float m, float mo, float l) { return ex2_approx(mo - m) / l; }
 
-// First place of warp w's share.  The division is 32 bits wide where it can be.
-__device__ __forceinline__ int64_t share_of(uint32_t w, int64_t total, int64_t warps) {
-  const uint64_t product = static_cast<uint64_t>(w) * static_cast<uint64_t>(total);
-  if (product >> 32 == 0) return static_cast<uint32_t>(product) / static_cast<uint32_t>(warps);
-  return static_cast<int64_t>(product / static_cast<uint64_t>(warps));
+// The shares of all warps: `extra` of them hold base + 1 places, the others base.  The host has
+// checked that the places of the largest lengths fit 32 bits.
+struct Shares {
+  uint32_t total, warps, base, extra;
+  __device__ __forceinline__ void set(uint32_t places, uint32_t most_warps) {
+    total = places;
+    warps = min(most_warps, places);
+    base = places / warps;
+    extra = places - base * warps;
+  }
+  __device__ __forceinline__ uint32_t start(uint32_t w) const { return w * base + min(w, extra); }
+  // The warp that holds a place.  There are some thousand at most, so the quotient is good to
+  // one in fp32.
+  __device__ __forceinline__ uint32_t owner(uint32_t place) const {
+    const uint32_t wide = extra * (base + 1);
+    const bool in = place < wide;
+    const float guess = __fdividef(static_cast<float>(in ? place : place - wide), static_cast<float>(in ? base + 1 : base));
+    uint32_t w = min((in ? 0u : extra) + static_cast<uint32_t>(guess), warps - 1);
+    if (start(w) > place) --w;
+    if (start(w + 1) <= place) ++w;
+    return w;
+  }
+};
+
+template <int D, int HEADS>
+__device__ __forceinline__ float* part_of(const Params& p, int warp, int k) {
+  return p.part + (static_cast<int64_t>(warp) * 2 + k) * (HEADS * part_stride(D));
 }
 
-// The warp whose share holds place u: the largest w with floor(w * total / warps) <= u.
-__device__ __forceinline__ int owner_of(int64_t u, int64_t total, int64_t warps) {
-  return static_cast<int>(((u + 1) * warps - 1) / total);
+// The parts in the workspace of a range that starts at `place`: that of the warp that begins it,
+// one of each later CTA (of its first warp), and one of the warp that ends it where that
+// is no CTA's first and went on to other ranges (otherwise it joined its neighbours').
+struct Parts {
+  int begin, end, ctas, count;
+  __device__ __forceinline__ Parts(uint32_t place, int units, const Shares& shares) {
+    begin = static_cast<int>(shares.owner(place));
+    end = static_cast<int>(shares.owner(place + units - 1));
+    ctas = end / WARPS - begin / WARPS;
+    const bool went_on = shares.start(end + 1) > place + units + RANGE_COST;
+    count = 1 + ctas + (end % WARPS != 0 && end != begin && went_on ? 1 : 0);
+  }
+  __device__ __forceinline__ int warp(int i) const {
+    return i == 0 ? begin : (i <= ctas ? (begin / WARPS + i) * WARPS : end);
+  }
+};
+
+// Sums of one head, spread over the 16 lanes of half a warp.
+template <int D>
+struct Sums {
+  static constexpr int V = D / 16;  // neighbouring dimensions of a lane
+  float m, mo, l, v[V];
+  __device__ __forceinline__ void start() {
+    m = mo = NONE;
+    l = 0.f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = 0.f;
+  }
+  // To maxima that are at least the present ones.
+  __device__ __forceinline__ void raise(float bm, float bo) {
+    l *= ex2_approx(m - bm);
+    const float f = ex2_approx(mo - bo);
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] *= f;
+    m = bm;
+    mo = bo;
+  }
+  __device__ __forceinline__ void add(const float (&x)[V], float f) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = fmaf(x[j], f, v[j]);
+  }
+  static __device__ __forceinline__ void load(float (&x)[V], const float* row, int lane) {
+#pragma unroll
+    for (int j = 0; j < V; j += 4) {
+      const float4 y = *reinterpret_cast<const float4*>(row + V * lane + j);
+      x[j] = y.x;
+      x[j + 1] = y.y;
+      x[j + 2] = y.z;
+      x[j + 3] = y.w;
+    }
+  }
+  __device__ __forceinline__ void store(float* row, int lane) const {
+#pragma unroll
+    for (int j = 0; j < V; j += 4)
+      *reinterpret_cast<float4*>(row + V * lane + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+    if (lane == 0) *reinterpret_cast<float4*>(row + D) = make_float4(m, mo, l, 0.f);
+  }
+  __device__ __forceinline__ void write(const Params& p, int64_t row, int lane) const {
+    write_out<V>(p, row * D + V * lane, v, last_factor(m, mo, l));
+  }
+};
+
+// One head of a range from its parts, written by other SMs: read past L1, some at a time.
+template <int D, int HEADS>
+__device__ __forceinline__ void join_head(const Params& p, const Parts& parts, int64_t out_row, int h, int lane) {
+  constexpr int AHEAD = D == 256 ? 4 : 8;
+  Sums<D> sums{};
+  sums.start();
+#pragma unroll 1
+  for (int i0 = 0; i0 < parts.count; i0 += AHEAD) {
+    float x[AHEAD][Sums<D>::V];
+    float4 st[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const int i = min(i0 + j, parts.count - 1);
+      const float* row = part_of<D, HEADS>(p, parts.warp(i), i == 0 ? 1 : 0) + h * part_stride(D);
+      st[j] = __ldcg(reinterpret_cast<const float4*>(row + D));
+#pragma unroll
+      for (int k = 0; k < Sums<D>::V; k += 4) {
+        const float4 y = __ldcg(reinterpret_cast<const float4*>(row + Sums<D>::V * lane + k));
+        x[j][k] = y.x;
+        x[j][k + 1] = y.y;
+        x[j][k + 2] = y.z;
+        x[j][k + 3] = y.w;
+      }
+    }
+    float bm = sums.m, bo = sums.mo;
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      bm = fmaxf(bm, st[j].x);  // a part that is loaded twice changes no maximum
+      bo = fmaxf(bo, st[j].y);
+    }
+    sums.raise(bm, bo);
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      if (i0 + j < parts.count) {
+        sums.l = fmaf(st[j].z, ex2_approx(st[j].x - bm), sums.l);
+        sums.add(x[j], ex2_approx(st[j].y - bo));
+      }
+    }
+  }
+  sums.write(p, out_row, lane);
 }
 
 template <typename C, int D, int NT>
@@ -277,91 +424,90 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attention8_kernel(Params p, 
   constexpr int HEADS = 8 * NT;
   static_assert(HEADS * part_stride(D) * 4 <= STAGES * L::STAGE, "a warp's sums fit its ring");
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ Last s_last[WARPS];
+  __shared__ Piece s_last[WARPS];   // of each warp's last range: the part is in its ring
+  __shared__ Piece s_ended[WARPS];  // of its first, which others began: the part is in the workspace
+  __shared__ __align__(16) uint32_t s_place[WARPS];
+  __shared__ int s_join[2 * WARPS];
 
   pdl_begin();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, c4 = lane & 3;
   const int tiles = p.hkv * p.head_groups;
   const int me = static_cast<int>(blockIdx.x) * WARPS + warp;
-  Shared shared{0, 0, 0, 0};
 
   // ---- this warp's share, found 128 sequences at a time (four neighbours to a lane, so that
   // the loads of a round are in flight together).
   Walk run{};
-  int64_t place0, total = 0, warps;  // of this warp's range: the place of its first unit
+  Shares shares;
+  uint32_t place0;  // of this warp's range: the place of its first unit
   {
     constexpr int ROUND = 128;
-    int unit[4];
-    auto load_round = [&](int base) -> int {  // the units of a lane's four sequences
+    int context[4];
+    uint32_t mine = 0, upto = 0, total = 0;  // places of this lane's sequences, of all up to them, of all
+    const auto round = [&](int base) {
       Raw raw[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) raw[i] = load_raw(p.lens, p.index_bits, min(base + 4 * lane + i, p.batch - 1));
-      int sum = 0;
+      mine = 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        unit[i] = base + 4 * lane + i < p.batch ? units_of<D>(context_of(p, raw[i])) + RANGE_COST : 0;
-        sum += unit[i];
+        context[i] = context_of(p, raw[i]);
+        mine += base + 4 * lane + i < p.batch ? units_of<D>(context[i]) + RANGE_COST : 0;
       }
-      return sum;
-    };
-    int mine = 0;
-    for (int base = 0; base < p.batch; base += ROUND) {
-      mine = load_round(base);
-      int64_t sum = mine;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      total += sum;
-    }
-    total *= tiles;
-    warps = min(static_cast<int64_t>(gridDim.x) * WARPS, total);
-    const bool idle = me >= warps;  // fewer places than warps
-    const int64_t u0 = share_of(idle ? 0 : me, total, warps);
-    run.left = idle ? 0 : static_cast<int>(share_of(me + 1, total, warps) - u0);
-    // The sequence that holds place u0.
-    int64_t before = 0;  // places, of one head tile, of earlier rounds
-    for (int base = 0; base < p.batch; base += ROUND) {
-      if (p.batch > ROUND) mine = load_round(base);
-      int64_t upto = mine;
+      upto = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+        const uint32_t x = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += x;
       }
+    };
+#pragma unroll 1
+    for (int base = 0; base < p.batch; base += ROUND) {
+      round(base);
+      total += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    shares.set(total * tiles, gridDim.x * WARPS);
+    const bool idle = me >= static_cast<int>(shares.warps);  // fewer places than warps
+    const uint32_t u0 = shares.start(idle ? 0 : me);
+    run.left = idle ? 0 : static_cast<int>(shares.start(me + 1) - u0);
+    // The sequence that holds place u0.
+    uint32_t before = 0;  // places, of one head tile, of earlier rounds
+#pragma unroll 1
+    for (int base = 0; base < p.batch; base += ROUND) {
+      if (p.batch > ROUND) round(base);
       const uint32_t past = __ballot_sync(0xffffffffu, (before + upto) * tiles > u0);
       if (past != 0) {
-        const int at = __ffs(past) - 1;
-        int64_t prior = __shfl_sync(0xffffffffu, before + upto - mine, at);
-        int b = base + 4 * at, units = 0;
+        // Each lane looks among its own four; the first that has it tells the others.
+        uint32_t prior = before + upto - mine;
+        int i = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int n = __shfl_sync(0xffffffffu, unit[i], at);
-          if (units == 0) {
-            if ((prior + n) * tiles > u0) {
-              units = n;
-            } else {
-              prior += n;
-              ++b;
-            }
+        for (int k = 0; k < 3; ++k) {
+          const uint32_t behind = prior + units_of<D>(context[k]) + RANGE_COST;
+          if (i == k && behind * tiles <= u0) {
+            prior = behind;
+            ++i;
           }
         }
-        const uint32_t in = static_cast<uint32_t>(u0 - prior * tiles);  // below tiles * units, which the host checked
-        run.b = b;
-        run.h = static_cast<int>(in / static_cast<uint32_t>(units));
-        run.c = static_cast<int>(in - static_cast<uint32_t>(run.h) * units);
-        run.units = units - RANGE_COST;
+        const int here = i == 0 ? context[0] : i == 1 ? context[1] : i == 2 ? context[2] : context[3];
+        const int at = __ffs(past) - 1;
+        run.b = __shfl_sync(0xffffffffu, base + 4 * lane + i, at);
+        run.context = __shfl_sync(0xffffffffu, here, at);
+        run.units = units_of<D>(run.context);
+        const uint32_t in = u0 - __shfl_sync(0xffffffffu, prior, at) * tiles;
+        const int tile = static_cast<int>(in / static_cast<uint32_t>(run.units + RANGE_COST));
+        run.c = static_cast<int>(in) - tile * (run.units + RANGE_COST);
+        run.h = p.head_groups == 1 ? tile : tile / p.head_groups;
+        run.hg = tile - run.h * p.head_groups;
         place0 = u0 - run.c;
         break;
       }
       before += __shfl_sync(0xffffffffu, upto, 31);
     }
   }
-  run.context = context_of(p, run.b);
   run.next = load_raw(p.lens, p.index_bits, min(run.b + 1, p.batch - 1));
-
   if (run.c >= run.units) {  // the share starts behind a range
     place0 += run.units + RANGE_COST;
-    next_range<D>(p, run, tiles);
+    next_range<D>(p, run);
   }
 
   // ---- this warp's ring; `load` runs ahead of `run`.
@@ -371,28 +517,48 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attention8_kernel(Params p, 
   const int64_t slot_bytes = static_cast<int64_t>(p.hkv) * D;
   constexpr int CHUNKS = D / 16, PER = 32 / CHUNKS;  // chunks of a row, rows side by side
   const int r0 = lane / CHUNKS, ch = lane - r0 * CHUNKS;
+  // Where this lane's chunk of row r0 + i * PER lies: the row's number, modulo 8, is r0 ^ (i * PER
+  // % 8), so that the exchange of chunks is one XOR with a constant.
+  const int lane_chunk = (D == 64 ? ch : ch ^ r0) * 16;
   const int64_t lane_bytes = r0 * slot_bytes + ch * 16, step_bytes = PER * slot_bytes, to_v = p.v - p.k;
 
-  // The table entry of the row that this lane (lane % TILE) looks up for the tile of `w`.
-  auto look_up = [&](const Walk& w) -> Raw {
-    const int t = w.c * TILE + (lane & (TILE - 1));
-    const int j = p.block_shift >= 0 ? t >> p.block_shift : t / p.block_size;
-    return t < w.context ? load_raw(p.tables, p.index_bits, static_cast<int64_t>(w.b) * p.max_blocks + j) : Raw{0, 0};
+  // The block table, 32 entries at a time: lane i holds the block of page `first` + i, -1 where
+  // that is no page of the sequence or no block of the cache.  They serve the tiles before
+  // `until`; the entries after them -- of this range or the next -- are loaded ahead.
+  int page_block = -1, first = 0, until = 0, ahead_first = 0;
+  Raw ahead{0, 0};
+  auto load_pages = [&](int b, int from, int context) {
+    ahead_first = from;
+    const int pages = context > 0 ? block_of(p, context - 1) + 1 : 0;
+    ahead = from + lane < pages ? load_raw(p.tables, p.index_bits, static_cast<int64_t>(b) * p.max_blocks + from + lane)
+                                : Raw{0xFFFFFFFFu, 0xFFFFFFFFu};
   };
-  auto issue = [&](const Walk& w, Raw entry, int stage) {
+  auto turn_page = [&](const Walk& w) {
+    first = ahead_first;
+    const int pages = w.context > 0 ? block_of(p, w.context - 1) + 1 : 0;
+    const int64_t value = value_of(ahead, p.index_bits);
+    const bool found = value >= 0 && value < p.num_blocks;
+    if (first + lane < pages && !found) atomicOr(ctl.status, RK_DEV_ERR_BAD_INDEX);
+    page_block = found ? static_cast<int>(value) : -1;
+    until = first + 32 < pages ? (first + 32) * p.block_size / TILE : w.units;
+    if (until < w.units) {
+      load_pages(w.b, block_of(p, until * TILE), w.context);
+    } else {
+      const bool same = w.h + 1 < p.hkv || w.hg + 1 < p.head_groups;  // sequence
+      load_pages(same ? w.b : min(w.b + 1, p.batch - 1), 0, same ? w.context : context_of(p, w.next));
+    }
+  };
+  auto issue = [&](const Walk& w, int stage) {
     const int offset = ring + stage * L::STAGE;
     const uint32_t base = smem_base + offset;
-    const int kvh = p.head_groups == 1 ? w.h : w.h / p.head_groups;
     const int t = w.c * TILE + (lane & (TILE - 1));
-    const int off = p.block_shift >= 0 ? t & (p.block_size - 1) : t % p.block_size;
-    const int64_t value = value_of(entry, p.index_bits);
-    const bool in = t < w.context, found = value >= 0 && value < p.num_blocks;
-    if (in && !found && lane < TILE) atomicOr(ctl.status, RK_DEV_ERR_BAD_INDEX);
-    const int blk = in && found ? static_cast<int>(value) : -1;
+    const int page = block_of(p, t), off = t - page * p.block_size;
+    const int held = __shfl_sync(0xffffffffu, page_block, (page - first) & 31);
+    const int blk = t < w.context ? held : -1;
     const uint32_t mask = __ballot_sync(0xffffffffu, blk >= 0);
     if (lane == 0)
       *reinterpret_cast<uint32_t*>(smem + offset + L::MASK) = TILE == 32 ? mask : mask & 0xFFFFu;
-    const int64_t scale_at = static_cast<int64_t>(blk < 0 ? 0 : blk) * p.hkv + kvh;
+    const int64_t scale_at = static_cast<int64_t>(blk < 0 ? 0 : blk) * p.hkv + w.h;
     const uint32_t scale_bytes = blk < 0 ? 0u : 4u;
     if (TILE == 32) {
       cp_async4(base + L::SCALES + lane * 4, p.ks + scale_at, scale_bytes);
@@ -402,22 +568,23 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attention8_kernel(Params p, 
     }
     // Bytes from the start of a cache to this lane's row.
     const int64_t row_bytes = (static_cast<int64_t>(blk < 0 ? 0 : blk) * p.block_size + (blk < 0 ? 0 : off)) * slot_bytes;
-    const int head_bytes = kvh * D;
-    if (mask == 0xFFFFFFFFu && p.block_size % 16 == 0) {
+    const int head_bytes = w.h * D;
+    if (mask == 0xFFFFFFFFu && flag_of(p.block_size) % 16 == 0) {
       // Full tiles whose 16 positions lie side by side.
 #pragma unroll
       for (int sub = 0; sub < SUB; ++sub) {
         const uint8_t* from = p.k + __shfl_sync(0xffffffffu, row_bytes, 16 * sub) + head_bytes + lane_bytes;
 #pragma unroll
         for (int i = 0; i < 16 / PER; ++i) {
-          const int r = 16 * sub + i * PER + r0;
-          cp_async16(base + L::k_at(r, ch), from, 16);
-          cp_async16(base + L::v_at(r, ch), from + to_v, 16);
+          const int r = 16 * sub + i * PER;  // and r0
+          const uint32_t chunk = base + (D == 64 ? lane_chunk : lane_chunk ^ ((i * PER % 8) * 16));
+          cp_async16(chunk + r0 * D + r * D, from, 16);
+          cp_async16(chunk + r0 * L::V_STRIDE + L::K_BYTES + r * L::V_STRIDE, from + to_v, 16);
           from += step_bytes;
         }
       }
     } else {
-#pragma unroll 4
+#pragma unroll 1
       for (int i = 0; i < TILE / PER; ++i) {
         const int r = i * PER + r0;
         const uint8_t* from = p.k + __shfl_sync(0xffffffffu, row_bytes, r) + head_bytes + ch * 16;
@@ -428,46 +595,70 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attention8_kernel(Params p, 
     }
   };
 
-  Raw entry{0, 0};
-  if (load.left > 0) entry = look_up(load);
+  load_pages(load.b, block_of(p, load.c * TILE), load.context);
   auto load_next = [&](int stage) {  // always a group, so that the groups count the tiles
     if (load.left > 0) {
-      issue(load, entry, stage);
-      next_unit<D>(p, load, tiles);
-      if (load.left > 0) entry = look_up(load);
+      if (load.c >= until) turn_page(load);
+      issue(load, stage);
+      const int c = load.c;
+      next_unit<D>(p, load);
+      if (load.c <= c) until = 0;  // another range
     }
     cp_async_commit();
   };
+  // Queries of a head tile: lane (g, c4) holds head g's dimensions of its K chunks.  Where the
+  // registers allow it they are loaded a range ahead.
+  constexpr bool QUERIES_AHEAD = NT == 1 && D <= 128;
+  uint2 queries[NT][4 * KC];
+  auto load_queries = [&](int b, int h, int hg) {
+    const int64_t row0 = static_cast<int64_t>(b) * p.hq + h * p.group + hg * HEADS;
 #pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const bool live = nt * 8 + g < p.group - hg * HEADS;
+      const uint16_t* row = static_cast<const uint16_t*>(p.q) + (row0 + nt * 8 + g) * D;
+#pragma unroll
+      for (int j = 0; j < 4 * KC; ++j) {
+        queries[nt][j] = make_uint2(0, 0);
+        if (live) queries[nt][j] = __ldg(reinterpret_cast<const uint2*>(row + k_chunk<D>(c4, j >> 2) * 16 + (j & 3) * 4));
+      }
+    }
+  };
+  if (run.left > 0) load_queries(run.b, run.h, run.hg);
+  const uint32_t place_first = place0;
+
+#pragma unroll 1
   for (int s = 0; s < STAGES; ++s) load_next(s);
+  // The arrivals of the range that this warp may begin: tagged early where the last launch left
+  // them at 0.
+  if (lane == 0) atomicCAS(reinterpret_cast<unsigned long long*>(p.arrivals + me), 0ull, p.tag);
+
+  // Offsets of this lane's operands within a tile: K's chunks 2 c4 (and + 1: XOR 16) of row g, V's
+  // chunk g of rows 2 c4 (and + 1); rows 8 and 16 further on keep their place modulo 8.
+  const int k_lane = L::k_at(g, D == 64 ? c4 : 2 * c4), v_lane = L::K_BYTES + 2 * c4 * L::V_STRIDE + (g ^ (2 * c4)) * 16;
 
   int stage = 0;
-  Last mine{-1, 0, 0, 0, 0, 0};
+  Piece mine{}, ended{};
   float* const sums = reinterpret_cast<float*>(smem + ring);  // for the last range's part: no tile is left then
   while (run.left > 0) {
     const int length = min(run.units - run.c, run.left);  // units of the range that this warp holds
-    const int kvh = p.head_groups == 1 ? run.h : run.h / p.head_groups, hg = run.h - kvh * p.head_groups;
-    const int head0 = kvh * p.group + hg * HEADS;
-    const int nheads = min(HEADS, p.group - hg * HEADS);
+    const int head0 = run.h * p.group + run.hg * HEADS;
+    const int nheads = min(HEADS, p.group - run.hg * HEADS);
     const int64_t row0 = static_cast<int64_t>(run.b) * p.hq + head0;
+    if (!QUERIES_AHEAD && place0 != place_first) load_queries(run.b, run.h, run.hg);
     uint32_t qf[NT][4 * KC][2];
       float factor[NT][2];
       float o[NT][MT][4];
       float m[NT][2], mo[NT][2], l[NT][2];
-      // Queries of the head tile: lane (g, c4) holds head g's dimensions of its K chunks.
+      const int bf16 = flag_of(p.bf16);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const bool live = nt * 8 + g < nheads;
-        const int64_t row = (row0 + nt * 8 + g) * D;
         float f[4 * KC][4];
         float amax = 0.f;
 #pragma unroll
         for (int j = 0; j < 4 * KC; ++j) {
-          uint2 raw = make_uint2(0, 0);
-          const int64_t at = row + k_chunk<D>(c4, j >> 2) * 16 + (j & 3) * 4;
-          if (live) raw = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.q) + at));
-          const float2 a = p.bf16 ? Pack2<__nv_bfloat16>::to_floats(raw.x) : Pack2<__half>::to_floats(raw.x);
-          const float2 b = p.bf16 ? Pack2<__nv_bfloat16>::to_floats(raw.y) : Pack2<__half>::to_floats(raw.y);
+          const uint2 raw = queries[nt][j];
+          const float2 a = bf16 ? Pack2<__nv_bfloat16>::to_floats(raw.x) : Pack2<__half>::to_floats(raw.x);
+          const float2 b = bf16 ? Pack2<__nv_bfloat16>::to_floats(raw.y) : Pack2<__half>::to_floats(raw.y);
           f[j][0] = a.x;
           f[j][1] = a.y;
           f[j][2] = b.x;
@@ -500,6 +691,11 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attention8_kernel(Params p, 
           for (int i = 0; i < 4; ++i) o[nt][mt][i] = 0.f;
       }
 
+      if (QUERIES_AHEAD && run.left > run.units + RANGE_COST - run.c) {
+        const bool more = run.hg + 1 < p.head_groups, same = more || run.h + 1 < p.hkv;
+        load_queries(same ? run.b : run.b + 1, more ? run.h : same ? run.h + 1 : 0, more ? run.hg + 1 : 0);
+      }
+
       for (int step = 0; step < length; ++step) {
         cp_async_wait<STAGES - 1>();
         __syncwarp();
@@ -517,8 +713,8 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attention8_kernel(Params p, 
           for (int i = 0; i < KC; ++i) {
 #pragma unroll
             for (int t = 0; t < SUB; ++t) {
-              const uint4 ka = at_smem<uint4>(tile, L::k_at(16 * t + g, k_chunk<D>(c4, i)));
-              const uint4 kb = at_smem<uint4>(tile, L::k_at(16 * t + g + 8, k_chunk<D>(c4, i)));
+              const int at = (k_lane ^ ((i & 1) * 16)) + (i >> 1) * 128 + 16 * t * D;
+              const uint4 ka = at_smem<uint4>(tile, at), kb = at_smem<uint4>(tile, at + 8 * D);
               const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
@@ -601,8 +797,8 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attention8_kernel(Params p, 
           // byte side by side, are two rows of the operand.
 #pragma unroll
           for (int t = 0; t < SUB; ++t) {
-            const int row = 16 * t + 2 * c4;
             if (D == 64) {
+              const int row = 16 * t + 2 * c4;
               const int at = L::K_BYTES + g * 8;
               const uint2 va = at_smem<uint2>(tile, at + row * L::V_STRIDE), vb = at_smem<uint2>(tile, at + (row + 1) * L::V_STRIDE);
               const uint2 vc = at_smem<uint2>(tile, at + (row + 8) * L::V_STRIDE), vd = at_smem<uint2>(tile, at + (row + 9) * L::V_STRIDE);
@@ -623,8 +819,9 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attention8_kernel(Params p, 
             } else {
 #pragma unroll
               for (int h = 0; h < D / 128; ++h) {
-                const uint4 va = at_smem<uint4>(tile, L::v_at(row, g + 8 * h)), vb = at_smem<uint4>(tile, L::v_at(row + 1, g + 8 * h));
-                const uint4 vc = at_smem<uint4>(tile, L::v_at(row + 8, g + 8 * h)), vd = at_smem<uint4>(tile, L::v_at(row + 9, g + 8 * h));
+                const int at = v_lane + h * 128 + 16 * t * D, next = (v_lane ^ 16) + h * 128 + (16 * t + 1) * D;
+                const uint4 va = at_smem<uint4>(tile, at), vb = at_smem<uint4>(tile, next);
+                const uint4 vc = at_smem<uint4>(tile, at + 8 * D), vd = at_smem<uint4>(tile, next + 8 * D);
                 const uint32_t w0[4] = {va.x, va.y, va.z, va.w}, w1[4] = {vb.x, vb.y, vb.z, vb.w};
                 const uint32_t w2[4] = {vc.x, vc.y, vc.z, vc.w}, w3[4] = {vd.x, vd.y, vd.z, vd.w};
 #pragma unroll
@@ -654,16 +851,12 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attention8_kernel(Params p, 
       const bool final = run.left <= run.units + RANGE_COST - run.c;  // no other range follows
       float* part = sums;
       if (!whole) {
+        const Piece piece{place0, static_cast<int>(row0), nheads, run.units, run.c == 0, run.c + length == run.units};
         if (final) {
-          mine.place = place0;
-          mine.row = static_cast<int>(row0);
-          mine.heads = nheads;
-          mine.last = owner_of(place0 + run.units - 1, total, warps);
-          mine.begins = run.c == 0;
-          mine.ends = run.c + length == run.units;
-        } else {
-          part = p.part + static_cast<int64_t>(me) * 2 * HEADS * part_stride(D);  // part 0: it ends its range
-          shared.kept = 1;
+          mine = piece;
+        } else {  // part 0: it ends its range
+          part = part_of<D, HEADS>(p, me, 0);
+          ended = piece;
         }
       }
 #pragma unroll
@@ -698,143 +891,120 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attention8_kernel(Params p, 
           }
         }
     place0 += run.units + RANGE_COST;
-    next_range<D>(p, run, tiles);
+    next_range<D>(p, run);
   }
 
-  // ---- the warps' last ranges: neighbours that hold parts of one range join them.
-  if (lane == 0) s_last[warp] = mine;
+  // ---- the warps' last ranges: neighbours that hold parts of one range join them, in the output
+  // if they hold it all.
+  if (lane == 0) {
+    s_last[warp] = mine;
+    s_ended[warp] = ended;
+    s_place[warp] = mine.heads > 0 ? mine.place : ~uint32_t(warp);  // no place: unlike any other
+    s_join[2 * warp] = s_join[2 * warp + 1] = 0;
+  }
   __syncthreads();
+  const int me0 = me - warp;
+  const uint4 places = *reinterpret_cast<const uint4*>(s_place);
+  // Bit w: warp w's last range is that of the warp before.
+  const uint32_t joined = (places.x == places.y ? 2u : 0u) | (places.y == places.z ? 4u : 0u) | (places.z == places.w ? 8u : 0u);
+#pragma unroll 1
   for (int w = 0; w < WARPS;) {
-    const Last first = s_last[w];
-    int end = w + 1;  // behind the warps that share it
-    if (first.place < 0) {
-      ++w;
-      continue;
-    }
-    while (end < WARPS && s_last[end].place == first.place) ++end;
-    const bool whole = first.begins && s_last[end - 1].ends;
-    for (int h = warp; h < first.heads; h += WARPS) {
-      constexpr int V = D / 32;  // neighbouring dimensions of a lane
-      float m = NONE, mo = NONE, l = 0.f, v[V];
+    const int end = __ffs(~joined & (~1u << w)) - 1;  // behind the warps that share it
+    const int heads = s_last[w].heads;
+    const bool begins = s_last[w].begins, whole = begins && s_last[end - 1].ends;
+#pragma unroll 1
+    for (int h = threadIdx.x >> 4; h < heads; h += THREADS / 16) {
+      Sums<D> sums{};
+      sums.start();
+      float4 st[WARPS];
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[j] = 0.f;
-      const auto row = [&](int i) {
-        return reinterpret_cast<const float*>(smem + i * (STAGES * L::STAGE)) + h * part_stride(D);
-      };
-      for (int i = w; i < end; ++i) {
-        m = fmaxf(m, row(i)[D]);
-        mo = fmaxf(mo, row(i)[D + 1]);
+      for (int i = 0; i < WARPS; ++i) {
+        const float* row = reinterpret_cast<const float*>(smem + min(w + i, end - 1) * (STAGES * L::STAGE)) + h * part_stride(D);
+        st[i] = *reinterpret_cast<const float4*>(row + D);
       }
-      for (int i = w; i < end; ++i) {
-        l = fmaf(row(i)[D + 2], ex2_approx(row(i)[D] - m), l);
-        const float f = ex2_approx(row(i)[D + 1] - mo);
+      float bm = NONE, bo = NONE;
 #pragma unroll
-        for (int j = 0; j < V; j += 2) {
-          const float2 x = *reinterpret_cast<const float2*>(row(i) + V * lane + j);
-          v[j] = fmaf(x.x, f, v[j]);
-          v[j + 1] = fmaf(x.y, f, v[j + 1]);
+      for (int i = 0; i < WARPS; ++i) {
+        bm = fmaxf(bm, st[i].x);
+        bo = fmaxf(bo, st[i].y);
+      }
+      sums.raise(bm, bo);
+#pragma unroll
+      for (int i = 0; i < WARPS; ++i) {
+        if (w + i < end) {
+          const float* row = reinterpret_cast<const float*>(smem + (w + i) * (STAGES * L::STAGE)) + h * part_stride(D);
+          float x[Sums<D>::V];
+          Sums<D>::load(x, row, lane & 15);
+          sums.l = fmaf(st[i].z, ex2_approx(st[i].x - bm), sums.l);
+          sums.add(x, ex2_approx(st[i].y - bo));
         }
       }
       if (whole) {
-        write_lane<V>(p, (static_cast<int64_t>(first.row) + h) * D + V * lane, v, last_factor(m, mo, l));
+        sums.write(p, static_cast<int64_t>(s_last[w].row) + h, lane & 15);
       } else {
-        float* part = p.part + ((static_cast<int64_t>(me - warp + w) * 2 + (first.begins ? 1 : 0)) * HEADS + h) * part_stride(D);
-#pragma unroll
-        for (int j = 0; j < V; j += 2) *reinterpret_cast<float2*>(part + V * lane + j) = make_float2(v[j], v[j + 1]);
-        if (lane == 0) *reinterpret_cast<float4*>(part + D) = make_float4(m, mo, l, 0.f);
-      }
-    }
-    if (warp == w && !whole) {
-      if (first.begins) {
-        shared.row = first.row;
-        shared.heads = first.heads;
-        shared.last = first.last;
-      } else {
-        shared.kept = 1;
+        sums.store(part_of<D, HEADS>(p, me0 + w, begins) + h * part_stride(D), lane & 15);
       }
     }
     w = end;
   }
-  if (lane == 0) p.shared[me] = shared;
-}
 
-// Joins the parts of the ranges that several CTAs of the attention shared.  One CTA for those
-// that CTA blockIdx.x began, a warp for each head; the parts in order of their CTAs.
-constexpr int JOIN_THREADS = 256;
-
-template <int D>
-__global__ void __launch_bounds__(JOIN_THREADS, 4) paged_attention8_join_kernel(Params p) {
-  constexpr int V = D / 32;              // neighbouring dimensions of a lane
-  constexpr int AHEAD = D == 256 ? 4 : 8;  // parts whose sums are loaded together
-  pdl_begin();
-  const int lane = threadIdx.x & 31;
-  const int4* const all = reinterpret_cast<const int4*>(p.shared);
-  const int64_t part_floats = static_cast<int64_t>(p.tile_heads) * part_stride(D);
-  int4 info[WARPS];
-#pragma unroll
-  for (int w = 0; w < WARPS; ++w) info[w] = __ldg(all + blockIdx.x * WARPS + w);
-#pragma unroll
-  for (int w = 0; w < WARPS; ++w) {
-    const Shared shared{info[w].x, info[w].y, info[w].z, info[w].w};
-    if (shared.heads == 0) continue;
-    // The part that begins the range, one of each later CTA's first warp, and one of the
-    // warp that ends it where that is no CTA's first and did not join its neighbours.
-    const int ctas = shared.last / WARPS - static_cast<int>(blockIdx.x);
-    const int n = 1 + ctas + (shared.last % WARPS != 0 && __ldg(all + shared.last).w != 0 ? 1 : 0);
-    const float* const first = p.part + (static_cast<int64_t>(blockIdx.x) * WARPS + w) * 2 * part_floats + part_floats;
-    for (int h = threadIdx.x >> 5; h < shared.heads; h += JOIN_THREADS / 32) {
-      const auto row = [&](int i) -> const float* {
-        if (i == 0) return first + h * part_stride(D);
-        const int64_t from = i <= ctas ? (static_cast<int64_t>(blockIdx.x) + i) * WARPS : shared.last;
-        return p.part + from * 2 * part_floats + h * part_stride(D);
-      };
-      float m = NONE, mo = NONE, l = 0.f, v[V];
-#pragma unroll
-      for (int j = 0; j < V; ++j) v[j] = 0.f;
-      for (int i0 = 0; i0 < n; i0 += 32) {  // a lane for the statistics of each of 32 parts
-        const int count = min(32, n - i0);
-        float4 st = make_float4(NONE, NONE, 0.f, 0.f);
-        if (lane < count) st = *reinterpret_cast<const float4*>(row(i0 + lane) + D);
-        float bm = fmaxf(m, st.x), bo = fmaxf(mo, st.y);
-#pragma unroll
-        for (int x = 16; x > 0; x >>= 1) {
-          bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, x));
-          bo = fmaxf(bo, __shfl_xor_sync(0xffffffffu, bo, x));
-        }
-        float dl = st.z * ex2_approx(st.x - bm);
-#pragma unroll
-        for (int x = 16; x > 0; x >>= 1) dl += __shfl_xor_sync(0xffffffffu, dl, x);
-        l = fmaf(l, ex2_approx(m - bm), dl);
-        const float fo = ex2_approx(mo - bo), fi = ex2_approx(st.y - bo);
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[j] *= fo;
-        m = bm;
-        mo = bo;
-        for (int j0 = 0; j0 < count; j0 += AHEAD) {
-          float x[AHEAD][V];
-#pragma unroll
-          for (int j = 0; j < AHEAD; ++j) {
-            const float* from = row(i0 + min(j0 + j, count - 1)) + V * lane;
-#pragma unroll
-            for (int k = 0; k < V; k += 2) {
-              const float2 y = *reinterpret_cast<const float2*>(from + k);
-              x[j][k] = y.x;
-              x[j][k + 1] = y.y;
-            }
-          }
-#pragma unroll
-          for (int j = 0; j < AHEAD; ++j) {
-            const float f = __shfl_sync(0xffffffffu, fi, (j0 + j) & 31);
-            if (j0 + j < count) {
-#pragma unroll
-              for (int k = 0; k < V; ++k) v[k] = fmaf(x[j][k], f, v[k]);
-            }
-          }
-        }
-      }
-      write_lane<V>(p, (static_cast<int64_t>(shared.row) + h) * D + V * lane, v, last_factor(m, mo, l));
+  // ---- ranges that several CTAs, or this one through the workspace, hold parts of.  Every CTA
+  // counts its parts in; the last to come joins them all, in their order.  Lane 2 w + k of
+  // warp 0 stands for part k of warp w.
+  bool stands = false;
+  uint64_t seen = 0;
+  uint64_t* word = nullptr;
+  int count = 0;
+  uint32_t place = 0;
+  if (warp == 0 && lane < 2 * WARPS) {
+    const int w = lane >> 1, k = lane & 1;
+    const bool first = (joined >> w & 1u) == 0;  // of its neighbours
+    const int end = __ffs(~joined & (~1u << w)) - 1;
+    const Piece& last = s_last[w];
+    const Piece& over = s_ended[w];
+    const bool in_ended = k == 0 && over.heads > 0;
+    stands = in_ended || (first && last.heads > 0 && last.begins == k && !(last.begins && s_last[end - 1].ends));
+    if (stands) {
+      place = in_ended ? over.place : last.place;
+      const Parts parts(place, in_ended ? over.units : last.units, shares);
+      count = parts.count;
+      word = p.arrivals + parts.begin;
+      seen = *reinterpret_cast<volatile uint64_t*>(word);
     }
   }
+  if (!__syncthreads_or(stands)) return;
+  bool last_here = false;
+  if (stands) {
+    const uint32_t same = __match_any_sync(__activemask(), place);  // this CTA's parts of one range
+    if (lane == __ffs(same) - 1) {
+      fence_gpu();  // the CTA's parts before their count
+      if (arrive(word, seen, p.tag, __popc(same), count)) {
+        fence_gpu();  // the count before the parts
+        s_join[lane] = 1;
+        last_here = true;
+      }
+    }
+  }
+  if (!__syncthreads_or(last_here)) return;
+#pragma unroll 1
+  for (int i = 0; i < 2 * WARPS; ++i) {
+    if (s_join[i] == 0) continue;
+    const Piece piece = (i & 1) == 0 && s_ended[i >> 1].heads > 0 ? s_ended[i >> 1] : s_last[i >> 1];
+    const Parts parts(piece.place, piece.units, shares);
+#pragma unroll 1
+    for (int h = threadIdx.x >> 4; h < piece.heads; h += THREADS / 16)
+      join_head<D, HEADS>(p, parts, static_cast<int64_t>(piece.row) + h, h, lane & 15);
+  }
+}
+
+// A number that no workspace holds by chance: a count of the launches, spread over 64 bits by
+// an odd factor (2^64 over the golden ratio), from a start that differs from process to
+// process.
+uint64_t next_tag() {
+  static const uint64_t start = static_cast<uint64_t>(std::chrono::steady_clock::now().time_since_epoch().count()) << 20;
+  static std::atomic<uint64_t> launches{1};
+  const uint64_t x = (start + launches.fetch_add(1, std::memory_order_relaxed)) * 0x9E3779B97F4A7C15ull & ~uint64_t{0xFFFF};
+  return x != 0 ? x : 0x10000;
 }
 
 struct Plan {
@@ -868,20 +1038,14 @@ rk_status launch(const Params& p, const KernelCtl& ctl, cudaStream_t s) {
   }
   const int64_t ranges = static_cast<int64_t>(p.batch) * p.hkv * p.head_groups;
   const int64_t per_range = (static_cast<int64_t>(p.max_blocks) * p.block_size + unit_of(D) - 1) / unit_of(D);
-  // A warp counts its places, and a sequence's over its heads, in 32 bits.
-  if (static_cast<int64_t>(p.hkv) * p.head_groups > INT32_MAX / (per_range + RANGE_COST) ||
-      ranges > (int64_t{1} << 38) / (per_range + RANGE_COST))
-    return RK_ERR_UNSUPPORTED;
+  // Places are counted in 32 bits.
+  if (ranges > UINT32_MAX / (per_range + RANGE_COST + 1)) return RK_ERR_UNSUPPORTED;
   int64_t ctas = static_cast<int64_t>(device_sm_count()) * (resident < MAX_CTAS_PER_SM ? resident : MAX_CTAS_PER_SM);
   // Not more warps than units; RANGE_COST places of a range hold none.
   if (ranges <= ctas * WARPS && ranges * (per_range + RANGE_COST) < ctas * WARPS)
     ctas = (ranges * (per_range + RANGE_COST) + WARPS - 1) / WARPS;
   e = launch_kernel(kernel, dim3(static_cast<unsigned>(ctas)), dim3(THREADS), SMEM, s, 0, p, ctl);
   note_launch("paged_attention8_kernel");
-  if (e == cudaSuccess && per_range > 1) {
-    e = launch_kernel(paged_attention8_join_kernel<D>, dim3(static_cast<unsigned>(ctas)), dim3(JOIN_THREADS), 0, s, 0, p);
-    note_launch("paged_attention8_join_kernel");
-  }
   return cuda_status(e);
 }
 
@@ -899,7 +1063,7 @@ rk_status launch_d(const Params& p, int64_t head_dim, int nt, const KernelCtl& c
 size_t paged_attention8_workspace_bytes(int64_t hq, int64_t hkv, int64_t head_dim) {
   const pa8::Plan pl = pa8::plan(hq, hkv, head_dim);
   const size_t warps = static_cast<size_t>(device_sm_count()) * pa8::MAX_CTAS_PER_SM * pa8::WARPS;
-  return warps * (sizeof(pa8::Shared) + 2 * 8 * pl.nt * pa8::part_stride(static_cast<int>(head_dim)) * sizeof(float));
+  return warps * (sizeof(uint64_t) + 2 * 8 * pl.nt * pa8::part_stride(static_cast<int>(head_dim)) * sizeof(float));
 }
 
 rk_status paged_attention8_launch(const PagedAttention8Args& a, void* workspace, size_t workspace_bytes, cudaStream_t s) {
@@ -919,8 +1083,9 @@ rk_status paged_attention8_launch(const PagedAttention8Args& a, void* workspace,
   p.tables = a.block_tables;
   p.lens = a.context_lengths;
   p.out = a.out;
-  p.shared = static_cast<pa8::Shared*>(workspace);
-  p.part = reinterpret_cast<float*>(p.shared + device_sm_count() * pa8::MAX_CTAS_PER_SM * pa8::WARPS);
+  p.arrivals = static_cast<uint64_t*>(workspace);
+  p.part = reinterpret_cast<float*>(p.arrivals + device_sm_count() * pa8::MAX_CTAS_PER_SM * pa8::WARPS);
+  p.tag = pa8::next_tag();
   p.batch = static_cast<int>(a.batch);
   p.hq = static_cast<int>(a.hq);
   p.hkv = static_cast<int>(a.hkv);
@@ -930,9 +1095,10 @@ rk_status paged_attention8_launch(const PagedAttention8Args& a, void* workspace,
   p.num_blocks = static_cast<int>(a.num_blocks);
   p.block_size = static_cast<int>(a.block_size);
   p.max_blocks = static_cast<int>(a.max_blocks);
-  p.block_shift = -1;
-  for (int i = 0; i < 31; ++i)
-    if ((int64_t{1} << i) == a.block_size) p.block_shift = i;
+  int bits = 0;  // of block_size, rounded up to a power of two
+  while ((int64_t{1} << bits) < a.block_size) ++bits;
+  p.block_shift = 31 + bits;
+  p.block_multiplier = static_cast<uint32_t>((uint64_t{1} << p.block_shift) / static_cast<uint64_t>(a.block_size) + 1);
   p.index_bits = a.index_bits;
   p.bf16 = a.dt == RK_DTYPE_BF16;
   p.scale_log2 = a.scale * 1.44269504088896340736f;
