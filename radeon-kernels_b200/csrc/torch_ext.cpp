@@ -14,6 +14,7 @@
 //   gemm(a, b, variant) -> new tensor
 //   gemm_views(a, b, out=None, variant) -> C   (transposed views in place: rk_gemm_layout)
 //   gemv_*(input, weight) -> new tensor   (native_gemv.hip:343-391)
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
@@ -436,9 +437,9 @@ at::Tensor vector_rows(const at::Tensor& t, const char* name) {
 }
 
 // Rotary positions (rk_rotary_embedding): new dense [query_out, key_out].
-std::vector<at::Tensor> rotary_embedding(const at::Tensor& query_in, const at::Tensor& key_in,
-                                         const at::Tensor& positions_in, const at::Tensor& frequencies_in,
-                                         bool interleaved, double amplitude, bool inverse) {
+std::vector<at::Tensor> rotary_forward(const at::Tensor& query_in, const at::Tensor& key_in,
+                                       const at::Tensor& positions_in, const at::Tensor& frequencies_in,
+                                       bool interleaved, double amplitude, bool inverse) {
   TORCH_CHECK(query_in.is_cuda(), "query must be a CUDA tensor");
   c10::cuda::CUDAGuard guard(query_in.device());
   const at::Tensor query = strided_rows(query_in, "query"), key = strided_rows(key_in, "key");
@@ -454,6 +455,7 @@ std::vector<at::Tensor> rotary_embedding(const at::Tensor& query_in, const at::T
   TORCH_CHECK(key.size(0) == query.size(0) && key.size(2) == query.size(2),
               "query and key must share tokens and head_dim");
   TORCH_CHECK(positions.size(0) == query.size(0), "positions must hold one position per token");
+  TORCH_CHECK(!frequencies.requires_grad(), "frequencies must not require gradients");
   auto query_out = at::empty(query.sizes(), query.options());
   auto key_out = at::empty(key.sizes(), key.options());
   check_status(rk_rotary_embedding(query.data_ptr(), key.data_ptr(), positions.data_ptr(),
@@ -464,6 +466,40 @@ std::vector<at::Tensor> rotary_embedding(const at::Tensor& query_in, const at::T
                                    current_stream(query)),
                "rk_rotary_embedding");
   return {query_out, key_out};
+}
+
+std::vector<at::Tensor> rotary_embedding(const at::Tensor& query, const at::Tensor& key, const at::Tensor& positions,
+                                         const at::Tensor& frequencies, bool interleaved, double amplitude, bool inverse);
+
+// A rotation is linear in queries and keys: its gradient is the inverse rotation, which is this
+// function again, so gradients of gradients work too.
+struct RotaryFunction : public torch::autograd::Function<RotaryFunction> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& query,
+                                                const at::Tensor& key, const at::Tensor& positions,
+                                                const at::Tensor& frequencies, bool interleaved, double amplitude,
+                                                bool inverse) {
+    ctx->save_for_backward({positions, frequencies});
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["amplitude"] = amplitude;
+    ctx->saved_data["inverse"] = inverse;
+    at::AutoDispatchBelowADInplaceOrView below;
+    return rotary_forward(query, key, positions, frequencies, interleaved, amplitude, inverse);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    auto out = rotary_embedding(grads[0], grads[1], saved[0], saved[1], ctx->saved_data["interleaved"].toBool(),
+                                ctx->saved_data["amplitude"].toDouble(), !ctx->saved_data["inverse"].toBool());
+    const at::Tensor none;
+    return {out[0], out[1], none, none, none, none, none};
+  }
+};
+
+std::vector<at::Tensor> rotary_embedding(const at::Tensor& query, const at::Tensor& key, const at::Tensor& positions,
+                                         const at::Tensor& frequencies, bool interleaved, double amplitude, bool inverse) {
+  if (at::GradMode::is_enabled() && (query.requires_grad() || key.requires_grad()))
+    return RotaryFunction::apply(query, key, positions, frequencies, interleaved, amplitude, inverse);
+  return rotary_forward(query, key, positions, frequencies, interleaved, amplitude, inverse);
 }
 
 // Slot map of one step (rk_paged_slots): block_tables in place, new [slot_mapping, positions,
@@ -491,6 +527,31 @@ std::vector<at::Tensor> paged_slots(at::Tensor block_tables, const at::Tensor& c
                               block_size, free_blocks.size(0), num_tokens, bits, current_stream(block_tables)),
                "rk_paged_slots");
   return {slots, positions, lengths, used};
+}
+
+// Scratch of one call: from the caching allocator on the call's stream, and back to it when
+// the call has been issued, as a temporary tensor would be (a captured graph keeps it).
+class Scratch {
+ public:
+  Scratch(size_t bytes, rk_stream_t stream)
+      : bytes_(bytes),
+        data_(bytes > 0 ? c10::cuda::CUDACachingAllocator::raw_alloc_with_stream(bytes, reinterpret_cast<cudaStream_t>(stream))
+                        : nullptr) {}
+  ~Scratch() {
+    if (data_ != nullptr) c10::cuda::CUDACachingAllocator::raw_delete(data_);
+  }
+  Scratch(const Scratch&) = delete;
+  Scratch& operator=(const Scratch&) = delete;
+  void* data() const { return data_; }
+  size_t bytes() const { return bytes_; }
+
+ private:
+  size_t bytes_;
+  void* data_;
+};
+
+void check_no_grad(std::initializer_list<const at::Tensor*> tensors) {
+  for (const at::Tensor* t : tensors) TORCH_CHECK(!t->requires_grad(), "inference only: no input may require gradients");
 }
 
 rk_cache_dtype cache_dtype_of(const at::Tensor& t, const char* name) {
@@ -525,6 +586,7 @@ std::vector<at::Tensor> paged_cache_append_8bit(const at::Tensor& key_in, const 
                                                 at::Tensor value_scales, const at::Tensor& slot_mapping) {
   TORCH_CHECK(key_in.is_cuda(), "key must be a CUDA tensor");
   c10::cuda::CUDAGuard guard(key_in.device());
+  check_no_grad({&key_in, &value_in, &key_cache, &value_cache, &key_scales, &value_scales});
   const at::Tensor key = vector_rows(key_in, "key"), value = vector_rows(value_in, "value");
   TORCH_CHECK(key.scalar_type() == value.scalar_type(), "key and value must share a dtype");
   TORCH_CHECK(key.sizes() == value.sizes() && key.device() == value.device(),
@@ -538,14 +600,14 @@ std::vector<at::Tensor> paged_cache_append_8bit(const at::Tensor& key_in, const 
   size_t ws_bytes = 0;
   check_status(rk_paged_cache_append_8bit_workspace_size(key.size(0), key_cache.size(0), &ws_bytes),
                "rk_paged_cache_append_8bit_workspace_size");
-  at::Tensor ws;
-  if (ws_bytes > 0) ws = at::empty({static_cast<int64_t>(ws_bytes)}, key.options().dtype(at::kByte));
+  const rk_stream_t stream = current_stream(key);
+  const Scratch ws(ws_bytes, stream);
   check_status(rk_paged_cache_append_8bit(
                    key.data_ptr(), value.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
                    key_scales.data_ptr<float>(), value_scales.data_ptr<float>(), slot_mapping.data_ptr(), key.size(0),
                    key.size(1), key.size(2), key_cache.size(0), key_cache.size(1), key.stride(0), key.stride(1),
                    value.stride(0), value.stride(1), dtype_of(key, "key"), cache_dtype_of(key_cache, "key_cache"), bits,
-                   ws_bytes > 0 ? ws.data_ptr() : nullptr, ws_bytes, current_stream(key)),
+                   ws.data(), ws.bytes(), stream),
                "rk_paged_cache_append_8bit");
   return {key_cache, value_cache, key_scales, value_scales};
 }
@@ -557,6 +619,7 @@ at::Tensor paged_attention_decode_8bit(const at::Tensor& query_in, const at::Ten
                                        const at::Tensor& context_lengths, double scale) {
   check_rows(query_in, "query", 3);
   c10::cuda::CUDAGuard guard(query_in.device());
+  check_no_grad({&query_in, &key_cache, &value_cache, &key_scales, &value_scales});
   const at::Tensor query = aligned(query_in, 8) ? query_in : query_in.clone();
   check_cache8(key_cache, value_cache, key_scales, value_scales, query.device());
   const int bits = index_bits_of(block_tables, "block_tables", 2);
@@ -570,13 +633,14 @@ at::Tensor paged_attention_decode_8bit(const at::Tensor& query_in, const at::Ten
   size_t ws_bytes = 0;
   check_status(rk_paged_attention_decode_8bit_workspace_size(query.size(1), key_cache.size(2), query.size(2), &ws_bytes),
                "rk_paged_attention_decode_8bit_workspace_size");
-  auto ws = at::empty({static_cast<int64_t>(ws_bytes)}, query.options().dtype(at::kByte));
+  const rk_stream_t stream = current_stream(query);
+  const Scratch ws(ws_bytes, stream);
   check_status(rk_paged_attention_decode_8bit(
                    query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), key_scales.data_ptr<float>(),
                    value_scales.data_ptr<float>(), block_tables.data_ptr(), context_lengths.data_ptr(), out.data_ptr(),
                    query.size(0), query.size(1), key_cache.size(2), query.size(2), key_cache.size(0), key_cache.size(1),
                    block_tables.size(1), static_cast<float>(scale), dtype_of(query, "query"),
-                   cache_dtype_of(key_cache, "key_cache"), bits, ws.data_ptr(), ws_bytes, current_stream(query)),
+                   cache_dtype_of(key_cache, "key_cache"), bits, ws.data(), ws.bytes(), stream),
                "rk_paged_attention_decode_8bit");
   return out;
 }

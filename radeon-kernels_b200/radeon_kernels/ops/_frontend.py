@@ -126,39 +126,28 @@ def dispatch(
     )
 
 
-def cached_call(
-    runtime: Any,
-    operator: str,
-    tensors: Sequence[Any],
-    scalars: Sequence[Any],
-    resolve: Callable[[Sequence[Any], Sequence[Any]], Sequence[Any]] | None = None,
-) -> tuple[Any, Any]:
-    """(key, result) of a call: the result of the winner that served a call of the same kind
-    before -- the same shapes, strides, dtypes, devices, gradient flags and scalars, so every
-    check of the front-end would pass again -- or None where there was none.  The key is for
-    :func:`remember_call`; it is None where the runtime keeps no calls or an argument is no
-    tensor.  The entrypoint's arguments are the tensors and scalars, or ``resolve`` of them."""
+def quick_call(runtime: Any, key: Any, arguments: Sequence[Any]) -> Any:
+    """The result of the winner that served an earlier call with ``key``, or None.
 
-    find = getattr(runtime, "fast_find", None)
-    if find is None:
-        return None, None
-    try:
-        key = (operator, tuple([(t.shape, t.stride(), t.dtype, t.device, t.requires_grad) for t in tensors]),
-               tuple([(type(s), s) for s in scalars]))
-        cached = find(key)
-    except Exception:  # not tensors, or scalars that cannot be a key: the checks say so
-        return None, None
+    The key holds all that the operator's dispatch signature is made of, so the choice of the
+    winner stands.  The winner's entrypoint checks the arguments itself, before it launches
+    anything; where it refuses them, the front-end's checks run after all and say so in
+    their words."""
+
+    cached = runtime.fast_find(key)
     if cached is None:
-        return key, None
-    arguments = (*tensors, *scalars) if resolve is None else resolve(tensors, scalars)
-    return key, runtime.fast_run(cached, arguments)
+        return None
+    try:
+        return runtime.fast_run(cached, arguments)
+    except (RuntimeError, TypeError, ValueError):
+        return None
 
 
 def remember_call(runtime: Any, key: Any, operator: str, device_index: int, signature: Mapping[str, Any]) -> None:
-    """Lets later calls with ``key`` go straight to the winner that ``signature`` selected, if it did."""
+    """Lets :func:`quick_call` with ``key`` use the winner that ``signature`` selected, if it did."""
 
     if key is not None:
         runtime.fast_alias(key, runtime.fast_key(operator, device_index, signature))
 
 
-__all__ = ["Args", "cached_call", "dispatch", "remember_call"]
+__all__ = ["Args", "dispatch", "quick_call", "remember_call"]

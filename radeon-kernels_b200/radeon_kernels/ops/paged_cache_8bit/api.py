@@ -32,7 +32,7 @@ from __future__ import annotations
 from typing import Any
 
 from radeon_kernels.ops._common import torch_runtime
-from radeon_kernels.ops._frontend import Args, cached_call, dispatch, remember_call
+from radeon_kernels.ops._frontend import Args, dispatch, quick_call, remember_call
 from radeon_kernels.ops._runtime import OperatorRuntime, default_operator_runtime
 from radeon_kernels.providers import cuda_builtin
 
@@ -66,11 +66,7 @@ def _check_cache(args: Args) -> tuple[str, tuple[int, ...]]:
 
 
 def _execute_append(key: Any, value: Any, key_cache: Any, value_cache: Any, key_scales: Any, value_scales: Any,
-                    slot_mapping: Any, *, torch_module: Any, runtime: OperatorRuntime) -> Any:
-    tensors = (key, value, key_cache, value_cache, key_scales, value_scales, slot_mapping)
-    call, result = cached_call(runtime, "paged_cache_append_8bit", tensors, ())
-    if result is not None:
-        return tuple(result)
+                    slot_mapping: Any, *, torch_module: Any, runtime: OperatorRuntime, key_of_call: Any = None) -> Any:
     args = Args("paged_cache_append_8bit", torch_module, key=key, value=value, key_cache=key_cache,
                 value_cache=value_cache, key_scales=key_scales, value_scales=value_scales, slot_mapping=slot_mapping)
     args.tensors(key=3, value=3).alike("key", "value")
@@ -99,17 +95,13 @@ def _execute_append(key: Any, value: Any, key_cache: Any, value_cache: Any, key_
         native_arguments=(key, value, key_cache, value_cache, key_scales, value_scales, slot_mapping),
         fallback=cuda_builtin.paged_cache_append_8bit, fallback_selected=cuda_builtin.SELECTED_PAGED_APPEND_8BIT,
     )
-    remember_call(runtime, call, "paged_cache_append_8bit", context.device_index, signature)
+    remember_call(runtime, key_of_call, "paged_cache_append_8bit", context.device_index, signature)
     return tuple(result)
 
 
 def _execute_attention(query: Any, key_cache: Any, value_cache: Any, key_scales: Any, value_scales: Any,
                        block_tables: Any, context_lengths: Any, scale: float | None = None, *, torch_module: Any,
-                       runtime: OperatorRuntime) -> Any:
-    tensors = (query, key_cache, value_cache, key_scales, value_scales, block_tables, context_lengths)
-    call, result = cached_call(runtime, "paged_attention_decode_8bit", tensors, (scale,), resolve=_with_scale)
-    if result is not None:
-        return result
+                       runtime: OperatorRuntime, key_of_call: Any = None) -> Any:
     args = Args("paged_attention_decode_8bit", torch_module, query=query, key_cache=key_cache, value_cache=value_cache,
                 key_scales=key_scales, value_scales=value_scales, block_tables=block_tables,
                 context_lengths=context_lengths)
@@ -142,29 +134,42 @@ def _execute_attention(query: Any, key_cache: Any, value_cache: Any, key_scales:
         fallback=cuda_builtin.paged_attention_decode_8bit,
         fallback_selected=cuda_builtin.SELECTED_PAGED_ATTENTION_8BIT,
     )
-    remember_call(runtime, call, "paged_attention_decode_8bit", context.device_index, signature)
+    remember_call(runtime, key_of_call, "paged_attention_decode_8bit", context.device_index, signature)
     return result
-
-
-def _with_scale(tensors: tuple[Any, ...], scalars: tuple[Any, ...]) -> tuple[Any, ...]:
-    """The entrypoint's arguments: a scale of None is 1/sqrt(head_dim)."""
-
-    (scale,) = scalars
-    return (*tensors, float(scale) if scale is not None else tensors[0].shape[2] ** -0.5)
 
 
 def paged_cache_append_8bit(key: Any, value: Any, key_cache: Any, value_cache: Any, key_scales: Any,
                             value_scales: Any, slot_mapping: Any) -> tuple[Any, Any, Any, Any]:
     """Store new keys and values in an 8-bit paged cache, in place; returns caches and scales."""
 
+    runtime, call = default_operator_runtime(), None
+    try:
+        call = ("paged_cache_append_8bit", key.dtype, key.device, key_cache.dtype, key_cache.shape[1:], slot_mapping.dtype)
+        result = quick_call(runtime, call, (key, value, key_cache, value_cache, key_scales, value_scales, slot_mapping))
+        if result is not None:
+            return tuple(result)
+    except AttributeError:
+        call = None  # no tensors: the checks say so
     return _execute_append(key, value, key_cache, value_cache, key_scales, value_scales, slot_mapping,
-                           torch_module=torch_runtime("paged_cache_append_8bit"), runtime=default_operator_runtime())
+                           torch_module=torch_runtime("paged_cache_append_8bit"), runtime=runtime, key_of_call=call)
 
 
 def paged_attention_decode_8bit(query: Any, key_cache: Any, value_cache: Any, key_scales: Any, value_scales: Any,
                                 block_tables: Any, context_lengths: Any, scale: float | None = None) -> Any:
     """Attend one query token per sequence over an 8-bit paged K/V cache."""
 
+    runtime, call = default_operator_runtime(), None
+    if scale is None or type(scale) is float:
+        try:
+            shape = query.shape
+            call = ("paged_attention_decode_8bit", query.dtype, query.device, shape[1:], key_cache.dtype, key_cache.shape[1:],
+                    block_tables.dtype, scale is None)
+            result = quick_call(runtime, call, (query, key_cache, value_cache, key_scales, value_scales, block_tables,
+                                                context_lengths, shape[2] ** -0.5 if scale is None else scale))
+            if result is not None:
+                return result
+        except (AttributeError, IndexError):
+            call = None  # no tensors of the right ranks: the checks say so
     return _execute_attention(query, key_cache, value_cache, key_scales, value_scales, block_tables, context_lengths,
-                              scale, torch_module=torch_runtime("paged_attention_decode_8bit"),
-                              runtime=default_operator_runtime())
+                              scale, torch_module=torch_runtime("paged_attention_decode_8bit"), runtime=runtime,
+                              key_of_call=call)

@@ -30,7 +30,7 @@ from __future__ import annotations
 from typing import Any
 
 from radeon_kernels.ops._common import device_index_of, torch_runtime
-from radeon_kernels.ops._frontend import Args, cached_call, dispatch, remember_call
+from radeon_kernels.ops._frontend import Args, dispatch, quick_call, remember_call
 from radeon_kernels.ops._runtime import OperatorRuntime, default_operator_runtime
 from radeon_kernels.providers import cuda_builtin
 
@@ -38,11 +38,7 @@ MAXIMUM_TOKENS = 2**31 - 1
 
 
 def _execute(block_tables: Any, context_lengths: Any, new_lengths: Any, free_blocks: Any, num_tokens: int,
-             block_size: int, *, torch_module: Any, runtime: OperatorRuntime) -> Any:
-    call, result = cached_call(runtime, "paged_slots", (block_tables, context_lengths, new_lengths, free_blocks),
-                               (num_tokens, block_size))
-    if result is not None:
-        return tuple(result)
+             block_size: int, *, torch_module: Any, runtime: OperatorRuntime, key_of_call: Any = None) -> Any:
     args = Args("paged_slots", torch_module, block_tables=block_tables, context_lengths=context_lengths,
                 new_lengths=new_lengths, free_blocks=free_blocks)
     args.indices(block_tables=2, context_lengths=1, new_lengths=1, free_blocks=1)
@@ -64,7 +60,7 @@ def _execute(block_tables: Any, context_lengths: Any, new_lengths: Any, free_blo
         native_arguments=(block_tables, context_lengths, new_lengths, free_blocks, num_tokens, block_size),
         fallback=cuda_builtin.paged_slots, fallback_selected=cuda_builtin.SELECTED_PAGED_SLOTS,
     )
-    remember_call(runtime, call, "paged_slots", device_index, signature)
+    remember_call(runtime, key_of_call, "paged_slots", device_index, signature)
     return tuple(result)
 
 
@@ -72,5 +68,15 @@ def paged_slots(block_tables: Any, context_lengths: Any, new_lengths: Any, free_
                 block_size: int) -> tuple[Any, Any, Any, Any]:
     """Extend the block tables by a step's new blocks and map its tokens to cache slots."""
 
+    runtime, call = default_operator_runtime(), None
+    if type(num_tokens) is int and type(block_size) is int:
+        try:
+            call = ("paged_slots", block_tables.dtype, block_tables.device, block_size)
+            result = quick_call(runtime, call, (block_tables, context_lengths, new_lengths, free_blocks, num_tokens,
+                                                block_size))
+            if result is not None:
+                return tuple(result)
+        except AttributeError:
+            call = None  # no tensor: the checks say so
     return _execute(block_tables, context_lengths, new_lengths, free_blocks, num_tokens, block_size,
-                    torch_module=torch_runtime("paged_slots"), runtime=default_operator_runtime())
+                    torch_module=torch_runtime("paged_slots"), runtime=runtime, key_of_call=call)

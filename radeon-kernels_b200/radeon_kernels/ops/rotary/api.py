@@ -25,7 +25,7 @@ import math
 from typing import Any
 
 from radeon_kernels.ops._common import torch_runtime
-from radeon_kernels.ops._frontend import Args, cached_call, dispatch, remember_call
+from radeon_kernels.ops._frontend import Args, dispatch, quick_call, remember_call
 from radeon_kernels.ops._runtime import OperatorRuntime, default_operator_runtime
 from radeon_kernels.providers import cuda_builtin
 
@@ -35,11 +35,7 @@ SCALINGS = ("none", "linear", "ntk", "yarn")
 
 
 def _execute(query: Any, key: Any, positions: Any, frequencies: Any, interleaved: bool = False,
-             amplitude: float = 1.0, *, torch_module: Any, runtime: OperatorRuntime) -> Any:
-    call, result = cached_call(runtime, "rotary_embedding", (query, key, positions, frequencies),
-                               (interleaved, amplitude))
-    if result is not None:
-        return tuple(result)
+             amplitude: float = 1.0, *, torch_module: Any, runtime: OperatorRuntime, key_of_call: Any = None) -> Any:
     args = Args("rotary_embedding", torch_module, query=query, key=key, positions=positions, frequencies=frequencies)
     args.tensors(query=3, key=3).alike("query", "key").indices(positions=1)
     args.expect(isinstance(frequencies, torch_module.Tensor), "frequencies must be a PyTorch tensor", TypeError)
@@ -72,7 +68,7 @@ def _execute(query: Any, key: Any, positions: Any, frequencies: Any, interleaved
         native_arguments=(query, key, positions, frequencies, interleaved, float(amplitude)),
         fallback=cuda_builtin.rotary_embedding, fallback_selected=cuda_builtin.SELECTED_ROTARY,
     )
-    remember_call(runtime, call, "rotary_embedding", context.device_index, signature)
+    remember_call(runtime, key_of_call, "rotary_embedding", context.device_index, signature)
     return tuple(result)
 
 
@@ -80,8 +76,18 @@ def rotary_embedding(query: Any, key: Any, positions: Any, frequencies: Any, *, 
                      amplitude: float = 1.0) -> tuple[Any, Any]:
     """Rotate queries and keys by their positions; returns new ``(query, key)``."""
 
+    runtime, call = default_operator_runtime(), None
+    if type(amplitude) is float and type(interleaved) is bool:
+        try:
+            call = ("rotary_embedding", query.dtype, query.device, query.shape[1:], key.shape[1], positions.dtype,
+                    frequencies.shape, interleaved, query.requires_grad or key.requires_grad)
+            result = quick_call(runtime, call, (query, key, positions, frequencies, interleaved, amplitude))
+            if result is not None:
+                return tuple(result)
+        except (AttributeError, IndexError):
+            call = None  # no tensors of the right ranks: the checks say so
     return _execute(query, key, positions, frequencies, interleaved, amplitude,
-                    torch_module=torch_runtime("rotary_embedding"), runtime=default_operator_runtime())
+                    torch_module=torch_runtime("rotary_embedding"), runtime=runtime, key_of_call=call)
 
 
 def rotary_frequencies(rotary_dim: int, *, base: float = 10000.0, scaling: str = "none", factor: float = 1.0,

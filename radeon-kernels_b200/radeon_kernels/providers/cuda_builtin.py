@@ -286,49 +286,10 @@ def sdpa(torch_module: Any, query: Any, key: Any, value: Any, is_causal: bool, s
 
 
 # ------------------------------------------------- rotary positions and the 8-bit cache
-_ROTARY_FUNCTION: Any = None
+def rotary_embedding(torch_module: Any, *arguments: Any) -> Any:
+    """rk_rotary_embedding; the binding's autograd node rotates gradients back."""
 
-
-def _rotary_function() -> Any:
-    global _ROTARY_FUNCTION
-    if _ROTARY_FUNCTION is None:
-        import torch
-
-        class _RotaryFunction(torch.autograd.Function):
-            """A rotation is linear in queries and keys: its gradient is the inverse rotation,
-            which is this function again (so gradients of gradients work too)."""
-
-            @staticmethod
-            def forward(ctx: Any, query: Any, key: Any, positions: Any, frequencies: Any, interleaved: bool,
-                        amplitude: float, inverse: bool) -> Any:
-                ctx.save_for_backward(positions, frequencies)
-                ctx.how = (interleaved, amplitude, inverse)
-                return tuple(
-                    _native.extension().rotary_embedding(query, key, positions, frequencies, interleaved, amplitude, inverse)
-                )
-
-            @staticmethod
-            def backward(ctx: Any, grad_query: Any, grad_key: Any) -> Any:
-                interleaved, amplitude, inverse = ctx.how
-                out = _rotate(torch, grad_query, grad_key, *ctx.saved_tensors, interleaved, amplitude, not inverse)
-                return (*out, None, None, None, None, None)
-
-        _ROTARY_FUNCTION = _RotaryFunction
-    return _ROTARY_FUNCTION
-
-
-def _rotate(torch_module: Any, query: Any, key: Any, positions: Any, frequencies: Any, interleaved: bool,
-            amplitude: float, inverse: bool) -> Any:
-    if _needs_grad(torch_module, query, key):
-        return _rotary_function().apply(query, key, positions, frequencies, interleaved, amplitude, inverse)
-    return _native.extension().rotary_embedding(query, key, positions, frequencies, interleaved, amplitude, inverse)
-
-
-def rotary_embedding(torch_module: Any, query: Any, key: Any, positions: Any, frequencies: Any, interleaved: bool,
-                     amplitude: float) -> Any:
-    """rk_rotary_embedding, with the inverse rotation as its gradient."""
-
-    return _rotate(torch_module, query, key, positions, frequencies, interleaved, amplitude, False)
+    return _native.extension().rotary_embedding(*arguments)
 
 
 def paged_slots(torch_module: Any, block_tables: Any, context_lengths: Any, new_lengths: Any, free_blocks: Any,

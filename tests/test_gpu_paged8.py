@@ -625,3 +625,104 @@ def test_a_prefill_and_decode_loop(kind, graph):
         lengths.copy_(got[2])
         free.copy_(torch.roll(free, -used))
     assert device_status() == _native.RK_OK
+
+
+# --------------------------------------------------------------------- many divisions of work
+def _plain64(p):
+    """The definition in float64 on the GPU, sequence by sequence, and the bound of ref.attention."""
+    import torch
+
+    dim, heads = p.query.shape[2], p.caches[0].shape[2]
+    outs, bounds = [], []
+    for b, n in enumerate(p.lengths.tolist()):
+        blocks = p.tables[b, : -(-n // p.size)].long()
+        k, v = [(c.view(torch.uint8)[blocks].view(c.dtype).double() * s[blocks].double()[:, None, :, None])
+                .reshape(-1, heads, dim)[:n] for c, s in zip(p.caches, p.scales)]
+        q = p.query[b].double().view(heads, -1, dim)
+        s = torch.einsum("hgd,thd->hgt", q, k) * dim**-0.5
+        w = torch.softmax(s, -1)
+        outs.append(torch.einsum("hgt,thd->hgd", w, v).reshape(-1, dim))
+        a = torch.einsum("hgt,thd->hgd", w, v.abs())
+        near = (torch.einsum("hgd,thd->hgt", q.abs(), k.abs()) * dim**-0.5).amax(-1, keepdim=True)
+        down = (k.abs().sum(-1).amax(0) * dim**-0.5 * 2.0**-25)[:, None, None] * q.abs().amax(-1, keepdim=True)
+        bound = a * (2.0**-10 + 2 * (near * (dim + 16) * 2.0**-24 + 2.0**-18 + down))
+        bound = bound + n * 2.0**-25 * w.amax(-1, keepdim=True) * v.abs().amax()
+        bounds.append(bound.reshape(-1, dim))
+    out, bound = torch.stack(outs), torch.stack(bounds)
+    return out, bound + out.abs() * ref.HALF_STEP[p.dtype] * (1 + 2.0**-10) + ref.TINY[p.dtype]
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_attention_of_many_lengths(seed):
+    """Random batches: every way in which the warps' shares can cut the sequences and heads.  Three
+    calls back to back, the middle one of another batch: workspaces are handed on uncleared."""
+    import torch
+
+    rng = np.random.default_rng(100 + seed)
+    dim = int(rng.choice([64, 128, 256]))
+    kv_heads, group = int(rng.choice([1, 2, 3, 8])), int(rng.choice([1, 4, 5, 8, 12]))
+    batch = int(rng.choice([1, 2, 5, 17, 70, 150]))
+    longest = int(rng.choice([40, 500, 3000, 9000]) if batch < 50 else rng.choice([40, 900]))
+    lengths = np.maximum(1, (longest * rng.random(batch) ** 3)).astype(int).tolist()
+    make = lambda n, s: Problem(n, kv_heads * group, kv_heads, dim, int(rng.choice([8, 16, 32, 20])),  # noqa: E731
+                                str(rng.choice(["bf16", "fp16"])), str(rng.choice(["e4m3", "int8"])),
+                                str(rng.choice(["int32", "int64"])), seed=s)
+    p, other = make(lengths, seed), make(lengths[::-1][: max(1, batch // 2)], seed + 1000)
+    outs = [p.run(), other.run(), p.run(), p.run()]
+    want, bound = _plain64(p)
+    for out in (outs[0], outs[2], outs[3]):
+        assert ((out.double() - want).abs() <= bound).all()
+        assert torch.equal(out, outs[0])
+    want, bound = _plain64(other)
+    assert ((outs[1].double() - want).abs() <= bound).all()
+
+
+def test_refusals_after_calls_of_the_same_kind():
+    """A call that differs from a served one only in what the front-end checks is refused as ever."""
+    import torch
+
+    import radeon_kernels as rk
+
+    p = Problem([70, 3], 8, 2, 128, 16, seed=1)
+    p.run()
+    p.run()
+    args = [p.query, *p.caches, *p.scales, p.tables, p.lengths]
+    for at, bad, error in (
+        (0, p.query[:1], ValueError), (0, p.query.cpu(), ValueError), (0, p.query[None], ValueError),
+        (2, p.caches[1].view(torch.uint8), TypeError), (3, p.scales[0].double(), TypeError), (4, p.scales[1][:-1], ValueError),
+        (5, p.tables.long(), TypeError), (5, p.tables.t().contiguous().t(), ValueError), (6, [3, 4], TypeError),
+        (0, p.query.clone().requires_grad_(True), ValueError), (0, p.query.transpose(0, 1).contiguous().transpose(0, 1), ValueError),
+    ):
+        with pytest.raises(error, match="paged_attention_decode_8bit"):
+            rk.paged_attention_decode_8bit(*args[:at], bad, *args[at + 1 :])
+    for scale, error in ((0.0, ValueError), (float("inf"), ValueError), (-1.0, ValueError), (True, TypeError), ("a", TypeError)):
+        with pytest.raises(error, match="paged_attention_decode_8bit scale"):
+            rk.paged_attention_decode_8bit(*args, scale)
+    rows = torch.zeros((2, 2, 128), dtype=torch.bfloat16, device="cuda")
+    slots = torch.tensor([-1, -1], device="cuda")
+    rk.paged_cache_append_8bit(rows, rows, *p.caches, *p.scales, slots)
+    for bad in ((rows, rows[:1]), (rows.half(), rows), (rows[..., :64], rows[..., :64])):
+        with pytest.raises((ValueError, TypeError), match="paged_cache_append_8bit"):
+            rk.paged_cache_append_8bit(*bad, *p.caches, *p.scales, slots)
+    with pytest.raises(ValueError, match="one slot per token"):
+        rk.paged_cache_append_8bit(rows, rows, *p.caches, *p.scales, slots[:1])
+    lengths = torch.ones(2, dtype=torch.int32, device="cuda")
+    tables = torch.zeros((2, 3), dtype=torch.int32, device="cuda")
+    rk.paged_slots(tables, lengths, lengths, lengths, num_tokens=2, block_size=4)
+    with pytest.raises(TypeError, match="same dtype"):
+        rk.paged_slots(tables, lengths.long(), lengths, lengths, num_tokens=2, block_size=4)
+    with pytest.raises(ValueError, match="num_tokens"):
+        rk.paged_slots(tables, lengths, lengths, lengths, num_tokens=-1, block_size=4)
+    with pytest.raises(TypeError, match="num_tokens"):
+        rk.paged_slots(tables, lengths, lengths, lengths, num_tokens=True, block_size=4)
+    frequencies, positions = rk.rotary_frequencies(128), torch.arange(2, device="cuda")
+    rk.rotary_embedding(rows, rows, positions, frequencies)
+    for changed, error in (
+        ((rows, rows, positions[:1], frequencies), ValueError), ((rows, rows[:1], positions, frequencies), ValueError),
+        ((rows, rows.half(), positions, frequencies), TypeError), ((rows, rows, positions.cpu(), frequencies), ValueError),
+    ):
+        with pytest.raises(error, match="rotary_embedding"):
+            rk.rotary_embedding(*changed)
+    with pytest.raises(TypeError, match="interleaved"):
+        rk.rotary_embedding(rows, rows, positions, frequencies, interleaved=0)
+    device_status()

@@ -10,7 +10,7 @@ import pytest
 
 from fakes import FakeDevice, FakeTensor, FakeTorch
 from radeon_kernels import _native, rotary_frequencies
-from radeon_kernels.ops._frontend import cached_call, remember_call
+from radeon_kernels.ops._frontend import quick_call, remember_call
 from radeon_kernels.ops.paged_cache_8bit.api import _execute_append, _execute_attention
 from radeon_kernels.ops.paged_slots.api import _execute as execute_slots
 from radeon_kernels.ops.rotary.api import _execute as execute_rotary
@@ -202,8 +202,8 @@ def test_frequencies_refuse(changes, error):
 
 # ------------------------------------------------------------------------ the call cache
 class Remembering:
-    def __init__(self):
-        self.calls, self.ran = {}, []
+    def __init__(self, error=None):
+        self.calls, self.ran, self.error = {}, [], error
 
     def fast_key(self, operator, device, signature):
         return operator
@@ -216,30 +216,26 @@ class Remembering:
 
     def fast_run(self, cached, arguments):
         self.ran.append((cached, arguments))
+        if self.error is not None:
+            raise self.error
         return "ran"
 
 
 def test_calls_of_a_kind_go_straight_to_their_winner():
-    torch = pytest.importorskip("torch")
     runtime = Remembering()
-    x = torch.zeros(2, 3)
-    key, result = cached_call(runtime, "op", (x,), (1, 2.0))
-    assert result is None
-    remember_call(runtime, key, "op", 0, {})
-    y = torch.ones(2, 3)
-    assert cached_call(runtime, "op", (y,), (1, 2.0))[1] == "ran"
-    assert runtime.ran[0][1][0] is y and runtime.ran[0][1][1:] == (1, 2.0)
-    # Anything that a check could look at makes another kind.
-    for tensor in (torch.zeros(3, 2), torch.zeros(3, 2).t(), torch.zeros(2, 3, dtype=torch.float64),
-                   torch.zeros(2, 3, requires_grad=True), torch.zeros(2, 6)[:, ::2], torch.zeros(2, 3, device="meta")):
-        assert cached_call(runtime, "op", (tensor,), (1, 2.0))[1] is None
-    for scalars in ((True, 2.0), (1, 2), (1, 2.5), (1.0, 2.0)):
-        assert cached_call(runtime, "op", (x,), scalars)[1] is None
-    assert cached_call(runtime, "other", (x,), (1, 2.0))[1] is None
-    assert cached_call(runtime, "op", ([1],), ()) == (None, None)  # no tensor
-    assert cached_call(runtime, "op", (x,), ([1],)) == (None, None)  # no key
-    assert cached_call(Capture(), "op", (x,), ()) == (None, None)  # a runtime that keeps none
-    remember_call(runtime, None, "op", 0, {})
+    assert quick_call(runtime, ("op", 1), (2, 3)) is None and runtime.ran == []
+    remember_call(runtime, ("op", 1), "op", 0, {})
+    assert quick_call(runtime, ("op", 1), (2, 3)) == "ran" and runtime.ran == [("op", (2, 3))]
+    assert quick_call(runtime, ("op", 2), (2, 3)) is None
+    remember_call(runtime, None, "op", 0, {})  # a call that has no key
+    for error in (RuntimeError("refused"), TypeError("no tensor"), ValueError("bad")):
+        refusing = Remembering(error)
+        remember_call(refusing, ("op", 1), "op", 0, {})
+        assert quick_call(refusing, ("op", 1), ()) is None  # the front-end's checks speak
+    with pytest.raises(KeyboardInterrupt):
+        interrupted = Remembering(KeyboardInterrupt())
+        remember_call(interrupted, ("op", 1), "op", 0, {})
+        quick_call(interrupted, ("op", 1), ())
 
 
 def test_the_call_cache_is_bounded(monkeypatch):
