@@ -500,7 +500,7 @@ RK_API rk_status rk_paged_slots(void* block_tables, const void* context_lengths,
  * written is skipped, and it and slots >= num_blocks * block_size make the next
  * rk_device_status() report RK_ERR_INVALID_ARGUMENT.  head_dim 64, 128 or 256; 1 <=
  * block_size <= 1024; tokens < 2^30.  workspace: rk_paged_cache_append_8bit_workspace_size()
- * bytes, uninitialised.  No counterpart in the reference.
+ * bytes, 16-byte aligned, uninitialised.  No counterpart in the reference.
  */
 RK_API rk_status rk_paged_cache_append_8bit(const void* key, const void* value, void* key_cache,
                                             void* value_cache, float* key_scales,

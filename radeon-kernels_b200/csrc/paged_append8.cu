@@ -34,9 +34,16 @@ namespace {
 
 constexpr int THREADS = 256;
 constexpr int WARPS = THREADS / 32;
-constexpr int SPAN = 64;           // tokens of a CTA at most
-constexpr int SCAN_TOKENS = 2048;  // more tokens than this: claims
+constexpr int SCAN_TOKENS = 2048;  // more tokens than this: a list of runs and claims
 constexpr int HELD = 8;            // 16-byte vectors a lane keeps
+constexpr int APPEND_CTAS = 3;      // resident on an SM
+
+// The tokens of one block: `len` from `token` on, ascending from `offset` to `last` in `block`.
+struct Run {
+  int32_t token, block;
+  int16_t offset, len, last;
+  int16_t rival;  // whether another run of the block is known
+};
 
 struct AppendParams {
   const void* rows[2];  // keys, values
@@ -44,32 +51,118 @@ struct AppendParams {
   uint8_t* cache[2];
   float* scales[2];
   const void* slots;
-  const int32_t* claims;  // per block: the first token of its first run; null: look through the slots
-  int64_t tokens, capacity;  // capacity: num_blocks * block_size
-  int heads, block_size, span, index_bits;
+  int32_t* claims;  // per block: a token that starts a run of it; or anything
+  int32_t* counts;  // per THREADS tokens: the runs that start there,
+  Run* runs;        // listed from the first of those tokens' places on
+  int parts;        // CTAs that share a list
+  int64_t capacity;  // num_blocks * block_size
+  int32_t tokens;
+  int heads, block_size, index_bits;
 };
 
-__device__ __forceinline__ int64_t slot_of(const void* slots, int index_bits, int64_t t) {
-  return index_bits == 32 ? static_cast<int64_t>(static_cast<const int32_t*>(slots)[t])
-                          : static_cast<const int64_t*>(slots)[t];
+__device__ __forceinline__ int64_t slot_of(const AppendParams& p, int64_t t) {
+  return p.index_bits == 32 ? static_cast<int64_t>(static_cast<const int32_t*>(p.slots)[t])
+                            : static_cast<const int64_t*>(p.slots)[t];
+}
+__device__ __forceinline__ int block_of(const AppendParams& p, int64_t slot) {
+  return p.capacity <= INT32_MAX ? static_cast<int>(static_cast<uint32_t>(slot) / static_cast<uint32_t>(p.block_size))
+                                 : static_cast<int>(slot / p.block_size);
 }
 
-// Whether token t starts a run; `slot` is its slot, inside the cache.
-__device__ __forceinline__ bool starts_run(const void* slots, int index_bits, int64_t t, int64_t slot, int block_size) {
-  if (t == 0) return true;
-  const int64_t before = slot_of(slots, index_bits, t - 1);
-  return before < 0 || before >= slot || before / block_size != slot / block_size;
+// Whether a token in `slot`, inside the cache, goes on with the run of one in `before`.
+__device__ __forceinline__ bool goes_on(const AppendParams& p, int64_t before, int64_t slot, int block) {
+  return before >= 0 && before < slot && before >= static_cast<int64_t>(block) * p.block_size;
 }
 
-__global__ void __launch_bounds__(THREADS)
-    append_claim_kernel(const void* slots, int index_bits, int64_t tokens, int64_t capacity, int block_size,
-                        int32_t* claims) {
+// Tokens after `from` that go on with the run of `block`, counted by a warp.
+__device__ __forceinline__ int more_tokens(const AppendParams& p, int64_t from, int block, int lane) {
+  int more = 0;
+  for (;;) {
+    const int64_t t = from + 1 + more + lane;
+    bool on = false;
+    if (t < p.tokens) {
+      const int64_t slot = slot_of(p, t);
+      on = slot < p.capacity && slot < (static_cast<int64_t>(block) + 1) * p.block_size && goes_on(p, slot_of(p, t - 1), slot, block);
+    }
+    const uint32_t off = ~__ballot_sync(0xffffffffu, on);
+    if (off != 0) return more + __ffs(off) - 1;
+    more += 32;  // slots ascend within a block, so this ends after block_size of them
+  }
+}
+
+// Whether `other` is a token that starts a run of `block`.
+__device__ __forceinline__ bool starts_run(const AppendParams& p, int32_t other, int block) {
+  if (other < 0 || other >= p.tokens) return false;
+  const int64_t slot = slot_of(p, other), first = static_cast<int64_t>(block) * p.block_size;
+  return slot >= first && slot < first + p.block_size && !(other > 0 && goes_on(p, slot_of(p, other - 1), slot, block));
+}
+
+// Lists the runs and looks for blocks that have several.  A thread per token.  Each run leaves its
+// token in its block's claim and sees what was there: anything, since nothing clears the
+// claims, or the token of a run that came before it, which the slots tell apart.  Of several
+// runs of a block all but the first to come see another, and the first finds another's token
+// in the claim afterwards.
+__global__ void __launch_bounds__(THREADS) append_runs_kernel(AppendParams p, KernelCtl ctl) {
+  __shared__ uint32_t s_breaks[WARPS];  // tokens that do not go on with the one before
+  __shared__ int s_starts[WARPS];
   pdl_begin();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t t = static_cast<int64_t>(blockIdx.x) * THREADS + threadIdx.x;
-  if (t >= tokens) return;
-  const int64_t slot = slot_of(slots, index_bits, t);
-  if (slot < 0 || slot >= capacity) return;
-  if (starts_run(slots, index_bits, t, slot, block_size)) atomicMin(claims + slot / block_size, static_cast<int32_t>(t));
+  int64_t slot = -1;
+  int block = -1;
+  bool on = false;
+  if (t < p.tokens) {
+    slot = slot_of(p, t);
+    if (slot >= p.capacity) {
+      atomicOr(ctl.status, RK_DEV_ERR_BAD_INDEX);
+      slot = -1;
+    }
+    if (slot >= 0) {
+      block = block_of(p, slot);
+      on = t > 0 && goes_on(p, slot_of(p, t - 1), slot, block);
+    }
+  }
+  const uint32_t breaks = ~__ballot_sync(0xffffffffu, on);
+  if (lane == 0) s_breaks[warp] = breaks;
+  __syncthreads();
+  const bool starts = slot >= 0 && !on;
+  int len = 0;
+  bool open = false;  // no break behind it in this CTA
+  if (starts) {
+    uint32_t rest = breaks & (lane == 31 ? 0u : ~0u << (lane + 1));
+    int w = warp;
+    while (rest == 0 && ++w < WARPS) rest = s_breaks[w];
+    open = w == WARPS;
+    len = (open ? THREADS : w * 32 + __ffs(rest) - 1) - static_cast<int>(threadIdx.x);
+  }
+  // At most one run of a CTA is open: its warp follows it.
+  const uint32_t opens = __ballot_sync(0xffffffffu, open);
+  if (opens != 0) {
+    const int who = __ffs(opens) - 1;
+    const int more = more_tokens(p, static_cast<int64_t>(blockIdx.x) * THREADS + THREADS - 1,
+                                 __shfl_sync(0xffffffffu, block, who), lane);
+    if (lane == who) len += more;
+  }
+  const uint32_t who = __ballot_sync(0xffffffffu, starts);
+  if (lane == 0) s_starts[warp] = __popc(who);
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) {
+    before += w < warp ? s_starts[w] : 0;
+    all += s_starts[w];
+  }
+  if (threadIdx.x == 0) p.counts[blockIdx.x] = all;
+  if (starts) {
+    const int32_t claimed = atomicExch(p.claims + block, static_cast<int32_t>(t));
+    const int64_t first = static_cast<int64_t>(block) * p.block_size;
+    Run run{static_cast<int32_t>(t), block, 0, 0, 0, 0};
+    run.offset = static_cast<int16_t>(slot - first);
+    run.len = static_cast<int16_t>(len);
+    run.last = static_cast<int16_t>((len == 1 ? slot : slot_of(p, t + len - 1)) - first);
+    run.rival = claimed != static_cast<int32_t>(t) && starts_run(p, claimed, block);
+    p.runs[static_cast<int64_t>(blockIdx.x) * THREADS + before + __popc(who & ((1u << lane) - 1))] = run;
+  }
 }
 
 template <typename T>
@@ -102,163 +195,183 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t w, float was, float inv) {
   return C::pack4((a.x * was) * inv, (a.y * was) * inv, (b.x * was) * inv, (b.y * was) * inv);
 }
 
+// One run of one head of K or V (`pair` < heads: K), by a warp.
+template <typename T, typename C, int D>
+__device__ __forceinline__ void append_run(const AppendParams& p, const Run& run, int pair, int lane) {
+  constexpr int LANES = D / 8;      // lanes of a row, 8 elements each
+  constexpr int ROWS = 32 / LANES;  // rows side by side
+  const int row = lane / LANES, at = (lane - row * LANES) * 8;
+  const bool which = pair >= p.heads;
+  const int head = which ? pair - p.heads : pair;
+  const int64_t stride = which ? p.token_stride[1] : p.token_stride[0];
+  const T* src = static_cast<const T*>(which ? p.rows[1] : p.rows[0]) + run.token * stride +
+                 head * (which ? p.head_stride[1] : p.head_stride[0]) + at;
+  const int rows = run.len - row;  // from this lane's first on, ROWS apart
+  uint4 held[HELD];
+  {
+    const T* from = src + row * stride;
+#pragma unroll
+    for (int k = 0; k < HELD; ++k) {
+      held[k] = make_uint4(0, 0, 0, 0);
+      if (k * ROWS < rows) held[k] = ld_stream_v4(from);
+      from += ROWS * stride;
+    }
+  }
+  const int64_t slot_bytes = static_cast<int64_t>(p.heads) * D;
+  const int64_t slot0 = static_cast<int64_t>(run.block) * p.block_size;
+  uint8_t* dst = (which ? p.cache[1] : p.cache[0]) + slot0 * slot_bytes + static_cast<int64_t>(head) * D + at;
+  float* scale = (which ? p.scales[1] : p.scales[0]) + static_cast<int64_t>(run.block) * p.heads + head;
+  const float was_raw = run.offset == 0 ? 0.f : *scale;
+  const float was = was_raw > 0.f && was_raw < INFINITY ? was_raw : 0.f;
+
+  float amax = 0.f;
+#pragma unroll
+  for (int k = 0; k < HELD; ++k) amax = fmaxf(amax, amax8<T>(held[k]));
+  // Unpacked again for the store: kept from here, their fp32 values would take twice the
+  // registers of the rows themselves.
+#pragma unroll
+  for (int k = 0; k < HELD; ++k) asm volatile("" : "+r"(held[k].x), "+r"(held[k].y), "+r"(held[k].z), "+r"(held[k].w));
+#pragma unroll 1
+  for (int r = row + HELD * ROWS; r < run.len; r += ROWS)
+    amax = fmaxf(amax, amax8<T>(*reinterpret_cast<const uint4*>(src + r * stride)));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  const float now = fmaxf(was, C::scale_for(amax));
+  const float inv = 1.0f / now;
+
+  const bool dense = run.last - run.offset == run.len - 1;  // no holes
+  if (run.offset > 0 && now != was) {
+    // Rows that stay: those below the last new one that the run does not write.
+#pragma unroll 1
+    for (int r = row; r < run.last; r += ROWS) {
+      bool stays = r < run.offset;
+      if (!stays && !dense) {
+        int lo = 0, hi = run.len - 1;  // the run's slots ascend
+        while (lo < hi) {
+          const int mid = (lo + hi) >> 1;
+          if (slot_of(p, run.token + mid) - slot0 >= r) hi = mid;
+          else lo = mid + 1;
+        }
+        stays = slot_of(p, run.token + lo) - slot0 != r;
+      }
+      if (stays) {
+        uint2* cell = reinterpret_cast<uint2*>(dst + r * slot_bytes);
+        uint2 v = *cell;
+        v.x = rescale4<C>(v.x, was, inv);
+        v.y = rescale4<C>(v.y, was, inv);
+        *cell = v;
+      }
+    }
+  }
+  if (dense) {
+    uint8_t* to = dst + (run.offset + row) * slot_bytes;
+#pragma unroll
+    for (int k = 0; k < HELD; ++k) {
+      if (k * ROWS < rows) *reinterpret_cast<uint2*>(to) = store8<T, C>(held[k], inv);
+      to += ROWS * slot_bytes;
+    }
+  }
+#pragma unroll 1
+  for (int r = row + (dense ? HELD * ROWS : 0); r < run.len; r += ROWS) {
+    const int64_t o = dense ? run.offset + r : slot_of(p, run.token + r) - slot0;
+    *reinterpret_cast<uint2*>(dst + o * slot_bytes) = store8<T, C>(*reinterpret_cast<const uint4*>(src + r * stride), inv);
+  }
+  __syncwarp();  // every lane has read the old scale
+  if (lane == 0) *scale = now;
+}
+
+// Few tokens: a CTA (of each 8 heads of K and V) per token, which goes on if a run starts there.
 template <typename T, typename C, int D>
 __global__ void __launch_bounds__(THREADS) paged_append8_kernel(AppendParams p, KernelCtl ctl) {
-  constexpr int LANES = D / 8;     // lanes of a row, 8 elements each
-  constexpr int ROWS = 32 / LANES;  // rows side by side
-  __shared__ int64_t s_token[SPAN];  // first token of each run that starts here
-  __shared__ int64_t s_slot[SPAN];   // and its slot
-  __shared__ int s_len[SPAN];
-  __shared__ int s_drop[SPAN];
-  __shared__ int s_runs;
   pdl_begin();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * p.span;
-  const int span = static_cast<int>(min(static_cast<int64_t>(p.span), p.tokens - t0));
-  if (threadIdx.x == 0) s_runs = 0;
-  __syncthreads();
-  if (threadIdx.x < span) {
-    const int64_t t = t0 + threadIdx.x;
-    const int64_t slot = slot_of(p.slots, p.index_bits, t);
-    if (slot >= p.capacity) {
-      atomicOr(ctl.status, RK_DEV_ERR_BAD_INDEX);
-    } else if (slot >= 0 && starts_run(p.slots, p.index_bits, t, slot, p.block_size)) {
-      const int at = atomicAdd(&s_runs, 1);  // any order: runs are independent
-      s_token[at] = t;
-      s_slot[at] = slot;
-      s_drop[at] = p.claims != nullptr && p.claims[slot / p.block_size] != t;
-    }
+  const int pair = static_cast<int>(blockIdx.y) * WARPS + warp;
+  const int64_t t = blockIdx.x;
+  const int64_t slot = slot_of(p, t);
+  const int64_t before = t > 0 ? slot_of(p, t - 1) : -1;
+  if (slot >= p.capacity && threadIdx.x == 0 && blockIdx.y == 0) atomicOr(ctl.status, RK_DEV_ERR_BAD_INDEX);
+  if (slot < 0 || slot >= p.capacity) return;
+  const int block = block_of(p, slot);
+  if (goes_on(p, before, slot, block)) return;
+  // A block that an earlier token went to has been stored by that run.
+  const int64_t slot0 = static_cast<int64_t>(block) * p.block_size;
+  bool seen = false;
+  for (int64_t i = threadIdx.x; i < t; i += THREADS) {
+    const int64_t other = slot_of(p, i);
+    seen = seen || (other >= slot0 && other < slot0 + p.block_size);
   }
-  __syncthreads();
-  const int runs = s_runs;
-  for (int i = warp; i < runs; i += WARPS) {
-    // Length of the run: 32 tokens at a time, until one does not continue it.
-    const int64_t first = s_token[i], block = s_slot[i] / p.block_size;
-    int64_t len = 1;
-    for (;;) {
-      const int64_t t = first + len + lane;
-      bool on = false;
-      if (t < p.tokens) {
-        const int64_t slot = slot_of(p.slots, p.index_bits, t), before = slot_of(p.slots, p.index_bits, t - 1);
-        on = slot > before && slot < p.capacity && before >= 0 && slot / p.block_size == block;
-      }
-      const uint32_t off = ~__ballot_sync(0xffffffffu, on);
-      if (off != 0) {
-        len += __ffs(off) - 1;
-        break;
-      }
-      len += 32;
-    }
-    if (p.claims == nullptr) {
-      bool seen = false;
-      for (int64_t t = lane; t < first; t += 32) {
-        const int64_t slot = slot_of(p.slots, p.index_bits, t);
-        seen = seen || (slot >= 0 && slot < p.capacity && slot / p.block_size == block);
-      }
-      if (lane == 0) s_drop[i] = 0;
-      __syncwarp();
-      if (__any_sync(0xffffffffu, seen) && lane == 0) s_drop[i] = 1;
-    }
-    if (lane == 0) {
-      s_len[i] = static_cast<int>(len);  // slots ascend within a block: at most block_size
-      if (s_drop[i]) atomicOr(ctl.status, RK_DEV_ERR_BAD_INDEX);
-    }
+  if (__syncthreads_or(seen)) {
+    if (threadIdx.x == 0 && blockIdx.y == 0) atomicOr(ctl.status, RK_DEV_ERR_BAD_INDEX);
+    return;
   }
-  __syncthreads();
+  if (pair >= 2 * p.heads) return;
+  const int len = 1 + more_tokens(p, t, block, lane);
+  const Run run{static_cast<int32_t>(t), block, static_cast<int16_t>(slot - slot0), static_cast<int16_t>(len),
+                static_cast<int16_t>((len == 1 ? slot : slot_of(p, t + len - 1)) - slot0), 0};
+  append_run<T, C, D>(p, run, pair, lane);
+}
 
+// Many tokens: `parts` CTAs for each list, whose warps take the runs' heads of K and V in turn.
+template <typename T, typename C, int D>
+__global__ void __launch_bounds__(THREADS, APPEND_CTAS) paged_append8_runs_kernel(AppendParams p, KernelCtl ctl) {
+  pdl_begin();
+  const int lane = threadIdx.x & 31;
+  const int list = static_cast<int>(blockIdx.x) / p.parts, part = static_cast<int>(blockIdx.x) - list * p.parts;
   const int pairs = 2 * p.heads;
-  const int y_pairs = min(WARPS, pairs - static_cast<int>(blockIdx.y) * WARPS);  // of this CTA
-  const int row = lane / LANES, at = (lane - row * LANES) * 8;
-  for (int item = warp; item < runs * y_pairs; item += WARPS) {
-    const int i = item / y_pairs;
-    const int pair = static_cast<int>(blockIdx.y) * WARPS + item - i * y_pairs;
-    if (s_drop[i]) continue;
-    const int which = pair >= p.heads, head = which ? pair - p.heads : pair;
-    const int64_t first = s_token[i], slot0 = s_slot[i];
-    const int64_t block = slot0 / p.block_size;
-    const int offset0 = static_cast<int>(slot0 - block * p.block_size);
-    const int len = s_len[i];
-    const int64_t stride = which ? p.token_stride[1] : p.token_stride[0];
-    const T* src = static_cast<const T*>(which ? p.rows[1] : p.rows[0]) + first * stride +
-                   head * (which ? p.head_stride[1] : p.head_stride[0]) + at;
-    const int64_t slot_bytes = static_cast<int64_t>(p.heads) * D;
-    uint8_t* dst = (which ? p.cache[1] : p.cache[0]) + block * p.block_size * slot_bytes + static_cast<int64_t>(head) * D + at;
-    float* scale = (which ? p.scales[1] : p.scales[0]) + block * p.heads + head;
-    const float was_raw = offset0 == 0 ? 0.f : *scale;
-    const float was = was_raw > 0.f && was_raw < INFINITY ? was_raw : 0.f;
-
-    uint4 held[HELD];
-    float amax = 0.f;
-#pragma unroll
-    for (int k = 0; k < HELD; ++k) {
-      const int r = row + k * ROWS;
-      held[k] = make_uint4(0, 0, 0, 0);
-      if (r < len) held[k] = ld_stream_v4(src + r * stride);
-    }
-#pragma unroll
-    for (int k = 0; k < HELD; ++k) amax = fmaxf(amax, amax8<T>(held[k]));
-    for (int r = row + HELD * ROWS; r < len; r += ROWS)
-      amax = fmaxf(amax, amax8<T>(*reinterpret_cast<const uint4*>(src + r * stride)));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    const float now = fmaxf(was, C::scale_for(amax));
-    const float inv = 1.0f / now;
-
-    const int last = static_cast<int>(slot_of(p.slots, p.index_bits, first + len - 1) - block * p.block_size);
-    if (offset0 > 0 && now != was) {
-      // Rows that stay: those below the last new one that the run does not write.
-      const bool dense = last - offset0 == len - 1;
-      for (int r = row; r < last; r += ROWS) {
-        bool stays = r < offset0;
-        if (!stays && !dense) {
-          int lo = 0, hi = len - 1;  // the run's slots ascend
-          while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (slot_of(p.slots, p.index_bits, first + mid) - block * p.block_size >= r) hi = mid;
-            else lo = mid + 1;
-          }
-          stays = slot_of(p.slots, p.index_bits, first + lo) - block * p.block_size != r;
-        }
-        if (stays) {
-          uint2* cell = reinterpret_cast<uint2*>(dst + r * slot_bytes);
-          uint2 v = *cell;
-          v.x = rescale4<C>(v.x, was, inv);
-          v.y = rescale4<C>(v.y, was, inv);
-          *cell = v;
-        }
+  const int items = __ldg(p.counts + list) * pairs;
+#pragma unroll 1
+  for (int item = part * WARPS + (threadIdx.x >> 5); item < items; item += p.parts * WARPS) {
+    const int at = item / pairs, pair = item - at * pairs;
+    const int4 raw = __ldg(reinterpret_cast<const int4*>(p.runs) + static_cast<int64_t>(list) * THREADS + at);
+    const Run run{raw.x, raw.y, static_cast<int16_t>(raw.z & 0xFFFF), static_cast<int16_t>(raw.z >> 16),
+                  static_cast<int16_t>(raw.w & 0xFFFF), static_cast<int16_t>(raw.w >> 16)};
+    if (run.rival != 0 || __ldg(p.claims + run.block) != run.token) {
+      // The block has several runs: the first is stored, the others are not.
+      const int64_t slot0 = static_cast<int64_t>(run.block) * p.block_size;
+      bool seen = false;
+      for (int64_t t = lane; t < run.token; t += 32) {
+        const int64_t slot = slot_of(p, t);
+        seen = seen || (slot >= slot0 && slot < slot0 + p.block_size);
+      }
+      if (__any_sync(0xffffffffu, seen)) {
+        if (lane == 0 && pair == 0) atomicOr(ctl.status, RK_DEV_ERR_BAD_INDEX);
+        continue;
       }
     }
-#pragma unroll
-    for (int k = 0; k < HELD; ++k) {
-      const int r = row + k * ROWS;
-      if (r < len) {
-        const int64_t o = slot_of(p.slots, p.index_bits, first + r) - block * p.block_size;
-        *reinterpret_cast<uint2*>(dst + o * slot_bytes) = store8<T, C>(held[k], inv);
-      }
-    }
-    for (int r = row + HELD * ROWS; r < len; r += ROWS) {
-      const int64_t o = slot_of(p.slots, p.index_bits, first + r) - block * p.block_size;
-      *reinterpret_cast<uint2*>(dst + o * slot_bytes) =
-          store8<T, C>(*reinterpret_cast<const uint4*>(src + r * stride), inv);
-    }
-    __syncwarp();  // every lane has read the old scale
-    if (lane == 0) *scale = now;
+    append_run<T, C, D>(p, run, pair, lane);
   }
 }
 
+int64_t lists_of(int64_t tokens) { return (tokens + THREADS - 1) / THREADS; }
+
+template <typename T, typename C, int D>
+cudaError_t launch(const AppendParams& p, const KernelCtl& ctl, cudaStream_t s) {
+  if (p.runs == nullptr) {
+    const dim3 grid(static_cast<unsigned>(p.tokens), static_cast<unsigned>((2 * p.heads + WARPS - 1) / WARPS));
+    note_launch("paged_append8_kernel");
+    return launch_kernel(paged_append8_kernel<T, C, D>, grid, dim3(THREADS), 0, s, 0, p, ctl);
+  }
+  const int64_t lists = lists_of(p.tokens);
+  note_launch("paged_append8_runs_kernel");
+  return launch_kernel(paged_append8_runs_kernel<T, C, D>, dim3(static_cast<unsigned>(lists * p.parts)), dim3(THREADS), 0,
+                       s, 0, p, ctl);
+}
+
 template <typename T, typename C>
-cudaError_t launch_d(const AppendParams& p, int64_t head_dim, const KernelCtl& ctl, dim3 grid, cudaStream_t s) {
+cudaError_t launch_d(const AppendParams& p, int64_t head_dim, const KernelCtl& ctl, cudaStream_t s) {
   switch (head_dim) {
-    case 64: return launch_kernel(paged_append8_kernel<T, C, 64>, grid, dim3(THREADS), 0, s, 0, p, ctl);
-    case 128: return launch_kernel(paged_append8_kernel<T, C, 128>, grid, dim3(THREADS), 0, s, 0, p, ctl);
-    default: return launch_kernel(paged_append8_kernel<T, C, 256>, grid, dim3(THREADS), 0, s, 0, p, ctl);
+    case 64: return launch<T, C, 64>(p, ctl, s);
+    case 128: return launch<T, C, 128>(p, ctl, s);
+    default: return launch<T, C, 256>(p, ctl, s);
   }
 }
 
 }  // namespace
 
 size_t paged_append8_workspace_bytes(int64_t tokens, int64_t num_blocks) {
-  return tokens > SCAN_TOKENS ? static_cast<size_t>(num_blocks) * sizeof(int32_t) : 0;
+  if (tokens <= SCAN_TOKENS) return 0;
+  const int64_t lists = lists_of(tokens);
+  return static_cast<size_t>(lists) * THREADS * sizeof(Run) + static_cast<size_t>(num_blocks + lists) * sizeof(int32_t);
 }
 
 rk_status paged_append8_launch(const PagedAppend8Args& a, void* workspace, size_t workspace_bytes, cudaStream_t s) {
@@ -282,32 +395,29 @@ rk_status paged_append8_launch(const PagedAppend8Args& a, void* workspace, size_
   p.scales[1] = a.value_scales;
   p.slots = a.slot_mapping;
   p.index_bits = a.index_bits;
-  p.tokens = a.tokens;
+  p.tokens = static_cast<int32_t>(a.tokens);
   p.capacity = a.num_blocks * a.block_size;
   p.heads = static_cast<int>(a.kv_heads);
   p.block_size = static_cast<int>(a.block_size);
   if (need > 0) {
-    p.claims = static_cast<const int32_t*>(workspace);
-    cudaError_t e = cudaMemsetAsync(workspace, 0x7F, need, s);  // above every token index
-    if (e == cudaSuccess)
-      e = launch_kernel(append_claim_kernel, dim3(static_cast<unsigned>((a.tokens + THREADS - 1) / THREADS)),
-                        dim3(THREADS), 0, s, 0, a.slot_mapping, a.index_bits, a.tokens, p.capacity, p.block_size,
-                        static_cast<int32_t*>(workspace));
-    note_launch("append_claim_kernel");
+    const int64_t lists = lists_of(a.tokens);
+    p.runs = static_cast<Run*>(workspace);
+    p.claims = reinterpret_cast<int32_t*>(p.runs + lists * THREADS);
+    p.counts = p.claims + a.num_blocks;
+    // Enough CTAs to fill the GPU a few times, each with a run for every warp if blocks fill up.
+    const int64_t fill = static_cast<int64_t>(device_sm_count()) * APPEND_CTAS * 4;
+    const int64_t most = (THREADS / p.block_size + 1) * 2 * static_cast<int64_t>(p.heads) / WARPS + 1;
+    const int64_t parts = (fill + lists - 1) / lists;
+    p.parts = static_cast<int>(parts < most ? parts : most);
+    const cudaError_t e = launch_kernel(append_runs_kernel, dim3(static_cast<unsigned>(lists)), dim3(THREADS), 0, s, 0, p, ctl);
+    note_launch("append_runs_kernel");
     if (e != cudaSuccess) return cuda_status(e);
   }
-  // One token to a CTA while that fills the GPU, up to SPAN beyond.
-  const int64_t even = a.tokens / (4 * static_cast<int64_t>(device_sm_count()));
-  p.span = static_cast<int>(even < 1 ? 1 : (even > SPAN ? SPAN : even));
-  const dim3 grid(static_cast<unsigned>((a.tokens + p.span - 1) / p.span),
-                  static_cast<unsigned>((2 * p.heads + WARPS - 1) / WARPS));
   const bool bf16 = a.dt == RK_DTYPE_BF16, e4m3 = a.cache == RK_CACHE_E4M3;
-  const cudaError_t e =
-      bf16 ? (e4m3 ? launch_d<__nv_bfloat16, E4m3>(p, a.head_dim, ctl, grid, s)
-                   : launch_d<__nv_bfloat16, Int8>(p, a.head_dim, ctl, grid, s))
-           : (e4m3 ? launch_d<__half, E4m3>(p, a.head_dim, ctl, grid, s) : launch_d<__half, Int8>(p, a.head_dim, ctl, grid, s));
-  note_launch("paged_append8_kernel");
-  return cuda_status(e);
+  return cuda_status(bf16 ? (e4m3 ? launch_d<__nv_bfloat16, E4m3>(p, a.head_dim, ctl, s)
+                                  : launch_d<__nv_bfloat16, Int8>(p, a.head_dim, ctl, s))
+                          : (e4m3 ? launch_d<__half, E4m3>(p, a.head_dim, ctl, s)
+                                  : launch_d<__half, Int8>(p, a.head_dim, ctl, s)));
 }
 
 }  // namespace rk

@@ -286,7 +286,7 @@ def test_c_entries_check_their_arguments():
     size = ctypes.c_size_t(5)
     assert lib.rk_paged_cache_append_8bit_workspace_size(-1, 4, ctypes.byref(size)) == bad and size.value == 0
     assert lib.rk_paged_cache_append_8bit_workspace_size(10, 1000, ctypes.byref(size)) == ok and size.value == 0
-    assert lib.rk_paged_cache_append_8bit_workspace_size(100000, 1000, ctypes.byref(size)) == ok and size.value == 4000
+    assert lib.rk_paged_cache_append_8bit_workspace_size(100000, 1000, ctypes.byref(size)) == ok and size.value >= 4000
     assert lib.rk_paged_cache_append_8bit_workspace_size(10, 10, None) == bad
 
     def attention(batch=1, hq=2, hk=1, dim=64, blocks=1, size=16, width=1, scale=1.0, dt=1, kind=0, bits=32, p=null):
