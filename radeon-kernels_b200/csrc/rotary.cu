@@ -13,7 +13,8 @@
 // and used by every head: 1 / (query_heads + kv_heads) of the work of computing them where
 // they are used.
 //
-// What bounds it: the bytes of the queries and keys, read and written once.
+// What bounds it: the bytes of the queries and keys, read and written once (8192 tokens of 32 + 8
+// heads of 128 in bf16: 168 MB in 32.8 us, 5.1 TB/s; 16 tokens: 2.5 us, the launch).
 #include <cuda_runtime.h>
 
 #include "rk_device.cuh"
@@ -23,6 +24,7 @@ namespace rk {
 namespace {
 
 constexpr int THREADS = 256;
+constexpr int ROWS_AHEAD = 2;  // rows of a thread in flight, of two vectors each
 
 struct RotaryParams {
   const void* in[2];    // queries, keys
@@ -33,14 +35,14 @@ struct RotaryParams {
   int64_t tokens;
   int query_heads, heads;  // heads: query_heads + kv_heads
   int head_dim, half;
-  int units;        // work items per head
+  int units;        // work items per head: two vectors each (or elements, without vectors)
   int turn_units;   // the first of them that rotate
   int index_bits;
   float amplitude;
   int inverse;
 };
 
-// One 16-byte vector of each half (HALVES) or of neighbouring pairs (INTERLEAVED), turned.
+// Two vectors of 8 elements that a lane turns: the first and second elements of 8 pairs.
 template <typename T>
 __device__ __forceinline__ void turn_halves(uint4& a, uint4& b, const float2* cs) {
   uint32_t* pa = reinterpret_cast<uint32_t*>(&a);
@@ -54,75 +56,142 @@ __device__ __forceinline__ void turn_halves(uint4& a, uint4& b, const float2* cs
   }
 }
 
+// A vector of 4 neighbouring pairs.
 template <typename T>
 __device__ __forceinline__ void turn_pairs(uint4& a, const float2* cs) {
   uint32_t* pa = reinterpret_cast<uint32_t*>(&a);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float2 x = Pack2<T>::to_floats(pa[j]);
-    const float2 t = cs[j];
+  for (int j = 0; j < 4; j += 2) {
+    const float4 t = *reinterpret_cast<const float4*>(cs + j);
+    const float2 x = Pack2<T>::to_floats(pa[j]), y = Pack2<T>::to_floats(pa[j + 1]);
     pa[j] = Pack2<T>::from_floats(x.x * t.x - x.y * t.y, x.y * t.x + x.x * t.y);
+    pa[j + 1] = Pack2<T>::from_floats(y.x * t.z - y.y * t.w, y.y * t.z + y.x * t.w);
   }
 }
 
-// VEC: 16-byte vectors (head sizes, strides and pointers allow them); otherwise one pair or
-// one element per item.  `tokens_per_cta` tokens share a CTA and its table of cosines.
+// A CTA takes some tokens.  Each thread keeps one unit of a head (no division in the loop) and
+// walks over the heads of the tokens, ROWS of them in flight; the first are on their way while
+// the threads fill the table of the tokens' cosines and sines.  VEC: 16-byte vectors (head
+// sizes, strides and pointers allow them); otherwise a pair or an element at a time.
 template <typename T, bool INTERLEAVED, bool VEC>
-__global__ void __launch_bounds__(THREADS) rotary_kernel(RotaryParams p, int tokens_per_cta) {
+__global__ void __launch_bounds__(THREADS, VEC ? 6 : 1) rotary_kernel(RotaryParams p, int tokens_per_cta) {
+  constexpr int ROWS = VEC ? ROWS_AHEAD : 1;
   extern __shared__ float2 table[];  // [tokens_per_cta][half]
   pdl_begin();
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * tokens_per_cta;
   const int nt = static_cast<int>(min(static_cast<int64_t>(tokens_per_cta), p.tokens - t0));
+  const int rows = nt * p.heads;
+  const int side = min(p.units, THREADS);  // threads of a row
+  const int step = THREADS / side;         // rows side by side; threads left over take none
+  const int row0 = threadIdx.x / side;
+  int unit = row0 < step ? threadIdx.x - row0 * side : p.units;
+
+  // Elements of the unit's two vectors, and whether there is a second.
+  int first = 0, second = 0;
+  bool turns = false, both = false;
+  const auto look_at_unit = [&] {
+    turns = unit < p.turn_units;
+    if (!VEC) {
+      first = turns ? (INTERLEAVED ? 2 * unit : unit) : unit + p.half;  // behind the pairs one element each
+      second = INTERLEAVED ? first + 1 : first + p.half;
+      both = turns;
+    } else if (INTERLEAVED || !turns) {
+      first = INTERLEAVED ? unit * 16 : 2 * p.half + (unit - p.turn_units) * 16;
+      second = first + 8;
+      both = second < p.head_dim;
+    } else {
+      first = unit * 8;
+      second = first + p.half;
+      both = true;
+    }
+  };
+  // Walks over ROWS rows from (t, h) on, handing each its place in the loop.
+  const auto walk = [&](int row, int t, int h, const auto& visit) {
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+      if (row + k * step < rows) visit(k, t, h);
+      h += step;
+      while (h >= p.heads) {
+        h -= p.heads;
+        ++t;
+      }
+    }
+  };
+  uint4 a[ROWS], b[ROWS];
+  const auto source = [&](int t, int h) {
+    const bool key = h >= p.query_heads;
+    return static_cast<const T*>(key ? p.in[1] : p.in[0]) + (t0 + t) * (key ? p.token_stride[1] : p.token_stride[0]) +
+           (key ? h - p.query_heads : h) * (key ? p.head_stride[1] : p.head_stride[0]);
+  };
+  const auto load = [&](int k, int t, int h) {
+    if (VEC) {
+      const T* in = source(t, h);
+      a[k] = ld_stream_v4(in + first);
+      if (both) b[k] = ld_stream_v4(in + second);
+    }
+  };
+  const auto turn_and_store = [&](int k, int t, int h) {
+    const bool key = h >= p.query_heads;
+    const int head = key ? h - p.query_heads : h, nheads = key ? p.heads - p.query_heads : p.query_heads;
+    T* out = static_cast<T*>(key ? p.out[1] : p.out[0]) + ((t0 + t) * nheads + head) * p.head_dim;
+    const float2* cs = table + t * p.half;
+    if (VEC) {
+      if (INTERLEAVED) {
+        // The border between turned and copied elements lies on a vector's.
+        if (first < 2 * p.half) turn_pairs<T>(a[k], cs + first / 2);
+        if (second < 2 * p.half) turn_pairs<T>(b[k], cs + second / 2);
+      } else if (turns) {
+        turn_halves<T>(a[k], b[k], cs + first);
+      }
+      *reinterpret_cast<uint4*>(out + first) = a[k];
+      if (both) *reinterpret_cast<uint4*>(out + second) = b[k];
+    } else {
+      const T* in = source(t, h);
+      if (turns) {
+        const float x = to_f32(in[first]), y = to_f32(in[second]);
+        const float2 c = cs[unit];
+        out[first] = from_f32<T>(x * c.x - y * c.y);
+        out[second] = from_f32<T>(y * c.x + x * c.y);
+      } else {
+        out[first] = in[first];
+      }
+    }
+  };
+
+  const int start_t = row0 / p.heads, start_h = row0 - start_t * p.heads;
+  int row = unit < p.units ? row0 : rows, t = start_t, h = start_h;
+  look_at_unit();
+  walk(row, t, h, load);
+
   for (int i = threadIdx.x; i < nt * p.half; i += THREADS) {
-    const int t = i / p.half, f = i - t * p.half;
+    const int at = i / p.half, f = i - at * p.half;
     const double position = p.index_bits == 32
-                                ? static_cast<double>(static_cast<const int32_t*>(p.positions)[t0 + t])
-                                : static_cast<double>(static_cast<const int64_t*>(p.positions)[t0 + t]);
-    const double turns = position * (p.frequencies[f] * 0.15915494309189533577);  // 1 / (2 pi)
+                                ? static_cast<double>(static_cast<const int32_t*>(p.positions)[t0 + at])
+                                : static_cast<double>(static_cast<const int64_t*>(p.positions)[t0 + at]);
+    const double turned = position * (p.frequencies[f] * 0.15915494309189533577);  // 1 / (2 pi)
     float s, c;
-    sincospif(2.0f * static_cast<float>(turns - rint(turns)), &s, &c);
+    sincospif(2.0f * static_cast<float>(turned - rint(turned)), &s, &c);
     table[i] = make_float2(c * p.amplitude, (p.inverse ? -s : s) * p.amplitude);
   }
   __syncthreads();
-  const int items = nt * p.heads * p.units;
-  for (int item = threadIdx.x; item < items; item += THREADS) {
-    const int row = item / p.units, unit = item - row * p.units;
-    const int t = row / p.heads, h = row - t * p.heads;
-    const int which = h >= p.query_heads;
-    const int head = which ? h - p.query_heads : h;
-    const int nheads = which ? p.heads - p.query_heads : p.query_heads;
-    const T* in = static_cast<const T*>((which ? p.in[1] : p.in[0])) + (t0 + t) * (which ? p.token_stride[1] : p.token_stride[0]) + head * (which ? p.head_stride[1] : p.head_stride[0]);
-    T* out = static_cast<T*>((which ? p.out[1] : p.out[0])) + ((t0 + t) * nheads + head) * p.head_dim;
-    const float2* cs = table + t * p.half;
-    if (VEC) {
-      if (unit < p.turn_units) {
-        if (INTERLEAVED) {
-          uint4 a = ld_stream_v4(in + unit * 8);
-          turn_pairs<T>(a, cs + unit * 4);
-          *reinterpret_cast<uint4*>(out + unit * 8) = a;
-        } else {
-          uint4 a = ld_stream_v4(in + unit * 8);
-          uint4 b = ld_stream_v4(in + p.half + unit * 8);
-          turn_halves<T>(a, b, cs + unit * 8);
-          *reinterpret_cast<uint4*>(out + unit * 8) = a;
-          *reinterpret_cast<uint4*>(out + p.half + unit * 8) = b;
-        }
-      } else {
-        const int at = 2 * p.half + (unit - p.turn_units) * 8;
-        *reinterpret_cast<uint4*>(out + at) = ld_stream_v4(in + at);
-      }
-    } else {
-      if (unit < p.turn_units) {
-        const int ia = INTERLEAVED ? 2 * unit : unit, ib = INTERLEAVED ? 2 * unit + 1 : unit + p.half;
-        const float a = to_f32(in[ia]), b = to_f32(in[ib]);
-        const float2 t2 = cs[unit];
-        out[ia] = from_f32<T>(a * t2.x - b * t2.y);
-        out[ib] = from_f32<T>(b * t2.x + a * t2.y);
-      } else {
-        const int at = 2 * p.half + unit - p.turn_units;
-        out[at] = in[at];
-      }
+
+#pragma unroll 1
+  while (row < rows) {
+    walk(row, t, h, turn_and_store);
+    row += ROWS * step;
+    h += ROWS * step;
+    while (h >= p.heads) {
+      h -= p.heads;
+      ++t;
     }
+    if (row >= rows && unit + side < p.units) {  // heads of more units than threads
+      unit += side;
+      row = row0;
+      t = start_t;
+      h = start_h;
+      look_at_unit();
+    }
+    walk(row, t, h, load);
   }
 }
 
@@ -164,14 +233,23 @@ rk_status rotary_launch(const RotaryArgs& a, cudaStream_t s) {
   for (int w = 0; w < 2; ++w)
     vec = vec && aligned16(p.in[w]) && aligned16(p.out[w]) && p.token_stride[w] % 8 == 0 && p.head_stride[w] % 8 == 0;
   if (vec) {
-    p.turn_units = a.interleaved ? p.half / 4 : p.half / 8;
-    p.units = p.turn_units + (p.head_dim - 2 * p.half) / 8;
+    // Two vectors to a unit: neighbours, or the two halves of the pairs.
+    p.turn_units = p.half / 8;  // interleaved units look at their elements
+    p.units = a.interleaved ? (p.head_dim + 15) / 16 : p.turn_units + (p.head_dim - 2 * p.half + 15) / 16;
   } else {
     p.turn_units = p.half;
     p.units = p.half + p.head_dim - 2 * p.half;
   }
-  // Few tokens: one CTA each, so that they spread over the SMs.  Many: four to a CTA.
-  const int per_cta = p.tokens >= 16 * static_cast<int64_t>(device_sm_count()) ? 4 : 1;
+  // Few tokens: one CTA each, so that they spread over the SMs.  Many: two to a CTA, or three where
+  // two leave over a third of its last round of rows empty (8192 tokens of 32 + 8 heads of
+  // 128: 32.8 us with three, 34.0 with two, 37.7 with one, 38.3 with eight; 4099 tokens of 32
+  // heads, which fill the round: 15.0, 14.4, 16.7, 20.2).
+  int per_cta = 1;
+  if (p.tokens >= 16 * static_cast<int64_t>(device_sm_count())) {
+    const int round = ROWS_AHEAD * (THREADS / (p.units < THREADS ? p.units : THREADS));
+    const auto filled = [&](int t) { return static_cast<float>(t * p.heads) / ((t * p.heads + round - 1) / round * round); };
+    per_cta = filled(3) > filled(2) + 0.2f ? 3 : 2;
+  }
   const cudaError_t e = a.dt == RK_DTYPE_BF16 ? launch<__nv_bfloat16>(p, a.interleaved, vec, per_cta, s)
                                               : launch<__half>(p, a.interleaved, vec, per_cta, s);
   note_launch("rotary_kernel");
