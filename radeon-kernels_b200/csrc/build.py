@@ -106,6 +106,7 @@ def _torch_flags() -> tuple[list[str], list[str]]:
         "-lc10_cuda",
         "-ltorch",
         "-ltorch_cpu",
+        "-ltorch_cuda",
         "-ltorch_python",
     ]
     return cflags, ldflags

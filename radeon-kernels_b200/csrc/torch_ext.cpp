@@ -14,6 +14,7 @@
 //   gemm(a, b, variant) -> new tensor
 //   gemm_views(a, b, out=None, variant) -> C   (transposed views in place: rk_gemm_layout)
 //   gemv_*(input, weight) -> new tensor   (native_gemv.hip:343-391)
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -411,6 +412,12 @@ at::Tensor sdpa(const at::Tensor& query, const at::Tensor& key, const at::Tensor
   return out;
 }
 
+// A new dense tensor, without the dispatcher's share of at::empty (about a microsecond, which is a
+// tenth of a small call).
+at::Tensor new_dense(at::IntArrayRef sizes, at::ScalarType dtype, const at::Device& device) {
+  return at::Tensor(at::detail::empty_cuda(sizes, dtype, device, c10::nullopt));
+}
+
 // Index tensors of one call: int32 or int64, CUDA, contiguous.
 int index_bits_of(const at::Tensor& t, const char* name, int64_t rank) {
   TORCH_CHECK(t.is_cuda() && t.dim() == rank && t.is_contiguous(), name, " must be a contiguous CUDA tensor of rank ",
@@ -456,8 +463,8 @@ std::vector<at::Tensor> rotary_forward(const at::Tensor& query_in, const at::Ten
               "query and key must share tokens and head_dim");
   TORCH_CHECK(positions.size(0) == query.size(0), "positions must hold one position per token");
   TORCH_CHECK(!frequencies.requires_grad(), "frequencies must not require gradients");
-  auto query_out = at::empty(query.sizes(), query.options());
-  auto key_out = at::empty(key.sizes(), key.options());
+  auto query_out = new_dense(query.sizes(), query.scalar_type(), query.device());
+  auto key_out = new_dense(key.sizes(), key.scalar_type(), key.device());
   check_status(rk_rotary_embedding(query.data_ptr(), key.data_ptr(), positions.data_ptr(),
                                    frequencies.data_ptr<double>(), query_out.data_ptr(), key_out.data_ptr(),
                                    query.size(0), query.size(1), key.size(1), query.size(2), 2 * frequencies.size(0),
@@ -517,10 +524,11 @@ std::vector<at::Tensor> paged_slots(at::Tensor block_tables, const at::Tensor& c
               "lengths must hold one entry per row of block_tables");
   TORCH_CHECK(num_tokens >= 0, "num_tokens must not be negative");
   c10::cuda::CUDAGuard guard(block_tables.device());
-  auto slots = at::empty({num_tokens}, block_tables.options().dtype(at::kLong));
-  auto positions = at::empty({num_tokens}, block_tables.options());
-  auto lengths = at::empty({block_tables.size(0)}, block_tables.options());
-  auto used = at::empty({1}, block_tables.options());
+  const at::ScalarType index = block_tables.scalar_type();
+  auto slots = new_dense({num_tokens}, at::kLong, block_tables.device());
+  auto positions = new_dense({num_tokens}, index, block_tables.device());
+  auto lengths = new_dense({block_tables.size(0)}, index, block_tables.device());
+  auto used = new_dense({1}, index, block_tables.device());
   check_status(rk_paged_slots(block_tables.data_ptr(), context_lengths.data_ptr(), new_lengths.data_ptr(),
                               free_blocks.data_ptr(), slots.data_ptr<int64_t>(), positions.data_ptr(),
                               lengths.data_ptr(), used.data_ptr(), block_tables.size(0), block_tables.size(1),
@@ -629,7 +637,7 @@ at::Tensor paged_attention_decode_8bit(const at::Tensor& query_in, const at::Ten
   TORCH_CHECK(block_tables.size(0) == query.size(0) && context_lengths.size(0) == query.size(0),
               "index tensors must have one row per sequence");
   TORCH_CHECK(key_cache.size(3) == query.size(2), "query and cache head dimensions must match");
-  auto out = at::empty_like(query);
+  auto out = new_dense(query.sizes(), query.scalar_type(), query.device());
   size_t ws_bytes = 0;
   check_status(rk_paged_attention_decode_8bit_workspace_size(query.size(1), key_cache.size(2), query.size(2), &ws_bytes),
                "rk_paged_attention_decode_8bit_workspace_size");
