@@ -53,7 +53,7 @@ constexpr int THREADS = WARPS * 32;
 constexpr int STAGES = 3;
 constexpr int MAX_CTAS_PER_SM = 4;   // sizes the workspace
 constexpr int RANGE_COST = 2;        // what starting and ending a range costs, in units
-constexpr float SLACK = 8.0f;        // a running maximum is raised when it is passed by 2^SLACK
+constexpr float SLACK = 256.0f;      // a running maximum is raised when a weight is this much above it
 constexpr float NONE = -3.402823466e38f;  // a maximum before any score: finite, so that -inf - NONE = -inf
 
 // Positions of a unit, which is one tile of a warp.
@@ -422,6 +422,7 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attention8_kernel(Params p, 
   constexpr int KC = D / 64;   // 16-byte chunks of a K row per lane
   constexpr int MT = D / 16;   // MMA tiles of 16 dimensions
   constexpr int HEADS = 8 * NT;
+  constexpr uint32_t FULL = TILE == 32 ? 0xFFFFFFFFu : 0xFFFFu;
   static_assert(HEADS * part_stride(D) * 4 <= STAGES * L::STAGE, "a warp's sums fit its ring");
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ Piece s_last[WARPS];   // of each warp's last range: the part is in its ring
@@ -648,7 +649,7 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attention8_kernel(Params p, 
     uint32_t qf[NT][4 * KC][2];
       float factor[NT][2];
       float o[NT][MT][4];
-      float m[NT][2], mo[NT][2], l[NT][2];
+      float m[NT][2], mo[NT][2], c[NT][2], l[NT][2];  // of heads 2 c4, 2 c4 + 1: c = 2^(m - mo)
       const int bf16 = flag_of(p.bf16);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -683,7 +684,7 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attention8_kernel(Params p, 
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           m[nt][i] = mo[nt][i] = NONE;
-          l[nt][i] = 0.f;
+          l[nt][i] = c[nt][i] = 0.f;
         }
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
@@ -727,53 +728,77 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attention8_kernel(Params p, 
               }
             }
           }
-          // Rows g and g + 8 of each 16.
-          bool raise = false;
-          float w[NT][SUB][4];
+          // Rows g and g + 8 of each 16: p = 2^(score - m), and the weights of V, w = p * vs * c.
+          float weight[NT][SUB][4];
+          float most = 0.f;
 #pragma unroll
           for (int t = 0; t < SUB; ++t) {
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
               const int row = 16 * t + 8 * r + g;
-              const float ks = at_smem<float>(tile, L::SCALES + row * 4);
-              const float lv = lg2_approx(at_smem<float>(tile, L::SCALES + (TILE + row) * 4));
-              const bool in = (mask >> row) & 1u;
+              const float ks = at_smem<float>(tile, L::SCALES + row * 4), vs = at_smem<float>(tile, L::SCALES + (TILE + row) * 4);
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                  float& x = s[nt][t][2 * r + i];
-                  x = in ? (x + s2[nt][t][2 * r + i]) * (ks * factor[nt][i]) : -INFINITY;
-                  w[nt][t][2 * r + i] = in ? x + lv : -INFINITY;
-                  raise = raise || x > m[nt][i] + SLACK || w[nt][t][2 * r + i] > mo[nt][i] + SLACK;
+                  const int e = 2 * r + i;
+                  s[nt][t][e] += s2[nt][t][e];
+                  float x = fmaf(s[nt][t][e], ks * factor[nt][i], -m[nt][i]);
+                  if (mask != FULL && !((mask >> row) & 1u)) x = -INFINITY;
+                  const float pw = ex2_approx(x);
+                  s2[nt][t][e] = pw;
+                  weight[nt][t][e] = pw * (vs * c[nt][i]);
+                  most = fmax3(most, pw, weight[nt][t][e]);
                 }
               }
             }
           }
-          if (__any_sync(0xffffffffu, raise)) {
+          if (__any_sync(0xffffffffu, most > SLACK)) {
+            // The maxima are raised to what they have become, and all sums brought to them.
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
               for (int i = 0; i < 2; ++i) {
-                float a = m[nt][i], b = mo[nt][i];
+                float bm = m[nt][i], bo = mo[nt][i];
 #pragma unroll
                 for (int t = 0; t < SUB; ++t) {
-                  a = fmax3(a, s[nt][t][i], s[nt][t][i + 2]);
-                  b = fmax3(b, w[nt][t][i], w[nt][t][i + 2]);
+#pragma unroll
+                  for (int r = 0; r < 2; ++r) {
+                    const int row = 16 * t + 8 * r + g;
+                    const float ks = at_smem<float>(tile, L::SCALES + row * 4), vs = at_smem<float>(tile, L::SCALES + (TILE + row) * 4);
+                    const float x = (mask >> row) & 1u ? s[nt][t][2 * r + i] * (ks * factor[nt][i]) : -INFINITY;
+                    bm = fmaxf(bm, x);
+                    bo = fmaxf(bo, x + lg2_approx(vs));
+                  }
                 }
 #pragma unroll
                 for (int x = 4; x < 32; x <<= 1) {
-                  a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, x));
-                  b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, x));
+                  bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, x));
+                  bo = fmaxf(bo, __shfl_xor_sync(0xffffffffu, bo, x));
                 }
-                const float down_l = ex2_approx(m[nt][i] - a), down_o = ex2_approx(mo[nt][i] - b);
-                m[nt][i] = a;
-                mo[nt][i] = b;
-                l[nt][i] *= down_l;
+                // c = 2^(m - mo), kept within fp32 (scales of 2^-126, or none but zeros).
+                bo = bm - fminf(bm - bo, 126.f);
+                l[nt][i] *= ex2_approx(m[nt][i] - bm);
+                const float down = ex2_approx(mo[nt][i] - bo);
+                c[nt][i] = ex2_approx(bm - bo);
+                m[nt][i] = bm;
+                mo[nt][i] = bo;
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
-                  o[nt][mt][i] *= down_o;
-                  o[nt][mt][i + 2] *= down_o;
+                  o[nt][mt][i] *= down;
+                  o[nt][mt][i + 2] *= down;
+                }
+#pragma unroll
+                for (int t = 0; t < SUB; ++t) {
+#pragma unroll
+                  for (int r = 0; r < 2; ++r) {
+                    const int row = 16 * t + 8 * r + g;
+                    const float ks = at_smem<float>(tile, L::SCALES + row * 4), vs = at_smem<float>(tile, L::SCALES + (TILE + row) * 4);
+                    float x = fmaf(s[nt][t][2 * r + i], ks * factor[nt][i], -bm);
+                    if (!((mask >> row) & 1u)) x = -INFINITY;
+                    s2[nt][t][2 * r + i] = ex2_approx(x);
+                    weight[nt][t][2 * r + i] = s2[nt][t][2 * r + i] * (vs * c[nt][i]);
+                  }
                 }
               }
             }
@@ -783,14 +808,10 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attention8_kernel(Params p, 
           for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int t = 0; t < SUB; ++t) {
-              float e[4];
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                l[nt][i & 1] += ex2_approx(s[nt][t][i] - m[nt][i & 1]);
-                e[i] = ex2_approx(w[nt][t][i] - mo[nt][i & 1]);
-              }
-              pf[nt][t][0] = transpose8x8(Pack2<__half>::from_floats(e[0], e[1]));
-              pf[nt][t][1] = transpose8x8(Pack2<__half>::from_floats(e[2], e[3]));
+              for (int i = 0; i < 4; ++i) l[nt][i & 1] += s2[nt][t][i];
+              pf[nt][t][0] = transpose8x8(Pack2<__half>::from_floats(weight[nt][t][0], weight[nt][t][1]));
+              pf[nt][t][1] = transpose8x8(Pack2<__half>::from_floats(weight[nt][t][2], weight[nt][t][3]));
             }
           }
           // V^T: a lane's 16 (D 64: 8) bytes of positions 2 c4, 2 c4 + 1, and those + 8, byte by
