@@ -188,11 +188,58 @@ __device__ __forceinline__ float lg2_approx(float x) {
   return y;
 }
 
+// a / b for quotients below 2^21, where fp32 is off by one at most.
+__device__ __forceinline__ uint32_t quotient(uint32_t a, uint32_t b) {
+  uint32_t q = static_cast<uint32_t>(__fdividef(static_cast<float>(a), static_cast<float>(b)));
+  const int rest = static_cast<int>(a - q * b);
+  if (rest < 0) --q;
+  if (rest >= static_cast<int>(b)) ++q;
+  return q;
+}
+
+// The shares of all warps: `extra` of them hold base + 1 places, the others base.  The host has
+// checked that the places of the largest lengths fit 32 bits.
+struct Shares {
+  uint32_t total, warps, base, extra;
+  __device__ __forceinline__ void set(uint32_t places, uint32_t most_warps) {
+    total = places;
+    warps = min(most_warps, places);
+    base = quotient(places, warps);
+    extra = places - base * warps;
+  }
+  __device__ __forceinline__ uint32_t start(uint32_t w) const { return w * base + min(w, extra); }
+  // The warp that holds a place.
+  __device__ __forceinline__ uint32_t owner(uint32_t place) const {
+    const uint32_t wide = extra * (base + 1);
+    const bool in = place < wide;
+    return (in ? 0u : extra) + quotient(in ? place : place - wide, in ? base + 1 : base);
+  }
+};
+
+// The parts in the workspace of a range that starts at `place`: that of the warp that begins it,
+// one of each later CTA (of its first warp), and one of the warp that ends it where that
+// is no CTA's first and went on to other ranges (otherwise it joined its neighbours').
+struct Parts {
+  int begin, end, ctas, count;
+  Parts() = default;
+  __device__ __forceinline__ Parts(uint32_t place, int units, const Shares& shares) {
+    begin = static_cast<int>(shares.owner(place));
+    end = static_cast<int>(shares.owner(place + units - 1));
+    ctas = end / WARPS - begin / WARPS;
+    const bool went_on = shares.start(end + 1) > place + units + RANGE_COST;
+    count = 1 + ctas + (end % WARPS != 0 && end != begin && went_on ? 1 : 0);
+  }
+  __device__ __forceinline__ int warp(int i) const {
+    return i == 0 ? begin : (i <= ctas ? (begin / WARPS + i) * WARPS : end);
+  }
+};
+
 // A range of which a warp holds a part.
 struct Piece {
   uint32_t place;  // of the range's first unit
-  int row, heads, units;  // heads 0: there is none
+  int row, heads;  // of the output; no heads: there is no piece
   int begins, ends;  // whether the part holds the range's first and last unit
+  Parts parts;
 };
 
 // Adds `parts` to the arrivals of a range and returns whether that makes `all`.  A word that does not
@@ -282,51 +329,10 @@ __device__ __forceinline__ void write_out(const Params& p, int64_t element, cons
 // other.  Without a position it is 1 / 0, and the sums 0.
 __device__ __forceinline__ float last_factor(float m, float mo, float l) { return ex2_approx(mo - m) / l; }
 
-// The shares of all warps: `extra` of them hold base + 1 places, the others base.  The host has
-// checked that the places of the largest lengths fit 32 bits.
-struct Shares {
-  uint32_t total, warps, base, extra;
-  __device__ __forceinline__ void set(uint32_t places, uint32_t most_warps) {
-    total = places;
-    warps = min(most_warps, places);
-    base = places / warps;
-    extra = places - base * warps;
-  }
-  __device__ __forceinline__ uint32_t start(uint32_t w) const { return w * base + min(w, extra); }
-  // The warp that holds a place.  There are some thousand at most, so the quotient is good to
-  // one in fp32.
-  __device__ __forceinline__ uint32_t owner(uint32_t place) const {
-    const uint32_t wide = extra * (base + 1);
-    const bool in = place < wide;
-    const float guess = __fdividef(static_cast<float>(in ? place : place - wide), static_cast<float>(in ? base + 1 : base));
-    uint32_t w = min((in ? 0u : extra) + static_cast<uint32_t>(guess), warps - 1);
-    if (start(w) > place) --w;
-    if (start(w + 1) <= place) ++w;
-    return w;
-  }
-};
-
 template <int D, int HEADS>
 __device__ __forceinline__ float* part_of(const Params& p, int warp, int k) {
   return p.part + (static_cast<int64_t>(warp) * 2 + k) * (HEADS * part_stride(D));
 }
-
-// The parts in the workspace of a range that starts at `place`: that of the warp that begins it,
-// one of each later CTA (of its first warp), and one of the warp that ends it where that
-// is no CTA's first and went on to other ranges (otherwise it joined its neighbours').
-struct Parts {
-  int begin, end, ctas, count;
-  __device__ __forceinline__ Parts(uint32_t place, int units, const Shares& shares) {
-    begin = static_cast<int>(shares.owner(place));
-    end = static_cast<int>(shares.owner(place + units - 1));
-    ctas = end / WARPS - begin / WARPS;
-    const bool went_on = shares.start(end + 1) > place + units + RANGE_COST;
-    count = 1 + ctas + (end % WARPS != 0 && end != begin && went_on ? 1 : 0);
-  }
-  __device__ __forceinline__ int warp(int i) const {
-    return i == 0 ? begin : (i <= ctas ? (begin / WARPS + i) * WARPS : end);
-  }
-};
 
 // Sums of one head, spread over the 16 lanes of half a warp.
 template <int D>
@@ -376,7 +382,7 @@ struct Sums {
 // One head of a range from its parts, written by other SMs: read past L1, some at a time.
 template <int D, int HEADS>
 __device__ __forceinline__ void join_head(const Params& p, const Parts& parts, int64_t out_row, int h, int lane) {
-  constexpr int AHEAD = D == 256 ? 4 : 8;
+  constexpr int AHEAD = 4;
   Sums<D> sums{};
   sums.start();
 #pragma unroll 1
@@ -428,7 +434,7 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attention8_kernel(Params p, 
   __shared__ Piece s_last[WARPS];   // of each warp's last range: the part is in its ring
   __shared__ Piece s_ended[WARPS];  // of its first, which others began: the part is in the workspace
   __shared__ __align__(16) uint32_t s_place[WARPS];
-  __shared__ int s_join[2 * WARPS];
+  __shared__ int s_join[2 * WARPS], s_heads[WARPS];
 
   pdl_begin();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -495,7 +501,7 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attention8_kernel(Params p, 
         run.context = __shfl_sync(0xffffffffu, here, at);
         run.units = units_of<D>(run.context);
         const uint32_t in = u0 - __shfl_sync(0xffffffffu, prior, at) * tiles;
-        const int tile = static_cast<int>(in / static_cast<uint32_t>(run.units + RANGE_COST));
+        const int tile = static_cast<int>(quotient(in, run.units + RANGE_COST));
         run.c = static_cast<int>(in) - tile * (run.units + RANGE_COST);
         run.h = p.head_groups == 1 ? tile : tile / p.head_groups;
         run.hg = tile - run.h * p.head_groups;
@@ -639,6 +645,7 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attention8_kernel(Params p, 
 
   int stage = 0;
   Piece mine{}, ended{};
+  bool alone = false;
   float* const sums = reinterpret_cast<float*>(smem + ring);  // for the last range's part: no tile is left then
   while (run.left > 0) {
     const int length = min(run.units - run.c, run.left);  // units of the range that this warp holds
@@ -872,9 +879,14 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attention8_kernel(Params p, 
       const bool final = run.left <= run.units + RANGE_COST - run.c;  // no other range follows
       float* part = sums;
       if (!whole) {
-        const Piece piece{place0, static_cast<int>(row0), nheads, run.units, run.c == 0, run.c + length == run.units};
+        const Piece piece{place0, static_cast<int>(row0), nheads, run.c == 0, run.c + length == run.units,
+                          Parts(place0, run.units, shares)};
         if (final) {
           mine = piece;
+          // Whether it is the last range of a neighbour in the CTA, too.
+          alone = (warp == 0 || piece.begins) &&
+                  (warp == WARPS - 1 || piece.ends || shares.start(me + 2) > place0 + run.units + RANGE_COST);
+          if (alone) part = part_of<D, HEADS>(p, me, piece.begins);
         } else {  // part 0: it ends its range
           part = part_of<D, HEADS>(p, me, 0);
           ended = piece;
@@ -921,6 +933,7 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attention8_kernel(Params p, 
     s_last[warp] = mine;
     s_ended[warp] = ended;
     s_place[warp] = mine.heads > 0 ? mine.place : ~uint32_t(warp);  // no place: unlike any other
+    s_heads[warp] = alone ? 0 : mine.heads;                          // to join here
     s_join[2 * warp] = s_join[2 * warp + 1] = 0;
   }
   __syncthreads();
@@ -928,10 +941,29 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attention8_kernel(Params p, 
   const uint4 places = *reinterpret_cast<const uint4*>(s_place);
   // Bit w: warp w's last range is that of the warp before.
   const uint32_t joined = (places.x == places.y ? 2u : 0u) | (places.y == places.z ? 4u : 0u) | (places.z == places.w ? 8u : 0u);
+
+  // Lane 2 w + k of warp 0 stands for part k of warp w, if that stands for itself in the
+  // workspace; its range's arrivals are looked at already.
+  bool stands = false;
+  uint64_t seen = 0;
+  uint64_t* word = nullptr;
+  const Piece* piece = nullptr;
+  if (warp == 0 && lane < 2 * WARPS) {
+    const int w = lane >> 1, k = lane & 1;
+    piece = k == 0 && s_ended[w].heads > 0 ? &s_ended[w] : &s_last[w];
+    const int end = __ffs(~joined & (~1u << w)) - 1;  // behind the warps that share warp w's last range
+    const bool first = (joined >> w & 1u) == 0;
+    stands = piece == &s_ended[w] ||
+             (first && piece->heads > 0 && piece->begins == k && !(piece->begins && s_last[end - 1].ends));
+    if (stands) {
+      word = p.arrivals + piece->parts.begin;
+      seen = *reinterpret_cast<volatile uint64_t*>(word);
+    }
+  }
 #pragma unroll 1
   for (int w = 0; w < WARPS;) {
-    const int end = __ffs(~joined & (~1u << w)) - 1;  // behind the warps that share it
-    const int heads = s_last[w].heads;
+    const int end = __ffs(~joined & (~1u << w)) - 1;
+    const int heads = s_heads[w];
     const bool begins = s_last[w].begins, whole = begins && s_last[end - 1].ends;
 #pragma unroll 1
     for (int h = threadIdx.x >> 4; h < heads; h += THREADS / 16) {
@@ -970,36 +1002,14 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attention8_kernel(Params p, 
   }
 
   // ---- ranges that several CTAs, or this one through the workspace, hold parts of.  Every CTA
-  // counts its parts in; the last to come joins them all, in their order.  Lane 2 w + k of
-  // warp 0 stands for part k of warp w.
-  bool stands = false;
-  uint64_t seen = 0;
-  uint64_t* word = nullptr;
-  int count = 0;
-  uint32_t place = 0;
-  if (warp == 0 && lane < 2 * WARPS) {
-    const int w = lane >> 1, k = lane & 1;
-    const bool first = (joined >> w & 1u) == 0;  // of its neighbours
-    const int end = __ffs(~joined & (~1u << w)) - 1;
-    const Piece& last = s_last[w];
-    const Piece& over = s_ended[w];
-    const bool in_ended = k == 0 && over.heads > 0;
-    stands = in_ended || (first && last.heads > 0 && last.begins == k && !(last.begins && s_last[end - 1].ends));
-    if (stands) {
-      place = in_ended ? over.place : last.place;
-      const Parts parts(place, in_ended ? over.units : last.units, shares);
-      count = parts.count;
-      word = p.arrivals + parts.begin;
-      seen = *reinterpret_cast<volatile uint64_t*>(word);
-    }
-  }
+  // counts its parts in; the last to come joins them all, in their order.
   if (!__syncthreads_or(stands)) return;
   bool last_here = false;
   if (stands) {
-    const uint32_t same = __match_any_sync(__activemask(), place);  // this CTA's parts of one range
+    const uint32_t same = __match_any_sync(__activemask(), piece->place);  // this CTA's parts of one range
     if (lane == __ffs(same) - 1) {
       fence_gpu();  // the CTA's parts before their count
-      if (arrive(word, seen, p.tag, __popc(same), count)) {
+      if (arrive(word, seen, p.tag, __popc(same), piece->parts.count)) {
         fence_gpu();  // the count before the parts
         s_join[lane] = 1;
         last_here = true;
@@ -1010,11 +1020,11 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attention8_kernel(Params p, 
 #pragma unroll 1
   for (int i = 0; i < 2 * WARPS; ++i) {
     if (s_join[i] == 0) continue;
-    const Piece piece = (i & 1) == 0 && s_ended[i >> 1].heads > 0 ? s_ended[i >> 1] : s_last[i >> 1];
-    const Parts parts(piece.place, piece.units, shares);
+    const Piece& whose = (i & 1) == 0 && s_ended[i >> 1].heads > 0 ? s_ended[i >> 1] : s_last[i >> 1];
+    const Parts parts = whose.parts;
 #pragma unroll 1
-    for (int h = threadIdx.x >> 4; h < piece.heads; h += THREADS / 16)
-      join_head<D, HEADS>(p, parts, static_cast<int64_t>(piece.row) + h, h, lane & 15);
+    for (int h = threadIdx.x >> 4; h < whose.heads; h += THREADS / 16)
+      join_head<D, HEADS>(p, parts, static_cast<int64_t>(whose.row) + h, h, lane & 15);
   }
 }
 
