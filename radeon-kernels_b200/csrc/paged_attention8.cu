@@ -442,37 +442,32 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attention8_kernel(Params p, 
   const int tiles = p.hkv * p.head_groups;
   const int me = static_cast<int>(blockIdx.x) * WARPS + warp;
 
-  // ---- this warp's share, found 128 sequences at a time (four neighbours to a lane, so that
-  // the loads of a round are in flight together).
+  // ---- this warp's share: a sequence to a lane, 32 at a time, the next lengths under way.
   Walk run{};
   Shares shares;
   uint32_t place0;  // of this warp's range: the place of its first unit
   {
-    constexpr int ROUND = 128;
-    int context[4];
-    uint32_t mine = 0, upto = 0, total = 0;  // places of this lane's sequences, of all up to them, of all
-    const auto round = [&](int base) {
-      Raw raw[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) raw[i] = load_raw(p.lens, p.index_bits, min(base + 4 * lane + i, p.batch - 1));
-      mine = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        context[i] = context_of(p, raw[i]);
-        mine += base + 4 * lane + i < p.batch ? units_of<D>(context[i]) + RANGE_COST : 0;
-      }
-      upto = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t x = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += x;
-      }
+    const auto raw_of = [&](int base) { return load_raw(p.lens, p.index_bits, min(base + lane, p.batch - 1)); };
+    const auto places_of = [&](int base, int context) -> uint32_t {
+      return base + lane < p.batch ? units_of<D>(context) + RANGE_COST : 0;
     };
+    Raw raw = raw_of(0);
+    int context = 0;
+    uint32_t total = 0;
 #pragma unroll 1
-    for (int base = 0; base < p.batch; base += ROUND) {
-      round(base);
-      total += __shfl_sync(0xffffffffu, upto, 31);
+    for (int base = 0; base < p.batch; base += 32) {
+      const Raw next = raw_of(base + 32);
+      context = context_of(p, raw);
+      total += places_of(base, context);
+      raw = next;
     }
+    uint32_t upto = total;  // of the lanes up to this one
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    total = __shfl_sync(0xffffffffu, upto, 31);
     shares.set(total * tiles, gridDim.x * WARPS);
     const bool idle = me >= static_cast<int>(shares.warps);  // fewer places than warps
     const uint32_t u0 = shares.start(idle ? 0 : me);
@@ -480,27 +475,24 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attention8_kernel(Params p, 
     // The sequence that holds place u0.
     uint32_t before = 0;  // places, of one head tile, of earlier rounds
 #pragma unroll 1
-    for (int base = 0; base < p.batch; base += ROUND) {
-      if (p.batch > ROUND) round(base);
+    for (int base = 0; base < p.batch; base += 32) {
+      if (p.batch > 32) {
+        context = context_of(p, raw_of(base));
+        upto = places_of(base, context);
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const uint32_t x = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += x;
+        }
+      }
       const uint32_t past = __ballot_sync(0xffffffffu, (before + upto) * tiles > u0);
       if (past != 0) {
-        // Each lane looks among its own four; the first that has it tells the others.
-        uint32_t prior = before + upto - mine;
-        int i = 0;
-#pragma unroll
-        for (int k = 0; k < 3; ++k) {
-          const uint32_t behind = prior + units_of<D>(context[k]) + RANGE_COST;
-          if (i == k && behind * tiles <= u0) {
-            prior = behind;
-            ++i;
-          }
-        }
-        const int here = i == 0 ? context[0] : i == 1 ? context[1] : i == 2 ? context[2] : context[3];
         const int at = __ffs(past) - 1;
-        run.b = __shfl_sync(0xffffffffu, base + 4 * lane + i, at);
-        run.context = __shfl_sync(0xffffffffu, here, at);
+        run.b = base + at;
+        run.context = __shfl_sync(0xffffffffu, context, at);
         run.units = units_of<D>(run.context);
-        const uint32_t in = u0 - __shfl_sync(0xffffffffu, prior, at) * tiles;
+        const uint32_t prior = before + __shfl_sync(0xffffffffu, upto, at) - (run.units + RANGE_COST);
+        const uint32_t in = u0 - prior * tiles;
         const int tile = static_cast<int>(quotient(in, run.units + RANGE_COST));
         run.c = static_cast<int>(in) - tile * (run.units + RANGE_COST);
         run.h = p.head_groups == 1 ? tile : tile / p.head_groups;
