@@ -463,8 +463,8 @@ RK_API rk_status rk_rotary_embedding(const void* query, const void* key, const v
  *   slot_mapping    [tokens] int64: block * block_size + offset of every new token, the
  *                   requests' tokens one after the other; -1 behind the last;
  *   positions       [tokens]: its position in its request; 0 behind the last;
- *   lengths_out     [batch]: has + gets, at most max_blocks * block_size; may be
- *                   context_lengths only if it is not read again by this step;
+ *   lengths_out     [batch]: has + gets, at most max_blocks * block_size (not the same
+ *                   memory as context_lengths: it is read while this is written);
  *   blocks_used     [1]: entries of free_blocks that the step needs.
  * All index arrays but slot_mapping are int32 or int64 (index_bits).  Where free_blocks is too
  * short, entries and slots that miss a block are -1; tokens past the end of their table row
@@ -485,7 +485,8 @@ RK_API rk_status rk_paged_slots(void* block_tables, const void* context_lengths,
  * Appends new keys and values to a paged cache in 8 bits.  key, value: [tokens, kv_heads,
  * head_dim] of dtype `dt`, with strides between tokens and heads (in elements, multiples of
  * 8; 16-byte aligned); key_cache, value_cache: [num_blocks, block_size, kv_heads, head_dim]
- * of type `cache`; key_scales, value_scales: [num_blocks, kv_heads] fp32; slot_mapping:
+ * of type `cache`; key_scales, value_scales: [num_blocks, kv_heads] fp32, no two of the four
+ * the same memory; slot_mapping:
  * [tokens] int32 or int64 (index_bits), token t's place block * block_size + offset; a
  * negative slot skips the token.  Caches and scales are updated in place.  For each cache,
  * block and head that gets rows:
@@ -526,9 +527,12 @@ RK_API rk_status rk_paged_cache_append_8bit_workspace_size(int64_t tokens, int64
  * reported) as there; any query_heads / kv_heads and any block_size.  Scales are finite and
  * >= 0.  The caches are 16-byte aligned, the query 8-byte.  fp32 scores, softmax and sums;
  * the weights of V are rounded to fp16 (relative to the largest of the head), the output
- * once.  workspace: rk_paged_attention_decode_8bit_workspace_size() bytes, uninitialised, its
- * size independent of batch and lengths; calls that may overlap need one each.  No
- * counterpart in the reference.
+ * once.  The value scales of one head lie within 2^100 of one another, zeros aside.  out does not
+ * overlap an input.  workspace: rk_paged_attention_decode_8bit_workspace_size() bytes, 16-byte
+ * aligned, uninitialised, its size independent of batch and lengths; calls that may overlap
+ * need one each.  max_blocks_per_sequence * block_size < 2^31 - 64, and batch * kv_heads *
+ * (that / 32 + 3), for each started 8 to 16 query heads of a KV head, < 2^32.  No counterpart in
+ * the reference.
  */
 RK_API rk_status rk_paged_attention_decode_8bit(
     const void* query, const void* key_cache, const void* value_cache, const float* key_scales,

@@ -377,7 +377,7 @@ size_t paged_append8_workspace_bytes(int64_t tokens, int64_t num_blocks) {
 rk_status paged_append8_launch(const PagedAppend8Args& a, void* workspace, size_t workspace_bytes, cudaStream_t s) {
   if (a.tokens == 0) return RK_OK;
   const size_t need = paged_append8_workspace_bytes(a.tokens, a.num_blocks);
-  if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return RK_ERR_INVALID_ARGUMENT;
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned16(workspace))) return RK_ERR_INVALID_ARGUMENT;
   LaunchCtl lc;
   const rk_status st = launch_ctl(&lc);
   if (st != RK_OK) return st;

@@ -7,35 +7,48 @@
 // with k_t, v_t the stored 8-bit values of position t and ks, vs the scales of its block and
 // head.  Query head h reads KV head h / (query_heads / kv_heads).
 //
-// Work: the positions of every sequence are cut into units of 64, and the units of all
-// sequences and KV heads, laid end to end, are dealt out evenly: CTA w of W takes the units
-// [w * total / W, (w + 1) * total / W).  So one long sequence among short ones, or few
-// sequences, load every SM alike, whatever the width of the block table.  A CTA writes the
-// (sequence, KV head) ranges that it covers whole; of a range that it shares it leaves the
-// unnormalised sum and its statistics in the workspace, and a second kernel joins the parts in
-// CTA order (no atomics: results do not depend on timing).
+// Work.  The positions of every sequence are cut into units of 32 (16 at head_dim 256), and the
+// units of all sequences and head tiles (a KV head and up to 8 or 16 of its query heads),
+// laid end to end, are dealt out evenly to all warps of the GPU: each takes one stretch.  So one
+// long sequence among short ones, or few sequences, load every SM alike, whatever the width of
+// the block table.  A (sequence, head tile) is a range; RANGE_COST places between ranges stand
+// for what starting and ending one costs.
 //
-// A CTA is 4 warps; a unit is a tile of 16 positions for each, and the warps meet only at
-// the end of a range.  Each warp feeds itself through its own ring of shared memory
-// (cp.async, STAGES tiles of K and V with their scales), which runs on across the ends of
-// ranges.  The matrix products are mma.sync m16n8k16 on f16 operands:
+// A range that a warp holds whole goes to the output from its registers.  Of one that is cut,
+// each warp leaves the unnormalised sums and their statistics: the warps of a CTA join theirs
+// in shared memory, CTAs meet in the workspace, where every CTA counts its parts in and the
+// last to come joins them all, in their order, so that results do not depend on timing.
+// Nothing waits for another CTA.  (A second launch for the join measured 3 to 6 us more on
+// 16 x 2048 positions, and a device-wide fence at each CTA's end 2 us: hence one count
+// and one fence.)
+//
+// A warp feeds itself: a ring of STAGES units of K and V with their scales in shared memory,
+// filled by cp.async and running on across the ends of ranges; block-table entries 32 at a time
+// and queries are loaded a range ahead.  No barrier until the warp's stretch is done.
+//
+// The matrix products are mma.sync m16n8k16 on f16 operands:
 //   S^T[16 positions, 8 heads] = K[16, D] Q^T      O^T[16 dims, 8 heads] += V^T[16 dims, 16] P^T
 // so a KV head's query heads fill the 8 columns, and each 8-bit value is unpacked once, in
 // registers: both E4m3 and Int8 values are f16 numbers, exactly.  The order of a head's
 // dimensions within the products is free; it is chosen such that a lane's operands are 16
-// consecutive bytes of a row.  The 8-query-head tile of a unit needs 16 MMAs per 4 KB of
-// cache (D 128), a few per cent of the tensor pipe, so the products bound nothing; tcgen05
-// would add a round trip through tensor memory and need unpacked operands in shared memory.
+// consecutive bytes of a row, and its results 16 neighbouring dimensions.  16 MMAs go with 4 KB
+// of cache (D 128), a few per cent of the tensor pipe, so the products bound nothing; tcgen05
+// would add a round trip through tensor memory and unpacked operands in shared memory.
 //
-// Numbers: queries are brought to f16 by a power of two per head (exact unless a component is
-// 2^-14 of the head's largest: then it keeps 2^-25 of that).  Scores, maxima, sums and
-// accumulators are fp32.  The weights of V carry its scales, w_t = p_t * vs(t), and are
-// rounded to f16 for the product, relative to a maximum of their own (of s_t + log2 vs(t)), so
-// that the rounding is 2^-12 of the largest terms however the scales differ from block to block.
-// The running maxima are raised only when a value passes them by 2^8; in between p and w
-// may reach 2^8, far inside the range of both types.
+// Numbers.  Queries are brought to f16 by a power of two per head (exact unless a component is
+// below 2^-14 of the head's largest: then it keeps 2^-25 of that).  Scores, maxima, sums and
+// accumulators are fp32.  The weights of V carry its scales, w_t = p_t * vs(t) * c with c =
+// 2^(m - mo) for m the running maximum of the scores s (in powers of two) and mo that of s +
+// log2 vs, and are rounded to f16 for the product: half a step, 2^-11, of each, however the
+// scales differ from block to block, since the largest are near 1.  The maxima are raised
+// only when a weight passes them by SLACK; in between p and w may reach that, far inside the
+// range of both types, and the sums need no rescaling.
 //
-// What bounds it: the bytes of K and V.
+// What bounds it: the bytes of K and V, 1.07 GB in 205 us at 4 x 131072 positions of 8 heads of
+// 128 (5.2 TB/s; the same kernel without the products streams them in 187 us, and some SMs
+// finish their equal share 20 % before others).  At 16 x 2048 positions (67 MB, 21.5 us) the
+// start and the end: 2.2 us until the first loads leave (lengths, then table, then rows: each
+// waits for the one before), 4 us from the last tile to the last join.
 #include <cuda_runtime.h>
 
 #include <atomic>
@@ -51,10 +64,13 @@ namespace pa8 {
 constexpr int WARPS = 4;
 constexpr int THREADS = WARPS * 32;
 constexpr int STAGES = 3;
-constexpr int MAX_CTAS_PER_SM = 4;   // sizes the workspace
 constexpr int RANGE_COST = 2;        // what starting and ending a range costs, in units
 constexpr float SLACK = 256.0f;      // a running maximum is raised when a weight is this much above it
 constexpr float NONE = -3.402823466e38f;  // a maximum before any score: finite, so that -inf - NONE = -inf
+
+// CTAs of an SM that are launched (and that the workspace has room for): 3 fit at head_dim 64, 2
+// otherwise.
+__host__ __device__ constexpr int ctas_per_sm(int head_dim) { return head_dim == 64 ? 3 : 2; }
 
 // Positions of a unit, which is one tile of a warp.
 __host__ __device__ constexpr int unit_of(int head_dim) { return head_dim == 256 ? 16 : 32; }
@@ -102,9 +118,8 @@ struct Params {
   float scale_log2;
 };
 
-// A launch constant, hidden from the compiler, which would otherwise keep a copy of every loop for
-// each value of each flag: 75 KB of code at head_dim 128 instead of KBYTES, and the time to
-// fetch it, in every launch.
+// A launch constant, hidden from the compiler, which would otherwise keep a copy of a loop for each
+// value of each flag (5 KB of 62 at head_dim 128).
 __device__ __forceinline__ int flag_of(int v) {
   asm volatile("" : "+r"(v));
   return v;
@@ -1062,8 +1077,11 @@ rk_status launch(const Params& p, const KernelCtl& ctl, cudaStream_t s) {
   const int64_t ranges = static_cast<int64_t>(p.batch) * p.hkv * p.head_groups;
   const int64_t per_range = (static_cast<int64_t>(p.max_blocks) * p.block_size + unit_of(D) - 1) / unit_of(D);
   // Places are counted in 32 bits.
-  if (ranges > UINT32_MAX / (per_range + RANGE_COST + 1)) return RK_ERR_UNSUPPORTED;
-  int64_t ctas = static_cast<int64_t>(device_sm_count()) * (resident < MAX_CTAS_PER_SM ? resident : MAX_CTAS_PER_SM);
+  if (ranges > UINT32_MAX / (per_range + RANGE_COST + 1)) {
+    note_error("the block tables hold too many positions for one call");
+    return RK_ERR_UNSUPPORTED;
+  }
+  int64_t ctas = static_cast<int64_t>(device_sm_count()) * (resident < ctas_per_sm(D) ? resident : ctas_per_sm(D));
   // Not more warps than units; RANGE_COST places of a range hold none.
   if (ranges <= ctas * WARPS && ranges * (per_range + RANGE_COST) < ctas * WARPS)
     ctas = (ranges * (per_range + RANGE_COST) + WARPS - 1) / WARPS;
@@ -1085,12 +1103,12 @@ rk_status launch_d(const Params& p, int64_t head_dim, int nt, const KernelCtl& c
 
 size_t paged_attention8_workspace_bytes(int64_t hq, int64_t hkv, int64_t head_dim) {
   const pa8::Plan pl = pa8::plan(hq, hkv, head_dim);
-  const size_t warps = static_cast<size_t>(device_sm_count()) * pa8::MAX_CTAS_PER_SM * pa8::WARPS;
+  const size_t warps = static_cast<size_t>(device_sm_count()) * pa8::ctas_per_sm(static_cast<int>(head_dim)) * pa8::WARPS;
   return warps * (sizeof(uint64_t) + 2 * 8 * pl.nt * pa8::part_stride(static_cast<int>(head_dim)) * sizeof(float));
 }
 
 rk_status paged_attention8_launch(const PagedAttention8Args& a, void* workspace, size_t workspace_bytes, cudaStream_t s) {
-  if (workspace == nullptr || workspace_bytes < paged_attention8_workspace_bytes(a.hq, a.hkv, a.head_dim))
+  if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < paged_attention8_workspace_bytes(a.hq, a.hkv, a.head_dim))
     return RK_ERR_INVALID_ARGUMENT;
   LaunchCtl lc;
   const rk_status st = launch_ctl(&lc);
@@ -1107,7 +1125,7 @@ rk_status paged_attention8_launch(const PagedAttention8Args& a, void* workspace,
   p.lens = a.context_lengths;
   p.out = a.out;
   p.arrivals = static_cast<uint64_t*>(workspace);
-  p.part = reinterpret_cast<float*>(p.arrivals + device_sm_count() * pa8::MAX_CTAS_PER_SM * pa8::WARPS);
+  p.part = reinterpret_cast<float*>(p.arrivals + device_sm_count() * pa8::ctas_per_sm(static_cast<int>(a.head_dim)) * pa8::WARPS);
   p.tag = pa8::next_tag();
   p.batch = static_cast<int>(a.batch);
   p.hq = static_cast<int>(a.hq);

@@ -605,6 +605,8 @@ std::vector<at::Tensor> paged_cache_append_8bit(const at::Tensor& key_in, const 
               "slot_mapping must hold one slot per token, on the device of key");
   TORCH_CHECK(key_cache.size(2) == key.size(1) && key_cache.size(3) == key.size(2),
               "key and cache must share heads and head_dim");
+  TORCH_CHECK(key_cache.data_ptr() != value_cache.data_ptr() && key_scales.data_ptr() != value_scales.data_ptr(),
+              "keys and values must have caches and scales of their own");
   size_t ws_bytes = 0;
   check_status(rk_paged_cache_append_8bit_workspace_size(key.size(0), key_cache.size(0), &ws_bytes),
                "rk_paged_cache_append_8bit_workspace_size");

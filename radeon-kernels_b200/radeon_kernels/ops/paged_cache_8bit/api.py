@@ -83,6 +83,8 @@ def _execute_append(key: Any, value: Any, key_cache: Any, value_cache: Any, key_
     args.expect(args.dims("slot_mapping") == (tokens,), "slot_mapping must contain one slot per token")
     args.expect(all(args[n].is_contiguous() for n in ("key_cache", "value_cache", "key_scales", "value_scales",
                                                       "slot_mapping")), "caches, scales and slot_mapping must be contiguous")
+    args.expect(key_cache.data_ptr() != value_cache.data_ptr() and key_scales.data_ptr() != value_scales.data_ptr(),
+                "keys and values must have caches and scales of their own")
     context = args.context(*args.values)
     args.expect(not context.requires_grad, "is inference-only and does not support autograd")
     signature = {
@@ -119,6 +121,7 @@ def _execute_attention(query: Any, key_cache: Any, value_cache: Any, key_scales:
                 "head_dim must match cache and be one of 64, 128, 256")
     args.expect(query_heads % kv_heads == 0, "query_heads must be divisible by kv_heads")
     args.expect(table_rows == batch and max_blocks > 0, "block_tables must have shape [batch, max_blocks]")
+    args.expect(max_blocks * block_size < 2**31 - 64, "max_blocks * block_size must be below 2**31 - 64")
     args.expect(args.dims("context_lengths") == (batch,), "context_lengths must contain one length per sequence")
     context = args.inference_only(*args.values)
     scale_value, scale_mode = args.scale(scale, head_dim)

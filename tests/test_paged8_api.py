@@ -151,12 +151,17 @@ REFUSALS = [
     ("append", dict(**{**_cache_args(), "key_cache": T((10, 2048, 2, 128), "int8"),
                        "value_cache": T((10, 2048, 2, 128), "int8")}), ValueError, "block_size must be at most 1024"),
     ("append", dict(slot_mapping=T((5,), "int64", device=other)), ValueError, "same device"),
+    ("append", (lambda a: dict(value_cache=a["key_cache"], key_cache=a["key_cache"]))(_cache_args()), ValueError,
+     "caches and scales of their own"),
+    ("append", (lambda a: dict(value_scales=a["key_scales"], key_scales=a["key_scales"]))(_cache_args()), ValueError,
+     "caches and scales of their own"),
     ("attention", dict(query=T((3, 8))), ValueError, "query must be rank 3"),
     ("attention", dict(query=T((3, 7, 128))), ValueError, "divisible by kv_heads"),
     ("attention", dict(query=T((3, 8, 64))), ValueError, "head_dim must match cache"),
     ("attention", dict(block_tables=T((2, 4), "int32")), ValueError, "block_tables must have shape"),
     ("attention", dict(block_tables=T((3, 4), "int64")), TypeError, "same dtype"),
     ("attention", dict(context_lengths=T((4,), "int32")), ValueError, "one length per sequence"),
+    ("attention", dict(block_tables=T((3, 2**27), "int32")), ValueError, "below 2"),
     ("attention", dict(query=T((3, 8, 128), contiguous=False)), ValueError, "must be contiguous"),
     ("attention", dict(key_scales=T((10, 2), "float32", requires_grad=True)), ValueError, "inference-only"),
     ("attention", dict(scale=0.0), ValueError, "scale must be positive"),
