@@ -525,14 +525,14 @@ RK_API rk_status rk_paged_cache_append_8bit_workspace_size(int64_t tokens, int64
  * block_tables[b, t / block_size] and g the KV head of h.  Shapes, index types, empty
  * sequences (NaN), clamped lengths and block-table entries out of range (skipped and
  * reported) as there; any query_heads / kv_heads and any block_size.  Scales are finite and
- * >= 0.  The caches are 16-byte aligned, the query 8-byte.  fp32 scores, softmax and sums;
+ * >= 0.  The caches and out are 16-byte aligned, the query 8-byte.  fp32 scores, softmax and sums;
  * the weights of V are rounded to fp16 (relative to the largest of the head), the output
  * once.  The value scales of one head lie within 2^100 of one another, zeros aside.  out does not
  * overlap an input.  workspace: rk_paged_attention_decode_8bit_workspace_size() bytes, 16-byte
  * aligned, uninitialised, its size independent of batch and lengths; calls that may overlap
  * need one each.  max_blocks_per_sequence * block_size < 2^31 - 64, and batch * kv_heads *
- * (that / 32 + 3), for each started 8 to 16 query heads of a KV head, < 2^32.  No counterpart in
- * the reference.
+ * (that / 32 + 3) -- / 16 at head_dim 256 --, for each started 8 to 16 query heads of a KV
+ * head, < 2^31.  No counterpart in the reference.
  */
 RK_API rk_status rk_paged_attention_decode_8bit(
     const void* query, const void* key_cache, const void* value_cache, const float* key_scales,

@@ -579,8 +579,7 @@ rk_status rk_paged_attention_decode_8bit(
   if (query == nullptr || key_cache == nullptr || value_cache == nullptr || key_scales == nullptr ||
       value_scales == nullptr || block_tables == nullptr || context_lengths == nullptr || out == nullptr)
     return RK_ERR_INVALID_ARGUMENT;
-  if ((reinterpret_cast<uintptr_t>(query) & 7u) != 0 || (reinterpret_cast<uintptr_t>(out) & 3u) != 0 ||
-      !aligned16(key_cache) || !aligned16(value_cache))
+  if ((reinterpret_cast<uintptr_t>(query) & 7u) != 0 || !aligned16(out) || !aligned16(key_cache) || !aligned16(value_cache))
     return RK_ERR_UNSUPPORTED;
   // Positions of a unit's last tile stay below 2^31.
   if (num_blocks > INT32_MAX || block_size > INT32_MAX || max_blocks > INT32_MAX ||

@@ -304,6 +304,10 @@ def test_c_entries_check_their_arguments():
         assert attention(**changes) == bad, changes
     for changes in (dict(width=2**21, size=2**10), dict(p=ctypes.c_void_p(264 + 4))):
         assert attention(**{"p": some, **changes}) == no, changes
+    for at, offset in ((0, 4), (1, 8), (2, 8), (7, 8)):  # query; caches; output
+        pointers = [some] * 8
+        pointers[at] = ctypes.c_void_p(256 + offset)
+        assert lib.rk_paged_attention_decode_8bit(*pointers, 1, 2, 1, 64, 1, 16, 1, 1.0, 1, 0, 32, null, 0, null) == no, at
     assert lib.rk_paged_attention_decode_8bit_workspace_size(3, 2, 64, ctypes.byref(size)) == bad and size.value == 0
     assert lib.rk_paged_attention_decode_8bit_workspace_size(2, 2, 64, None) == bad
 
