@@ -8,8 +8,8 @@
 // head.  Query head h reads KV head h / (query_heads / kv_heads).
 //
 // Work.  The positions of every sequence are cut into units of 32 (16 at head_dim 256), and the
-// units of all sequences and head tiles (a KV head and up to 8 or 16 of its query heads),
-// laid end to end, are dealt out evenly to all warps of the GPU: each takes one stretch.  So one
+// units of all sequences and head tiles (a KV head and up to 8 or 16 of its query heads), laid
+// end to end, are dealt out evenly to all warps of the GPU: each takes one stretch.  So one
 // long sequence among short ones, or few sequences, load every SM alike, whatever the width of
 // the block table.  A (sequence, head tile) is a range; RANGE_COST places between ranges stand
 // for what starting and ending one costs.
@@ -95,7 +95,7 @@ struct Layout {
   }
 };
 
-// A part in the workspace: per head the unnormalised sum, then m, mo and l.
+// A head's part in the workspace: the unnormalised sum, then m, mo, l and nothing.
 __host__ __device__ constexpr int part_stride(int head_dim) { return head_dim + 4; }
 
 struct Params {
@@ -110,7 +110,7 @@ struct Params {
   float* part;      // [warp][2][heads of a tile][part_stride]: part 0 continues a range, part 1 begins one
   uint64_t* arrivals;  // [warp]: `tag` plus the parts written of the range that the warp begins; or anything
   uint64_t tag;        // of this launch; its low 16 bits are 0, the others not all
-  int batch, hq, hkv, group, head_groups, tile_heads;
+  int batch, hq, hkv, group, head_groups;
   int num_blocks, block_size, max_blocks;
   uint32_t block_multiplier;  // t / block_size = t * block_multiplier >> block_shift for t < 2^31
   int block_shift;
@@ -661,185 +661,207 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attention8_kernel(Params p, 
     const int64_t row0 = static_cast<int64_t>(run.b) * p.hq + head0;
     if (!QUERIES_AHEAD && place0 != place_first) load_queries(run.b, run.h, run.hg);
     uint32_t qf[NT][4 * KC][2];
-      float factor[NT][2];
-      float o[NT][MT][4];
-      float m[NT][2], mo[NT][2], c[NT][2], l[NT][2];  // of heads 2 c4, 2 c4 + 1: c = 2^(m - mo)
-      const int bf16 = flag_of(p.bf16);
+    float factor[NT][2];
+    float o[NT][MT][4];
+    float m[NT][2], mo[NT][2], c[NT][2], l[NT][2];  // of heads 2 c4, 2 c4 + 1: c = 2^(m - mo)
+    const int bf16 = flag_of(p.bf16);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float f[4 * KC][4];
-        float amax = 0.f;
+    for (int nt = 0; nt < NT; ++nt) {
+      float f[4 * KC][4];
+      float amax = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4 * KC; ++j) {
-          const uint2 raw = queries[nt][j];
-          const float2 a = bf16 ? Pack2<__nv_bfloat16>::to_floats(raw.x) : Pack2<__half>::to_floats(raw.x);
-          const float2 b = bf16 ? Pack2<__nv_bfloat16>::to_floats(raw.y) : Pack2<__half>::to_floats(raw.y);
-          f[j][0] = a.x;
-          f[j][1] = a.y;
-          f[j][2] = b.x;
-          f[j][3] = b.y;
+      for (int j = 0; j < 4 * KC; ++j) {
+        const uint2 raw = queries[nt][j];
+        const float2 a = bf16 ? Pack2<__nv_bfloat16>::to_floats(raw.x) : Pack2<__half>::to_floats(raw.x);
+        const float2 b = bf16 ? Pack2<__nv_bfloat16>::to_floats(raw.y) : Pack2<__half>::to_floats(raw.y);
+        f[j][0] = a.x;
+        f[j][1] = a.y;
+        f[j][2] = b.x;
+        f[j][3] = b.y;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) amax = fmaxf(amax, fabsf(f[j][e]));
-        }
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-        // 2^-e with 2^e <= amax < 2^(e+1), kept where both it and its inverse are normal.
-        const int e = min(max(static_cast<int>(__float_as_uint(amax) >> 23), 2), 252);
-        const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
-        const float up = __uint_as_float(static_cast<uint32_t>(e) << 23) * p.scale_log2;
-#pragma unroll
-        for (int j = 0; j < 4 * KC; ++j) {
-          qf[nt][j][0] = Pack2<__half>::from_floats(f[j][0] * down, f[j][1] * down);
-          qf[nt][j][1] = Pack2<__half>::from_floats(f[j][2] * down, f[j][3] * down);
-        }
-        // Lane (g, c4) holds the scores of heads 2 c4 and 2 c4 + 1.
-        factor[nt][0] = __shfl_sync(0xffffffffu, up, 8 * c4);
-        factor[nt][1] = __shfl_sync(0xffffffffu, up, 8 * c4 + 4);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          m[nt][i] = mo[nt][i] = NONE;
-          l[nt][i] = c[nt][i] = 0.f;
-        }
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[nt][mt][i] = 0.f;
+        for (int e = 0; e < 4; ++e) amax = fmaxf(amax, fabsf(f[j][e]));
       }
-
-      if (QUERIES_AHEAD && run.left > run.units + RANGE_COST - run.c) {
-        const bool more = run.hg + 1 < p.head_groups, same = more || run.h + 1 < p.hkv;
-        load_queries(same ? run.b : run.b + 1, more ? run.h : same ? run.h + 1 : 0, more ? run.hg + 1 : 0);
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      // 2^-e with 2^e <= amax < 2^(e+1), kept where both it and its inverse are normal.
+      const int e = min(max(static_cast<int>(__float_as_uint(amax) >> 23), 2), 252);
+      const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
+      const float up = __uint_as_float(static_cast<uint32_t>(e) << 23) * p.scale_log2;
+#pragma unroll
+      for (int j = 0; j < 4 * KC; ++j) {
+        qf[nt][j][0] = Pack2<__half>::from_floats(f[j][0] * down, f[j][1] * down);
+        qf[nt][j][1] = Pack2<__half>::from_floats(f[j][2] * down, f[j][3] * down);
       }
+      // Lane (g, c4) holds the scores of heads 2 c4 and 2 c4 + 1.
+      factor[nt][0] = __shfl_sync(0xffffffffu, up, 8 * c4);
+      factor[nt][1] = __shfl_sync(0xffffffffu, up, 8 * c4 + 4);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        m[nt][i] = mo[nt][i] = NONE;
+        l[nt][i] = c[nt][i] = 0.f;
+      }
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[nt][mt][i] = 0.f;
+    }
 
-      for (int step = 0; step < length; ++step) {
-        cp_async_wait<STAGES - 1>();
-        __syncwarp();
-        const uint8_t* tile = smem + ring + stage * L::STAGE;
-        const uint32_t mask = at_smem<uint32_t>(tile, L::MASK);
-        if (mask != 0) {
-          float s[NT][SUB][4], s2[NT][SUB][4];  // two chains of products: half the latency
+    if (QUERIES_AHEAD && run.left > run.units + RANGE_COST - run.c) {
+      const bool more = run.hg + 1 < p.head_groups, same = more || run.h + 1 < p.hkv;
+      load_queries(same ? run.b : run.b + 1, more ? run.h : same ? run.h + 1 : 0, more ? run.hg + 1 : 0);
+    }
+
+    for (int step = 0; step < length; ++step) {
+      cp_async_wait<STAGES - 1>();
+      __syncwarp();
+      const uint8_t* tile = smem + ring + stage * L::STAGE;
+      const uint32_t mask = at_smem<uint32_t>(tile, L::MASK);
+      if (mask != 0) {
+        float s[NT][SUB][4], s2[NT][SUB][4];  // two chains of products: half the latency
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int t = 0; t < SUB; ++t)
+          for (int t = 0; t < SUB; ++t)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) s[nt][t][i] = s2[nt][t][i] = 0.f;
+            for (int i = 0; i < 4; ++i) s[nt][t][i] = s2[nt][t][i] = 0.f;
 #pragma unroll
-          for (int i = 0; i < KC; ++i) {
-#pragma unroll
-            for (int t = 0; t < SUB; ++t) {
-              const int at = (k_lane ^ ((i & 1) * 16)) + (i >> 1) * 128 + 16 * t * D;
-              const uint4 ka = at_smem<uint4>(tile, at), kb = at_smem<uint4>(tile, at + 8 * D);
-              const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                uint32_t a0, a1, a2, a3;
-                C::halves(wa[j], a0, a2);
-                C::halves(wb[j], a1, a3);
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-                  mma16816((j & 1) ? s2[nt][t] : s[nt][t], a0, a1, a2, a3, qf[nt][4 * i + j][0], qf[nt][4 * i + j][1]);
-              }
-            }
-          }
-          // Rows g and g + 8 of each 16: p = 2^(score - m), and the weights of V, w = p * vs * c.
-          float weight[NT][SUB][4];
-          float most = 0.f;
+        for (int i = 0; i < KC; ++i) {
 #pragma unroll
           for (int t = 0; t < SUB; ++t) {
+            const int at = (k_lane ^ ((i & 1) * 16)) + (i >> 1) * 128 + 16 * t * D;
+            const uint4 ka = at_smem<uint4>(tile, at), kb = at_smem<uint4>(tile, at + 8 * D);
+            const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              const int row = 16 * t + 8 * r + g;
-              const float ks = at_smem<float>(tile, L::SCALES + row * 4), vs = at_smem<float>(tile, L::SCALES + (TILE + row) * 4);
+            for (int j = 0; j < 4; ++j) {
+              uint32_t a0, a1, a2, a3;
+              C::halves(wa[j], a0, a2);
+              C::halves(wb[j], a1, a3);
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                  const int e = 2 * r + i;
-                  s[nt][t][e] += s2[nt][t][e];
-                  float x = fmaf(s[nt][t][e], ks * factor[nt][i], -m[nt][i]);
-                  if (mask != FULL && !((mask >> row) & 1u)) x = -INFINITY;
-                  const float pw = ex2_approx(x);
-                  s2[nt][t][e] = pw;
-                  weight[nt][t][e] = pw * (vs * c[nt][i]);
-                  most = fmax3(most, pw, weight[nt][t][e]);
-                }
-              }
+              for (int nt = 0; nt < NT; ++nt)
+                mma16816((j & 1) ? s2[nt][t] : s[nt][t], a0, a1, a2, a3, qf[nt][4 * i + j][0], qf[nt][4 * i + j][1]);
             }
           }
-          if (__any_sync(0xffffffffu, most > SLACK)) {
-            // The maxima are raised to what they have become, and all sums brought to them.
+        }
+        // Rows g and g + 8 of each 16: p = 2^(score - m), and the weights of V, w = p * vs * c.
+        float weight[NT][SUB][4];
+        float most = 0.f;
+#pragma unroll
+        for (int t = 0; t < SUB; ++t) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const int row = 16 * t + 8 * r + g;
+            const float ks = at_smem<float>(tile, L::SCALES + row * 4), vs = at_smem<float>(tile, L::SCALES + (TILE + row) * 4);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
               for (int i = 0; i < 2; ++i) {
-                float bm = m[nt][i], bo = mo[nt][i];
+                const int e = 2 * r + i;
+                s[nt][t][e] += s2[nt][t][e];
+                float x = fmaf(s[nt][t][e], ks * factor[nt][i], -m[nt][i]);
+                if (mask != FULL && !((mask >> row) & 1u)) x = -INFINITY;
+                const float pw = ex2_approx(x);
+                s2[nt][t][e] = pw;
+                weight[nt][t][e] = pw * (vs * c[nt][i]);
+                most = fmax3(most, pw, weight[nt][t][e]);
+              }
+            }
+          }
+        }
+        if (__any_sync(0xffffffffu, most > SLACK)) {
+          // The maxima are raised to what they have become, and all sums brought to them.
 #pragma unroll
-                for (int t = 0; t < SUB; ++t) {
+          for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-                  for (int r = 0; r < 2; ++r) {
-                    const int row = 16 * t + 8 * r + g;
-                    const float ks = at_smem<float>(tile, L::SCALES + row * 4), vs = at_smem<float>(tile, L::SCALES + (TILE + row) * 4);
-                    const float x = (mask >> row) & 1u ? s[nt][t][2 * r + i] * (ks * factor[nt][i]) : -INFINITY;
-                    bm = fmaxf(bm, x);
-                    bo = fmaxf(bo, x + lg2_approx(vs));
-                  }
+            for (int i = 0; i < 2; ++i) {
+              float bm = m[nt][i], bo = mo[nt][i];
+#pragma unroll
+              for (int t = 0; t < SUB; ++t) {
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                  const int row = 16 * t + 8 * r + g;
+                  const float ks = at_smem<float>(tile, L::SCALES + row * 4), vs = at_smem<float>(tile, L::SCALES + (TILE + row) * 4);
+                  const float x = (mask >> row) & 1u ? s[nt][t][2 * r + i] * (ks * factor[nt][i]) : -INFINITY;
+                  bm = fmaxf(bm, x);
+                  bo = fmaxf(bo, x + lg2_approx(vs));
                 }
+              }
 #pragma unroll
-                for (int x = 4; x < 32; x <<= 1) {
-                  bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, x));
-                  bo = fmaxf(bo, __shfl_xor_sync(0xffffffffu, bo, x));
-                }
-                // c = 2^(m - mo), kept within fp32 (scales of 2^-126, or none but zeros).
-                bo = bm - fminf(bm - bo, 126.f);
-                l[nt][i] *= ex2_approx(m[nt][i] - bm);
-                const float down = ex2_approx(mo[nt][i] - bo);
-                c[nt][i] = ex2_approx(bm - bo);
-                m[nt][i] = bm;
-                mo[nt][i] = bo;
+              for (int x = 4; x < 32; x <<= 1) {
+                bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, x));
+                bo = fmaxf(bo, __shfl_xor_sync(0xffffffffu, bo, x));
+              }
+              // c = 2^(m - mo) and its inverse are kept normal numbers, for ex2.approx flushes the others
+              // (scales of 2^127 or 2^-126, or none but zeros).
+              bo = bm - fminf(fmaxf(bm - bo, -125.f), 125.f);
+              l[nt][i] *= ex2_approx(m[nt][i] - bm);
+              const float down = ex2_approx(mo[nt][i] - bo);
+              c[nt][i] = ex2_approx(bm - bo);
+              m[nt][i] = bm;
+              mo[nt][i] = bo;
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                  o[nt][mt][i] *= down;
-                  o[nt][mt][i + 2] *= down;
-                }
+              for (int mt = 0; mt < MT; ++mt) {
+                o[nt][mt][i] *= down;
+                o[nt][mt][i + 2] *= down;
+              }
 #pragma unroll
-                for (int t = 0; t < SUB; ++t) {
+              for (int t = 0; t < SUB; ++t) {
 #pragma unroll
-                  for (int r = 0; r < 2; ++r) {
-                    const int row = 16 * t + 8 * r + g;
-                    const float ks = at_smem<float>(tile, L::SCALES + row * 4), vs = at_smem<float>(tile, L::SCALES + (TILE + row) * 4);
-                    float x = fmaf(s[nt][t][2 * r + i], ks * factor[nt][i], -bm);
-                    if (!((mask >> row) & 1u)) x = -INFINITY;
-                    s2[nt][t][2 * r + i] = ex2_approx(x);
-                    weight[nt][t][2 * r + i] = s2[nt][t][2 * r + i] * (vs * c[nt][i]);
-                  }
+                for (int r = 0; r < 2; ++r) {
+                  const int row = 16 * t + 8 * r + g;
+                  const float ks = at_smem<float>(tile, L::SCALES + row * 4), vs = at_smem<float>(tile, L::SCALES + (TILE + row) * 4);
+                  float x = fmaf(s[nt][t][2 * r + i], ks * factor[nt][i], -bm);
+                  if (!((mask >> row) & 1u)) x = -INFINITY;
+                  s2[nt][t][2 * r + i] = ex2_approx(x);
+                  weight[nt][t][2 * r + i] = s2[nt][t][2 * r + i] * (vs * c[nt][i]);
                 }
               }
             }
           }
-          uint32_t pf[NT][SUB][2];
+        }
+        uint32_t pf[NT][SUB][2];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-            for (int t = 0; t < SUB; ++t) {
-#pragma unroll
-              for (int i = 0; i < 4; ++i) l[nt][i & 1] += s2[nt][t][i];
-              pf[nt][t][0] = transpose8x8(Pack2<__half>::from_floats(weight[nt][t][0], weight[nt][t][1]));
-              pf[nt][t][1] = transpose8x8(Pack2<__half>::from_floats(weight[nt][t][2], weight[nt][t][3]));
-            }
-          }
-          // V^T: a lane's 16 (D 64: 8) bytes of positions 2 c4, 2 c4 + 1, and those + 8, byte by
-          // byte side by side, are two rows of the operand.
+        for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
           for (int t = 0; t < SUB; ++t) {
-            if (D == 64) {
-              const int row = 16 * t + 2 * c4;
-              const int at = L::K_BYTES + g * 8;
-              const uint2 va = at_smem<uint2>(tile, at + row * L::V_STRIDE), vb = at_smem<uint2>(tile, at + (row + 1) * L::V_STRIDE);
-              const uint2 vc = at_smem<uint2>(tile, at + (row + 8) * L::V_STRIDE), vd = at_smem<uint2>(tile, at + (row + 9) * L::V_STRIDE);
-              const uint32_t w0[2] = {va.x, va.y}, w1[2] = {vb.x, vb.y}, w2[2] = {vc.x, vc.y}, w3[2] = {vd.x, vd.y};
 #pragma unroll
-              for (int j = 0; j < 2; ++j) {
+            for (int i = 0; i < 4; ++i) l[nt][i & 1] += s2[nt][t][i];
+            pf[nt][t][0] = transpose8x8(Pack2<__half>::from_floats(weight[nt][t][0], weight[nt][t][1]));
+            pf[nt][t][1] = transpose8x8(Pack2<__half>::from_floats(weight[nt][t][2], weight[nt][t][3]));
+          }
+        }
+        // V^T: a lane's 16 (D 64: 8) bytes of positions 2 c4, 2 c4 + 1, and those + 8, byte by
+        // byte side by side, are two rows of the operand.
+#pragma unroll
+        for (int t = 0; t < SUB; ++t) {
+          if (D == 64) {
+            const int row = 16 * t + 2 * c4;
+            const int at = L::K_BYTES + g * 8;
+            const uint2 va = at_smem<uint2>(tile, at + row * L::V_STRIDE), vb = at_smem<uint2>(tile, at + (row + 1) * L::V_STRIDE);
+            const uint2 vc = at_smem<uint2>(tile, at + (row + 8) * L::V_STRIDE), vd = at_smem<uint2>(tile, at + (row + 9) * L::V_STRIDE);
+            const uint32_t w0[2] = {va.x, va.y}, w1[2] = {vb.x, vb.y}, w2[2] = {vc.x, vc.y}, w3[2] = {vd.x, vd.y};
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                const uint32_t pick = x == 0 ? 0x5140u : 0x7362u;
+                uint32_t a0, a1, a2, a3;
+                C::halves(__byte_perm(w0[j], w1[j], pick), a0, a1);
+                C::halves(__byte_perm(w2[j], w3[j], pick), a2, a3);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+                  mma16816(o[nt][(2 * j + x) % MT], a0, a1, a2, a3, pf[nt][t][0], pf[nt][t][1]);
+              }
+            }
+          } else {
+#pragma unroll
+            for (int h = 0; h < D / 128; ++h) {
+              const int at = v_lane + h * 128 + 16 * t * D, next = (v_lane ^ 16) + h * 128 + (16 * t + 1) * D;
+              const uint4 va = at_smem<uint4>(tile, at), vb = at_smem<uint4>(tile, next);
+              const uint4 vc = at_smem<uint4>(tile, at + 8 * D), vd = at_smem<uint4>(tile, next + 8 * D);
+              const uint32_t w0[4] = {va.x, va.y, va.z, va.w}, w1[4] = {vb.x, vb.y, vb.z, vb.w};
+              const uint32_t w2[4] = {vc.x, vc.y, vc.z, vc.w}, w3[4] = {vd.x, vd.y, vd.z, vd.w};
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
                   const uint32_t pick = x == 0 ? 0x5140u : 0x7362u;
@@ -848,88 +870,67 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attention8_kernel(Params p, 
                   C::halves(__byte_perm(w2[j], w3[j], pick), a2, a3);
 #pragma unroll
                   for (int nt = 0; nt < NT; ++nt)
-                    mma16816(o[nt][(2 * j + x) % MT], a0, a1, a2, a3, pf[nt][t][0], pf[nt][t][1]);
+                    mma16816(o[nt][(8 * h + 2 * j + x) % MT], a0, a1, a2, a3, pf[nt][t][0], pf[nt][t][1]);
                 }
               }
+            }
+          }
+        }
+      }
+      __syncwarp();  // the tile is read
+      load_next(stage);
+      stage = stage + 1 == STAGES ? 0 : stage + 1;
+    }
+
+    // The end of a range.  A lane holds 16 (D 64: 8) neighbouring dimensions of two heads.
+    const bool whole = length == run.units;
+    const bool final = run.left <= run.units + RANGE_COST - run.c;  // no other range follows
+    float* part = sums;
+    if (!whole) {
+      const Piece piece{place0, static_cast<int>(row0), nheads, run.c == 0, run.c + length == run.units,
+                        Parts(place0, run.units, shares)};
+      if (final) {
+        mine = piece;
+        // Whether it is the last range of a neighbour in the CTA, too.
+        alone = (warp == 0 || piece.begins) &&
+                (warp == WARPS - 1 || piece.ends || shares.start(me + 2) > place0 + run.units + RANGE_COST);
+        if (alone) part = part_of<D, HEADS>(p, me, piece.begins);
+      } else {  // part 0: it ends its range
+        part = part_of<D, HEADS>(p, me, 0);
+        ended = piece;
+      }
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) l[nt][i] += __shfl_xor_sync(0xffffffffu, l[nt][i], x);
+        const int h = nt * 8 + 2 * c4 + i;
+        constexpr int N = D == 64 ? 8 : 16;
+        if (h < nheads) {
+          float* row = part + h * part_stride(D);
+          const float f = last_factor(m[nt][i], mo[nt][i], l[nt][i]);
+#pragma unroll
+          for (int k = 0; k < MT * 2 / N; ++k) {
+            float v[N];
+#pragma unroll
+            for (int j = 0; j < N / 2; ++j) {
+              v[2 * j] = o[nt][k * (N / 2) + j][i];
+              v[2 * j + 1] = o[nt][k * (N / 2) + j][i + 2];
+            }
+            const int d = N * g + 128 * k;
+            if (whole) {
+              write_out<N>(p, (row0 + h) * D + d, v, f);
             } else {
 #pragma unroll
-              for (int h = 0; h < D / 128; ++h) {
-                const int at = v_lane + h * 128 + 16 * t * D, next = (v_lane ^ 16) + h * 128 + (16 * t + 1) * D;
-                const uint4 va = at_smem<uint4>(tile, at), vb = at_smem<uint4>(tile, next);
-                const uint4 vc = at_smem<uint4>(tile, at + 8 * D), vd = at_smem<uint4>(tile, next + 8 * D);
-                const uint32_t w0[4] = {va.x, va.y, va.z, va.w}, w1[4] = {vb.x, vb.y, vb.z, vb.w};
-                const uint32_t w2[4] = {vc.x, vc.y, vc.z, vc.w}, w3[4] = {vd.x, vd.y, vd.z, vd.w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-#pragma unroll
-                  for (int x = 0; x < 2; ++x) {
-                    const uint32_t pick = x == 0 ? 0x5140u : 0x7362u;
-                    uint32_t a0, a1, a2, a3;
-                    C::halves(__byte_perm(w0[j], w1[j], pick), a0, a1);
-                    C::halves(__byte_perm(w2[j], w3[j], pick), a2, a3);
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-                      mma16816(o[nt][(8 * h + 2 * j + x) % MT], a0, a1, a2, a3, pf[nt][t][0], pf[nt][t][1]);
-                  }
-                }
-              }
+              for (int j = 0; j < N / 4; ++j)
+                reinterpret_cast<float4*>(row + d)[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
             }
           }
-        }
-        __syncwarp();  // the tile is read
-        load_next(stage);
-        stage = stage + 1 == STAGES ? 0 : stage + 1;
-      }
-
-      // The end of a range.  A lane holds 16 (D 64: 8) neighbouring dimensions of two heads.
-      const bool whole = length == run.units;
-      const bool final = run.left <= run.units + RANGE_COST - run.c;  // no other range follows
-      float* part = sums;
-      if (!whole) {
-        const Piece piece{place0, static_cast<int>(row0), nheads, run.c == 0, run.c + length == run.units,
-                          Parts(place0, run.units, shares)};
-        if (final) {
-          mine = piece;
-          // Whether it is the last range of a neighbour in the CTA, too.
-          alone = (warp == 0 || piece.begins) &&
-                  (warp == WARPS - 1 || piece.ends || shares.start(me + 2) > place0 + run.units + RANGE_COST);
-          if (alone) part = part_of<D, HEADS>(p, me, piece.begins);
-        } else {  // part 0: it ends its range
-          part = part_of<D, HEADS>(p, me, 0);
-          ended = piece;
+          if (!whole && g == 0) *reinterpret_cast<float4*>(row + D) = make_float4(m[nt][i], mo[nt][i], l[nt][i], 0.f);
         }
       }
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-#pragma unroll
-          for (int x = 4; x < 32; x <<= 1) l[nt][i] += __shfl_xor_sync(0xffffffffu, l[nt][i], x);
-          const int h = nt * 8 + 2 * c4 + i;
-          constexpr int N = D == 64 ? 8 : 16;
-          if (h < nheads) {
-            float* row = part + h * part_stride(D);
-            const float f = last_factor(m[nt][i], mo[nt][i], l[nt][i]);
-#pragma unroll
-            for (int k = 0; k < MT * 2 / N; ++k) {
-              float v[N];
-#pragma unroll
-              for (int j = 0; j < N / 2; ++j) {
-                v[2 * j] = o[nt][k * (N / 2) + j][i];
-                v[2 * j + 1] = o[nt][k * (N / 2) + j][i + 2];
-              }
-              const int d = N * g + 128 * k;
-              if (whole) {
-                write_out<N>(p, (row0 + h) * D + d, v, f);
-              } else {
-#pragma unroll
-                for (int j = 0; j < N / 4; ++j)
-                  reinterpret_cast<float4*>(row + d)[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-              }
-            }
-            if (!whole && g == 0) *reinterpret_cast<float4*>(row + D) = make_float4(m[nt][i], mo[nt][i], l[nt][i], 0.f);
-          }
-        }
     place0 += run.units + RANGE_COST;
     next_range<D>(p, run);
   }
@@ -1076,8 +1077,8 @@ rk_status launch(const Params& p, const KernelCtl& ctl, cudaStream_t s) {
   }
   const int64_t ranges = static_cast<int64_t>(p.batch) * p.hkv * p.head_groups;
   const int64_t per_range = (static_cast<int64_t>(p.max_blocks) * p.block_size + unit_of(D) - 1) / unit_of(D);
-  // Places are counted in 32 bits.
-  if (ranges > UINT32_MAX / (per_range + RANGE_COST + 1)) {
+  // Places are counted in 32 bits, and a warp's share stays below 2^21 of them (see quotient).
+  if (ranges > INT32_MAX / (per_range + RANGE_COST)) {
     note_error("the block tables hold too many positions for one call");
     return RK_ERR_UNSUPPORTED;
   }
@@ -1132,7 +1133,6 @@ rk_status paged_attention8_launch(const PagedAttention8Args& a, void* workspace,
   p.hkv = static_cast<int>(a.hkv);
   p.group = static_cast<int>(a.hq / a.hkv);
   p.head_groups = pl.head_groups;
-  p.tile_heads = 8 * pl.nt;
   p.num_blocks = static_cast<int>(a.num_blocks);
   p.block_size = static_cast<int>(a.block_size);
   p.max_blocks = static_cast<int>(a.max_blocks);

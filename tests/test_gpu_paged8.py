@@ -156,6 +156,13 @@ def test_repeated_slots_and_blocks_are_refused(tokens):
         _append(rng, _rows(rng, tokens, 2, 64, "bf16"), slots + tail, "int8", blocks, size)
 
 
+def test_many_runs_of_one_block():
+    """Each of thousands of tokens starts a run of the same block; one comes back to it much later."""
+    rng = np.random.default_rng(8)
+    _append(rng, _rows(rng, 2400, 2, 64, "bf16"), [37] * 2400, "int8", 4, 16)
+    _append(rng, _rows(rng, 2400, 2, 64, "bf16"), [37] + [-1] * 2380 + [38, 39] + [-1] * 16 + [5], "e4m3", 4, 16)
+
+
 @pytest.mark.parametrize("tokens", [5, 2500], ids=["scan", "claims"])
 def test_slots_outside_the_cache(tokens):
     rng = np.random.default_rng(5)
@@ -403,6 +410,14 @@ def test_scales_far_apart(kind):
                     else:
                         p.scales[0][block] *= 2.0 ** (j - 4)
         p.check(p.run())
+
+
+@pytest.mark.parametrize("exponent", [-126, -120, 120, 127])
+def test_value_scales_at_the_ends_of_fp32(exponent):
+    p = Problem([1, 45, 300], 8, 2, 128, 16, "bf16", "int8", seed=31)
+    p.caches[1].clamp_(-1, 1)  # the output stays finite
+    p.scales[1].fill_(2.0**exponent)
+    p.check(p.run())
 
 
 def test_all_value_scales_zero():
