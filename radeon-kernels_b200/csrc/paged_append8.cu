@@ -28,9 +28,9 @@
 // whatever they held is checked against the slots.
 //
 // What bounds it.  A decode step: launch and latency (a token each of 128 requests, 8 heads of
-// 128: 4.7 us on the device).  A prefill: the bytes, 2 in and 1 out per element (55k tokens
-// of 8 heads of 128 in bf16: 265 MB in 51 us, 5.2 TB/s, after 4.7 us for the list; 13k tokens
-// of 4 heads: 10.5 us with the list).
+// 128: 4.7 us on the device).  A prefill: the bytes, 2 in and 1 out per element (43k
+// tokens of 8 heads of 128 in bf16: 265 MB in 51 us, 5.2 TB/s, after 4.7 us for the list; 13k
+// tokens of 4 heads of 64: 10.5 us with the list).
 #include <cuda_runtime.h>
 
 #include "rk_cache8.cuh"

@@ -11,8 +11,9 @@
 // another.  New entries are taken from the free list by both the CTA that writes them and
 // those that need them; entries of blocks that a request had are only read.
 //
-// What bounds it: launch and memory latency (two dependent loads) for a decode step, the
-// bytes of the slot map and positions for a prefill.
+// What bounds it: launch and latency -- lengths, scan, table or free list, slot -- at all sizes of
+// use (a token each of 256 requests 3.3 us on the device, 64k tokens of 61 requests 4.4 us for
+// 1 MB written).
 #include <cuda_runtime.h>
 
 #include "rk_device.cuh"
@@ -88,21 +89,26 @@ __global__ void __launch_bounds__(THREADS) paged_slots_kernel(SlotParams<Index> 
     const int64_t want = (end + p.block_size - 1) / p.block_size;
     int64_t tokens = gets, blocks = want - old;
     scan2(tokens, blocks, warp_sums);
+    const int64_t first = free_base + blocks - (want - old);
     s_end[threadIdx.x] = token_base + tokens;
     s_has[threadIdx.x] = has;
-    s_first[threadIdx.x] = free_base + blocks - (want - old);
+    s_first[threadIdx.x] = first;
     s_old[threadIdx.x] = old;
     s_want[threadIdx.x] = want;
     __syncthreads();
     const int n = static_cast<int>(min(static_cast<int64_t>(THREADS), p.batch - base));
     if (blockIdx.x == 0 && r < p.batch) p.lengths[r] = static_cast<Index>(end);
-    // Table rows: a warp per request of this CTA's share.
-    for (int i = blockIdx.x + gridDim.x * (threadIdx.x >> 5); i < n; i += gridDim.x * (THREADS / 32)) {
-      for (int64_t j = s_old[i] + (threadIdx.x & 31); j < s_want[i]; j += 32) {
-        const int64_t at = s_first[i] + j - s_old[i];
-        if (at >= p.free_count) bad = true;
-        p.tables[(base + i) * p.max_blocks + j] = at < p.free_count ? p.free_blocks[at] : static_cast<Index>(-1);
-      }
+    // Table rows of this CTA's share of the requests.  Most steps give a request one block or
+    // none: a thread writes that of its own; the further ones a warp writes together.
+    const auto entry = [&](int64_t request, int64_t j, int64_t at) {
+      if (at >= p.free_count) bad = true;
+      p.tables[request * p.max_blocks + j] = at < p.free_count ? p.free_blocks[at] : static_cast<Index>(-1);
+    };
+    const bool mine = r < p.batch && threadIdx.x % gridDim.x == blockIdx.x;
+    if (mine && want > old) entry(r, old, first);
+    for (uint32_t more = __ballot_sync(0xffffffffu, mine && want > old + 1); more != 0; more &= more - 1) {
+      const int i = (threadIdx.x & ~31) + __ffs(more) - 1;
+      for (int64_t j = s_old[i] + 1 + (threadIdx.x & 31); j < s_want[i]; j += 32) entry(base + i, j, s_first[i] + j - s_old[i]);
     }
     // Tokens of these requests that fall into this CTA's stretch.
     const int64_t from = max(t0, token_base), to = min(t1, s_end[n - 1]);
