@@ -22,15 +22,16 @@
 // reported.
 //
 // Up to SCAN_TOKENS tokens a CTA per token looks for its run and through the earlier slots by
-// itself, in one launch.  Beyond that those looks would be quadratic: a launch before lists
-// the runs in the workspace, each leaves its token in its block's claim, and only where a claim
-// shows a second run of the block are the earlier slots read.  The claims need no clearing:
-// whatever they held is checked against the slots.
+// itself, in one launch.  Beyond that those looks would be quadratic: in a launch before, each
+// run leaves its token in its block's claim (workspace), and only where a claim shows a second
+// run of the block are the earlier slots read.  The claims need no clearing: whatever they
+// held is checked against the slots.  The storing launch starts beside it and waits for it only
+// when its first rows are there (13k tokens of 4 heads of 64: 10.5 -> 9.7 us; runs listed by the
+// first launch cost the second a wait at its start).
 //
 // What bounds it.  A decode step: launch and latency (a token each of 128 requests, 8 heads of
 // 128: 4.7 us on the device).  A prefill: the bytes, 2 in and 1 out per element (43k
-// tokens of 8 heads of 128 in bf16: 265 MB in 51 us, 5.2 TB/s, after 4.7 us for the list; 13k
-// tokens of 4 heads of 64: 10.5 us with the list).
+// tokens of 8 heads of 128 in bf16: 265 MB in 56 us, 4.7 TB/s), with 5 us of start and end.
 #include <cuda_runtime.h>
 
 #include "rk_cache8.cuh"
@@ -49,8 +50,7 @@ constexpr int APPEND_CTAS = 3;      // resident on an SM
 // The tokens of one block: `len` from `token` on, ascending from `offset` to `last` in `block`.
 struct Run {
   int32_t token, block;
-  int16_t offset, len, last;
-  int16_t rival;  // whether another run of the block is known
+  int16_t offset, len, last, unused;
 };
 
 struct AppendParams {
@@ -60,9 +60,8 @@ struct AppendParams {
   float* scales[2];
   const void* slots;
   int32_t* claims;  // per block: a token that starts a run of it; or anything
-  int32_t* counts;  // per THREADS tokens: the runs that start there,
-  Run* runs;        // listed from the first of those tokens' places on
-  int parts;        // CTAs that share a list
+  uint8_t* rivals;  // per token that starts a run: whether another run of its block is known
+  int parts;        // CTAs that share THREADS tokens
   int64_t capacity;  // num_blocks * block_size
   int32_t tokens;
   int heads, block_size, index_bits;
@@ -105,35 +104,56 @@ __device__ __forceinline__ bool starts_run(const AppendParams& p, int32_t other,
   return slot >= first && slot < first + p.block_size && !(other > 0 && goes_on(p, slot_of(p, other - 1), slot, block));
 }
 
-// Lists the runs and looks for blocks that have several.  A thread per token.  Each run leaves its
+__device__ __forceinline__ void wait_for_earlier_kernels() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// Looks for blocks that have several runs.  A thread per token.  Each run leaves its
 // token in its block's claim and sees what was there: anything, since nothing clears the
 // claims, or the token of a run that came before it, which the slots tell apart.  Of several
 // runs of a block all but the first to come see another, and the first finds another's token
 // in the claim afterwards.
-__global__ void __launch_bounds__(THREADS) append_runs_kernel(AppendParams p, KernelCtl ctl) {
-  __shared__ uint32_t s_breaks[WARPS];  // tokens that do not go on with the one before
-  __shared__ int s_starts[WARPS];
-  pdl_begin();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+__global__ void __launch_bounds__(THREADS) append_claims_kernel(AppendParams p, KernelCtl ctl) {
+  // The next kernel reads the call's inputs before it waits for this one: it may start once they
+  // are there.
+  wait_for_earlier_kernels();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int64_t t = static_cast<int64_t>(blockIdx.x) * THREADS + threadIdx.x;
+  if (t >= p.tokens) return;
+  const int64_t slot = slot_of(p, t), before = t > 0 ? slot_of(p, t - 1) : -1;
+  if (slot >= p.capacity) atomicOr(ctl.status, RK_DEV_ERR_BAD_INDEX);
+  if (slot < 0 || slot >= p.capacity) return;
+  const int block = block_of(p, slot);
+  if (goes_on(p, before, slot, block)) return;
+  const int32_t claimed = atomicExch(p.claims + block, static_cast<int32_t>(t));
+  p.rivals[t] = claimed != static_cast<int32_t>(t) && starts_run(p, claimed, block);
+}
+
+// The runs that start in THREADS tokens from t0 on, in their order; returns how many.
+__device__ __forceinline__ int list_runs(const AppendParams& p, int64_t t0, Run* runs) {
+  __shared__ int64_t s_slots[THREADS];
+  __shared__ uint32_t s_breaks[WARPS];  // tokens that do not go on with the one before
+  __shared__ uint32_t s_starts[WARPS];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t t = t0 + threadIdx.x;
   int64_t slot = -1;
   int block = -1;
   bool on = false;
   if (t < p.tokens) {
     slot = slot_of(p, t);
-    if (slot >= p.capacity) {
-      atomicOr(ctl.status, RK_DEV_ERR_BAD_INDEX);
-      slot = -1;
-    }
+    const int64_t before = t > 0 ? slot_of(p, t - 1) : -1;
+    if (slot >= p.capacity) slot = -1;
     if (slot >= 0) {
       block = block_of(p, slot);
-      on = t > 0 && goes_on(p, slot_of(p, t - 1), slot, block);
+      on = goes_on(p, before, slot, block);
     }
   }
-  const uint32_t breaks = ~__ballot_sync(0xffffffffu, on);
-  if (lane == 0) s_breaks[warp] = breaks;
-  __syncthreads();
   const bool starts = slot >= 0 && !on;
+  const uint32_t breaks = ~__ballot_sync(0xffffffffu, on), who = __ballot_sync(0xffffffffu, starts);
+  s_slots[threadIdx.x] = slot;
+  if (lane == 0) {
+    s_breaks[warp] = breaks;
+    s_starts[warp] = who;
+  }
+  __syncthreads();
   int len = 0;
   bool open = false;  // no break behind it in this CTA
   if (starts) {
@@ -145,32 +165,24 @@ __global__ void __launch_bounds__(THREADS) append_runs_kernel(AppendParams p, Ke
   }
   // At most one run of a CTA is open: its warp follows it.
   const uint32_t opens = __ballot_sync(0xffffffffu, open);
-  if (opens != 0) {
-    const int who = __ffs(opens) - 1;
-    const int more = more_tokens(p, static_cast<int64_t>(blockIdx.x) * THREADS + THREADS - 1,
-                                 __shfl_sync(0xffffffffu, block, who), lane);
-    if (lane == who) len += more;
-  }
-  const uint32_t who = __ballot_sync(0xffffffffu, starts);
-  if (lane == 0) s_starts[warp] = __popc(who);
-  __syncthreads();
+  int more = 0;
+  if (opens != 0) more = more_tokens(p, t0 + THREADS - 1, __shfl_sync(0xffffffffu, block, __ffs(opens) - 1), lane);
   int before = 0, all = 0;
 #pragma unroll
   for (int w = 0; w < WARPS; ++w) {
-    before += w < warp ? s_starts[w] : 0;
-    all += s_starts[w];
+    const int n = __popc(s_starts[w]);
+    before += w < warp ? n : 0;
+    all += n;
   }
-  if (threadIdx.x == 0) p.counts[blockIdx.x] = all;
   if (starts) {
-    const int32_t claimed = atomicExch(p.claims + block, static_cast<int32_t>(t));
     const int64_t first = static_cast<int64_t>(block) * p.block_size;
-    Run run{static_cast<int32_t>(t), block, 0, 0, 0, 0};
-    run.offset = static_cast<int16_t>(slot - first);
-    run.len = static_cast<int16_t>(len);
-    run.last = static_cast<int16_t>((len == 1 ? slot : slot_of(p, t + len - 1)) - first);
-    run.rival = claimed != static_cast<int32_t>(t) && starts_run(p, claimed, block);
-    p.runs[static_cast<int64_t>(blockIdx.x) * THREADS + before + __popc(who & ((1u << lane) - 1))] = run;
+    const int64_t last = open && more > 0 ? slot_of(p, t0 + THREADS - 1 + more) : s_slots[threadIdx.x + len - 1];
+    runs[before + __popc(who & ((1u << lane) - 1))] =
+        Run{static_cast<int32_t>(t), block, static_cast<int16_t>(slot - first),
+            static_cast<int16_t>(open ? len + more : len), static_cast<int16_t>(last - first), 0};
   }
+  __syncthreads();
+  return all;
 }
 
 template <typename T>
@@ -203,9 +215,10 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t w, float was, float inv) {
   return C::pack4((a.x * was) * inv, (a.y * was) * inv, (b.x * was) * inv, (b.y * was) * inv);
 }
 
-// One run of one head of K or V (`pair` < heads: K), by a warp.
-template <typename T, typename C, int D>
-__device__ __forceinline__ void append_run(const AppendParams& p, const Run& run, int pair, int lane) {
+// One run of one head of K or V (`pair` < heads: K), by a warp.  `is_first` says whether the run
+// is the first of its block; it is asked when the rows are there, before anything is stored.
+template <typename T, typename C, int D, typename First>
+__device__ __forceinline__ void append_run(const AppendParams& p, const Run& run, int pair, int lane, const First& is_first) {
   constexpr int LANES = D / 8;      // lanes of a row, 8 elements each
   constexpr int ROWS = 32 / LANES;  // rows side by side
   const int row = lane / LANES, at = (lane - row * LANES) * 8;
@@ -247,6 +260,7 @@ __device__ __forceinline__ void append_run(const AppendParams& p, const Run& run
   const float now = fmaxf(was, C::scale_for(amax));
   const float inv = 1.0f / now;
 
+  if (!is_first()) return;
   const bool dense = run.last - run.offset == run.len - 1;  // no holes
   if (run.offset > 0 && now != was) {
     // Rows that stay: those below the last new one that the run does not write.
@@ -316,24 +330,41 @@ __global__ void __launch_bounds__(THREADS) paged_append8_kernel(AppendParams p, 
   const int len = 1 + more_tokens(p, t, block, lane);
   const Run run{static_cast<int32_t>(t), block, static_cast<int16_t>(slot - slot0), static_cast<int16_t>(len),
                 static_cast<int16_t>((len == 1 ? slot : slot_of(p, t + len - 1)) - slot0), 0};
-  append_run<T, C, D>(p, run, pair, lane);
+  append_run<T, C, D>(p, run, pair, lane, [] { return true; });
 }
 
-// Many tokens: `parts` CTAs for each list, whose warps take the runs' heads of K and V in turn.
+// Many tokens: `parts` CTAs for each THREADS of them, whose warps take the runs' heads of K and V in
+// turn.  Each CTA lists the runs for itself and loads its warps' first rows while the claims
+// are still being made.
 template <typename T, typename C, int D>
 __global__ void __launch_bounds__(THREADS, APPEND_CTAS) paged_append8_runs_kernel(AppendParams p, KernelCtl ctl) {
-  pdl_begin();
+  __shared__ __align__(16) Run s_runs[THREADS];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int lane = threadIdx.x & 31;
   const int list = static_cast<int>(blockIdx.x) / p.parts, part = static_cast<int>(blockIdx.x) - list * p.parts;
   const int pairs = 2 * p.heads;
-  const int items = __ldg(p.counts + list) * pairs;
+  const int items = list_runs(p, static_cast<int64_t>(list) * THREADS, s_runs) * pairs;
+  bool waited = false;
 #pragma unroll 1
   for (int item = part * WARPS + (threadIdx.x >> 5); item < items; item += p.parts * WARPS) {
     const int at = item / pairs, pair = item - at * pairs;
-    const int4 raw = __ldg(reinterpret_cast<const int4*>(p.runs) + static_cast<int64_t>(list) * THREADS + at);
+    const int4 raw = *reinterpret_cast<const int4*>(s_runs + at);
     const Run run{raw.x, raw.y, static_cast<int16_t>(raw.z & 0xFFFF), static_cast<int16_t>(raw.z >> 16),
-                  static_cast<int16_t>(raw.w & 0xFFFF), static_cast<int16_t>(raw.w >> 16)};
-    if (run.rival != 0 || __ldg(p.claims + run.block) != run.token) {
+                  static_cast<int16_t>(raw.w & 0xFFFF), 0};
+    int32_t claim = 0;
+    uint32_t rival = 0;
+    const auto look = [&] {
+      claim = __ldcg(p.claims + run.block);
+      rival = __ldcg(p.rivals + run.token);
+    };
+    if (waited) look();
+    append_run<T, C, D>(p, run, pair, lane, [&] {
+      if (!waited) {
+        wait_for_earlier_kernels();
+        waited = true;
+        look();
+      }
+      if (rival == 0 && claim == run.token) return true;
       // The block has several runs: the first is stored, the others are not.
       const int64_t slot0 = static_cast<int64_t>(run.block) * p.block_size;
       bool seen = false;
@@ -341,20 +372,18 @@ __global__ void __launch_bounds__(THREADS, APPEND_CTAS) paged_append8_runs_kerne
         const int64_t slot = t0 + lane < run.token ? slot_of(p, t0 + lane) : -1;
         seen = __any_sync(0xffffffffu, slot >= slot0 && slot < slot0 + p.block_size) != 0;
       }
-      if (seen) {
-        if (lane == 0 && pair == 0) atomicOr(ctl.status, RK_DEV_ERR_BAD_INDEX);
-        continue;
-      }
-    }
-    append_run<T, C, D>(p, run, pair, lane);
+      if (seen && lane == 0 && pair == 0) atomicOr(ctl.status, RK_DEV_ERR_BAD_INDEX);
+      return !seen;
+    });
   }
+  if (!waited) wait_for_earlier_kernels();
 }
 
 int64_t lists_of(int64_t tokens) { return (tokens + THREADS - 1) / THREADS; }
 
 template <typename T, typename C, int D>
 cudaError_t launch(const AppendParams& p, const KernelCtl& ctl, cudaStream_t s) {
-  if (p.runs == nullptr) {
+  if (p.claims == nullptr) {
     const dim3 grid(static_cast<unsigned>(p.tokens), static_cast<unsigned>((2 * p.heads + WARPS - 1) / WARPS));
     note_launch("paged_append8_kernel");
     return launch_kernel(paged_append8_kernel<T, C, D>, grid, dim3(THREADS), 0, s, 0, p, ctl);
@@ -378,8 +407,7 @@ cudaError_t launch_d(const AppendParams& p, int64_t head_dim, const KernelCtl& c
 
 size_t paged_append8_workspace_bytes(int64_t tokens, int64_t num_blocks) {
   if (tokens <= SCAN_TOKENS) return 0;
-  const int64_t lists = lists_of(tokens);
-  return static_cast<size_t>(lists) * THREADS * sizeof(Run) + static_cast<size_t>(num_blocks + lists) * sizeof(int32_t);
+  return static_cast<size_t>(num_blocks) * sizeof(int32_t) + static_cast<size_t>(tokens);
 }
 
 rk_status paged_append8_launch(const PagedAppend8Args& a, void* workspace, size_t workspace_bytes, cudaStream_t s) {
@@ -409,16 +437,16 @@ rk_status paged_append8_launch(const PagedAppend8Args& a, void* workspace, size_
   p.block_size = static_cast<int>(a.block_size);
   if (need > 0) {
     const int64_t lists = lists_of(a.tokens);
-    p.runs = static_cast<Run*>(workspace);
-    p.claims = reinterpret_cast<int32_t*>(p.runs + lists * THREADS);
-    p.counts = p.claims + a.num_blocks;
-    // Enough CTAs to fill the GPU a few times, each with a run for every warp if blocks fill up.
+    p.claims = static_cast<int32_t*>(workspace);
+    p.rivals = reinterpret_cast<uint8_t*>(p.claims + a.num_blocks);
+    // CTAs that fill the GPU four times (43k tokens: 56 us; once 64, twice 57, eight times 62: each
+    // CTA lists its runs), each with a run for every warp if blocks fill up.
     const int64_t fill = static_cast<int64_t>(device_sm_count()) * APPEND_CTAS * 4;
     const int64_t most = (THREADS / p.block_size + 1) * 2 * static_cast<int64_t>(p.heads) / WARPS + 1;
     const int64_t parts = (fill + lists - 1) / lists;
     p.parts = static_cast<int>(parts < most ? parts : most);
-    const cudaError_t e = launch_kernel(append_runs_kernel, dim3(static_cast<unsigned>(lists)), dim3(THREADS), 0, s, 0, p, ctl);
-    note_launch("append_runs_kernel");
+    const cudaError_t e = launch_kernel(append_claims_kernel, dim3(static_cast<unsigned>(lists)), dim3(THREADS), 0, s, 0, p, ctl);
+    note_launch("append_claims_kernel");
     if (e != cudaSuccess) return cuda_status(e);
   }
   const bool bf16 = a.dt == RK_DTYPE_BF16, e4m3 = a.cache == RK_CACHE_E4M3;
