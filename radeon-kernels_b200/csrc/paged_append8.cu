@@ -26,13 +26,16 @@
 // run leaves its token in its block's claim (workspace), and only where a claim shows a second
 // run of the block are the earlier slots read.  The claims need no clearing: whatever they
 // held is checked against the slots.  The storing launch starts beside it and waits for it only
-// when its first rows are there (13k tokens of 4 heads of 64: 10.5 -> 9.7 us; runs listed by the
-// first launch cost the second a wait at its start).
+// when its first rows are there (13k tokens of 4 heads of 64: 9.7 us, and 10.5 with the runs listed
+// by the first launch).
 //
 // What bounds it.  A decode step: launch and latency (a token each of 128 requests, 8 heads of
-// 128: 4.7 us on the device).  A prefill: the bytes, 2 in and 1 out per element (43k
-// tokens of 8 heads of 128 in bf16: 265 MB in 56 us, 4.7 TB/s), with 5 us of start and end.
+// 128: 3.6 us on the device).  A prefill: the bytes, 2 in and 1 out per element (43k
+// tokens of 8 heads of 128 in bf16: 265 MB in 51 us, 5.2 TB/s), with 5 us of start and end; the
+// instructions are near (60 % of the issue slots with magnitudes taken in fp32, and 56 us).
 #include <cuda_runtime.h>
+
+#include <type_traits>
 
 #include "rk_cache8.cuh"
 #include "rk_device.cuh"
@@ -185,6 +188,7 @@ __device__ __forceinline__ int list_runs(const AppendParams& p, int64_t t0, Run*
   return all;
 }
 
+// The largest magnitude of 8 elements; infinities and NaN set no scale.
 template <typename T>
 __device__ __forceinline__ float amax8(const uint4& v) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -193,8 +197,23 @@ __device__ __forceinline__ float amax8(const uint4& v) {
   for (int j = 0; j < 4; ++j) {
     const float2 f = Pack2<T>::to_floats(w[j]);
     const float a = fabsf(f.x), b = fabsf(f.y);
-    m = fmaxf(m, a < INFINITY ? a : 0.f);  // infinities and NaN set no scale
+    m = fmaxf(m, a < INFINITY ? a : 0.f);
     m = fmaxf(m, b < INFINITY ? b : 0.f);
+  }
+  return m;
+}
+
+// The same, pair by pair in 16 bits, but for infinities, which it returns.
+template <typename T>
+__device__ __forceinline__ uint32_t max2(uint32_t m, const uint4& v) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t magnitude = w[j] & 0x7FFF7FFFu;
+    if constexpr (std::is_same<T, __half>::value)
+      asm("max.f16x2 %0, %0, %1;" : "+r"(m) : "r"(magnitude));  // NaN against a number: the number
+    else
+      asm("max.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(magnitude));
   }
   return m;
 }
@@ -245,9 +264,16 @@ __device__ __forceinline__ void append_run(const AppendParams& p, const Run& run
   const float was_raw = run.offset == 0 ? 0.f : *scale;
   const float was = was_raw > 0.f && was_raw < INFINITY ? was_raw : 0.f;
 
-  float amax = 0.f;
+  uint32_t most = 0;
 #pragma unroll
-  for (int k = 0; k < HELD; ++k) amax = fmaxf(amax, amax8<T>(held[k]));
+  for (int k = 0; k < HELD; ++k) most = max2<T>(most, held[k]);
+  const float2 of_most = Pack2<T>::to_floats(most);
+  float amax = fmaxf(of_most.x, of_most.y);
+  if (amax == INFINITY) {
+    amax = 0.f;
+#pragma unroll
+    for (int k = 0; k < HELD; ++k) amax = fmaxf(amax, amax8<T>(held[k]));
+  }
   // Unpacked again for the store: kept from here, their fp32 values would take twice the
   // registers of the rows themselves.
 #pragma unroll
@@ -439,8 +465,8 @@ rk_status paged_append8_launch(const PagedAppend8Args& a, void* workspace, size_
     const int64_t lists = lists_of(a.tokens);
     p.claims = static_cast<int32_t*>(workspace);
     p.rivals = reinterpret_cast<uint8_t*>(p.claims + a.num_blocks);
-    // CTAs that fill the GPU four times (43k tokens: 56 us; once 64, twice 57, eight times 62: each
-    // CTA lists its runs), each with a run for every warp if blocks fill up.
+    // CTAs that fill the GPU four times (43k tokens: the same from three to six; each lists its runs,
+    // so not more), each with a run for every warp if blocks fill up.
     const int64_t fill = static_cast<int64_t>(device_sm_count()) * APPEND_CTAS * 4;
     const int64_t most = (THREADS / p.block_size + 1) * 2 * static_cast<int64_t>(p.heads) / WARPS + 1;
     const int64_t parts = (fill + lists - 1) / lists;

@@ -14,7 +14,7 @@
 // they are used.
 //
 // What bounds it: the bytes of the queries and keys, read and written once (8192 tokens of 32 + 8
-// heads of 128 in bf16: 168 MB in 32.8 us, 5.1 TB/s; 16 tokens: 2.5 us, the launch).
+// heads of 128 in bf16: 168 MB in 29.1 us, 5.8 TB/s; 16 tokens: 2.4 us, the launch).
 #include <cuda_runtime.h>
 
 #include "rk_device.cuh"
@@ -42,32 +42,41 @@ struct RotaryParams {
   int inverse;
 };
 
-// Two vectors of 8 elements that a lane turns: the first and second elements of 8 pairs.
+// Where a pair's cosine and sine lie in its token's row of the table.  Lanes read 16 bytes each,
+// 64 apart (8 pairs, one unit): in order, four of every eight would meet in the same banks (8192
+// tokens of 32 + 8 heads of 128: 32.8 us instead of 29.2), so the unit's number exchanges its four.
+__device__ __forceinline__ int table_at(int pair) { return pair ^ ((pair >> 3) & 6); }
+
+// Two vectors of 8 elements that a lane turns: the first and second elements of 8 pairs, which are
+// those of `unit` in the table's row.
 template <typename T>
-__device__ __forceinline__ void turn_halves(uint4& a, uint4& b, const float2* cs) {
+__device__ __forceinline__ void turn_halves(uint4& a, uint4& b, const float2* row, int unit) {
   uint32_t* pa = reinterpret_cast<uint32_t*>(&a);
   uint32_t* pb = reinterpret_cast<uint32_t*>(&b);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const float2 x = Pack2<T>::to_floats(pa[j]), y = Pack2<T>::to_floats(pb[j]);
-    const float4 t = *reinterpret_cast<const float4*>(cs + 2 * j);  // cos, sin, cos, sin
+    const float4 t = *reinterpret_cast<const float4*>(row + unit * 8 + ((2 * j) ^ (unit & 6)));  // cos, sin, cos, sin
     pa[j] = Pack2<T>::from_floats(x.x * t.x - y.x * t.y, x.y * t.z - y.y * t.w);
     pb[j] = Pack2<T>::from_floats(y.x * t.x + x.x * t.y, y.y * t.z + x.y * t.w);
   }
 }
 
-// A vector of 4 neighbouring pairs.
+// A vector of 4 neighbouring pairs: the first (from = 0) or second (4) four of `unit`.
 template <typename T>
-__device__ __forceinline__ void turn_pairs(uint4& a, const float2* cs) {
+__device__ __forceinline__ void turn_pairs(uint4& a, const float2* row, int unit, int from) {
   uint32_t* pa = reinterpret_cast<uint32_t*>(&a);
 #pragma unroll
   for (int j = 0; j < 4; j += 2) {
-    const float4 t = *reinterpret_cast<const float4*>(cs + j);
+    const float4 t = *reinterpret_cast<const float4*>(row + unit * 8 + ((from + j) ^ (unit & 6)));
     const float2 x = Pack2<T>::to_floats(pa[j]), y = Pack2<T>::to_floats(pa[j + 1]);
     pa[j] = Pack2<T>::from_floats(x.x * t.x - x.y * t.y, x.y * t.x + x.x * t.y);
     pa[j + 1] = Pack2<T>::from_floats(y.x * t.z - y.y * t.w, y.y * t.z + y.x * t.w);
   }
 }
+
+// Pairs of a row of the table: whole units.
+__host__ __device__ constexpr int table_stride(int half) { return (half + 7) & ~7; }
 
 // A CTA takes some tokens.  Each thread keeps one unit of a head (no division in the loop) and
 // walks over the heads of the tokens, ROWS of them in flight; the first are on their way while
@@ -76,7 +85,8 @@ __device__ __forceinline__ void turn_pairs(uint4& a, const float2* cs) {
 template <typename T, bool INTERLEAVED, bool VEC>
 __global__ void __launch_bounds__(THREADS, VEC ? 6 : 1) rotary_kernel(RotaryParams p, int tokens_per_cta) {
   constexpr int ROWS = VEC ? ROWS_AHEAD : 1;
-  extern __shared__ float2 table[];  // [tokens_per_cta][half]
+  extern __shared__ __align__(16) float2 table[];  // [tokens_per_cta][stride]
+  const int stride = table_stride(p.half);
   pdl_begin();
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * tokens_per_cta;
   const int nt = static_cast<int>(min(static_cast<int64_t>(tokens_per_cta), p.tokens - t0));
@@ -134,14 +144,14 @@ __global__ void __launch_bounds__(THREADS, VEC ? 6 : 1) rotary_kernel(RotaryPara
     const bool key = h >= p.query_heads;
     const int head = key ? h - p.query_heads : h, nheads = key ? p.heads - p.query_heads : p.query_heads;
     T* out = static_cast<T*>(key ? p.out[1] : p.out[0]) + ((t0 + t) * nheads + head) * p.head_dim;
-    const float2* cs = table + t * p.half;
+    const float2* cs = table + t * stride;
     if (VEC) {
       if (INTERLEAVED) {
         // The border between turned and copied elements lies on a vector's.
-        if (first < 2 * p.half) turn_pairs<T>(a[k], cs + first / 2);
-        if (second < 2 * p.half) turn_pairs<T>(b[k], cs + second / 2);
+        if (first < 2 * p.half) turn_pairs<T>(a[k], cs, unit, 0);
+        if (second < 2 * p.half) turn_pairs<T>(b[k], cs, unit, 4);
       } else if (turns) {
-        turn_halves<T>(a[k], b[k], cs + first);
+        turn_halves<T>(a[k], b[k], cs, unit);
       }
       *reinterpret_cast<uint4*>(out + first) = a[k];
       if (both) *reinterpret_cast<uint4*>(out + second) = b[k];
@@ -149,7 +159,7 @@ __global__ void __launch_bounds__(THREADS, VEC ? 6 : 1) rotary_kernel(RotaryPara
       const T* in = source(t, h);
       if (turns) {
         const float x = to_f32(in[first]), y = to_f32(in[second]);
-        const float2 c = cs[unit];
+        const float2 c = cs[table_at(unit)];
         out[first] = from_f32<T>(x * c.x - y * c.y);
         out[second] = from_f32<T>(y * c.x + x * c.y);
       } else {
@@ -171,7 +181,7 @@ __global__ void __launch_bounds__(THREADS, VEC ? 6 : 1) rotary_kernel(RotaryPara
     const double turned = position * (p.frequencies[f] * 0.15915494309189533577);  // 1 / (2 pi)
     float s, c;
     sincospif(2.0f * static_cast<float>(turned - rint(turned)), &s, &c);
-    table[i] = make_float2(c * p.amplitude, (p.inverse ? -s : s) * p.amplitude);
+    table[at * stride + table_at(f)] = make_float2(c * p.amplitude, (p.inverse ? -s : s) * p.amplitude);
   }
   __syncthreads();
 
@@ -198,7 +208,7 @@ __global__ void __launch_bounds__(THREADS, VEC ? 6 : 1) rotary_kernel(RotaryPara
 template <typename T>
 cudaError_t launch(const RotaryParams& p, bool interleaved, bool vec, int per_cta, cudaStream_t s) {
   const dim3 grid(static_cast<unsigned>((p.tokens + per_cta - 1) / per_cta));
-  const size_t smem = static_cast<size_t>(per_cta) * p.half * sizeof(float2);
+  const size_t smem = static_cast<size_t>(per_cta) * table_stride(p.half) * sizeof(float2);
   if (interleaved)
     return vec ? launch_kernel(rotary_kernel<T, true, true>, grid, dim3(THREADS), smem, s, 0, p, per_cta)
                : launch_kernel(rotary_kernel<T, true, false>, grid, dim3(THREADS), smem, s, 0, p, per_cta);
@@ -240,16 +250,10 @@ rk_status rotary_launch(const RotaryArgs& a, cudaStream_t s) {
     p.turn_units = p.half;
     p.units = p.half + p.head_dim - 2 * p.half;
   }
-  // Few tokens: one CTA each, so that they spread over the SMs.  Many: two to a CTA, or three where
-  // two leave over a third of its last round of rows empty (8192 tokens of 32 + 8 heads of
-  // 128: 32.8 us with three, 34.0 with two, 37.7 with one, 38.3 with eight; 4099 tokens of 32
-  // heads, which fill the round: 15.0, 14.4, 16.7, 20.2).
-  int per_cta = 1;
-  if (p.tokens >= 16 * static_cast<int64_t>(device_sm_count())) {
-    const int round = ROWS_AHEAD * (THREADS / (p.units < THREADS ? p.units : THREADS));
-    const auto filled = [&](int t) { return static_cast<float>(t * p.heads) / ((t * p.heads + round - 1) / round * round); };
-    per_cta = filled(3) > filled(2) + 0.2f ? 3 : 2;
-  }
+  // Few tokens: one CTA each, so that they spread over the SMs.  Many: two to a CTA (8192 tokens of
+  // 32 + 8 heads of 128: 29.1 us with two, 33.9 with one, 30.0 with four; 1000 tokens: 7.4, 5.9,
+  // 10.5).
+  const int per_cta = p.tokens >= 16 * static_cast<int64_t>(device_sm_count()) ? 2 : 1;
   const cudaError_t e = a.dt == RK_DTYPE_BF16 ? launch<__nv_bfloat16>(p, a.interleaved, vec, per_cta, s)
                                               : launch<__half>(p, a.interleaved, vec, per_cta, s);
   note_launch("rotary_kernel");
