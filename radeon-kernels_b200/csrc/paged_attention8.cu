@@ -17,7 +17,9 @@
 // A range that a warp holds whole goes to the output from its registers.  Of one that is cut,
 // each warp leaves the unnormalised sums and their statistics: the warps of a CTA join theirs
 // in shared memory, CTAs meet in the workspace, where every CTA counts its parts in and the
-// last to come joins them all, in their order, so that results do not depend on timing.
+// last to come joins them all -- of ranges over many CTAs, those of a group of neighbours, and
+// the last group to be joined all groups --, in their order, so that results do not depend on
+// timing.
 // Nothing waits for another CTA.  (A second launch for the join measured 3 to 6 us more on
 // 16 x 2048 positions, and a device-wide fence at each CTA's end 2 us: hence one count
 // and one fence.)
@@ -65,6 +67,10 @@ constexpr int WARPS = 4;
 constexpr int THREADS = WARPS * 32;
 constexpr int STAGES = 3;
 constexpr int RANGE_COST = 2;        // what starting and ending a range costs, in units
+// Ranges over more CTAs than JOIN_ONCE are joined in two steps, JOIN_CTAS at a time first (one
+// sequence of 20000 positions, one KV head of 128 with 4 query heads, 40 CTAs: 32 us at once, 15 in
+// two steps; 17 CTAs of head_dim 256 with 8 query heads: 18.6 and 21.4).
+constexpr int JOIN_ONCE = 24, JOIN_CTAS = 16;
 constexpr float SLACK = 256.0f;      // a running maximum is raised when a weight is this much above it
 constexpr float NONE = -3.402823466e38f;  // a maximum before any score: finite, so that -inf - NONE = -inf
 
@@ -108,7 +114,9 @@ struct Params {
   const void* lens;
   void* out;
   float* part;      // [warp][2][heads of a tile][part_stride]: part 0 continues a range, part 1 begins one
-  uint64_t* arrivals;  // [warp]: `tag` plus the parts written of the range that the warp begins; or anything
+  // [2][warp]: `tag` plus the parts that have been written -- of the range that the warp begins, then of
+  // groups of CTAs of ranges that are joined in two steps -- or anything.
+  uint64_t* arrivals;
   uint64_t tag;        // of this launch; its low 16 bits are 0, the others not all
   int batch, hq, hkv, group, head_groups;
   int num_blocks, block_size, max_blocks;
@@ -246,6 +254,20 @@ struct Parts {
   }
   __device__ __forceinline__ int warp(int i) const {
     return i == 0 ? begin : (i <= ctas ? (begin / WARPS + i) * WARPS : end);
+  }
+  // Part i in the workspace: 1 where the warp begins the range, 0 where it goes on with it.
+  __device__ __forceinline__ int slot(int i) const { return i == 0 ? 1 : 0; }
+  // Ranges over many CTAs are joined in two steps: JOIN_CTAS neighbours at a time, into the first
+  // one's part, then those.
+  __device__ __forceinline__ int groups() const { return ctas < JOIN_ONCE ? 1 : ctas / JOIN_CTAS + 1; }
+  __device__ __forceinline__ int group_of(int cta) const { return (cta - begin / WARPS) / JOIN_CTAS; }
+  __device__ __forceinline__ int parts_of(int group) const {
+    return group + 1 < groups() ? JOIN_CTAS : count - group * JOIN_CTAS;
+  }
+  // Where a group's parts are counted, a warp of its first CTA.  Only one range goes from a CTA to the
+  // next, so a CTA begins one group at most, and goes on with one.
+  __device__ __forceinline__ int counter(int group) const {
+    return (begin / WARPS + group * JOIN_CTAS) * WARPS + (group == 0 ? 1 : 0);
   }
 };
 
@@ -394,46 +416,57 @@ struct Sums {
   }
 };
 
-// One head of a range from its parts, written by other SMs: read past L1, some at a time.
+// The heads of a range from `count` of its parts, `step` apart from `from` on, by a CTA: into the
+// output, or into the first of the parts.  They were written by other SMs: read past L1, some
+// at a time, by half a warp for each head.
 template <int D, int HEADS>
-__device__ __forceinline__ void join_head(const Params& p, const Parts& parts, int64_t out_row, int h, int lane) {
+__device__ __forceinline__ void join(const Params& p, const Piece& piece, int from, int step, int count, bool out) {
   constexpr int AHEAD = 4;
-  Sums<D> sums{};
-  sums.start();
+  const Parts parts = piece.parts;
+  const int column = threadIdx.x & 15;
 #pragma unroll 1
-  for (int i0 = 0; i0 < parts.count; i0 += AHEAD) {
-    float x[AHEAD][Sums<D>::V];
-    float4 st[AHEAD];
+  for (int h = threadIdx.x >> 4; h < piece.heads; h += THREADS / 16) {
+    Sums<D> sums{};
+    sums.start();
+#pragma unroll 1
+    for (int i0 = 0; i0 < count; i0 += AHEAD) {
+      float x[AHEAD][Sums<D>::V];
+      float4 st[AHEAD];
 #pragma unroll
-    for (int j = 0; j < AHEAD; ++j) {
-      const int i = min(i0 + j, parts.count - 1);
-      const float* row = part_of<D, HEADS>(p, parts.warp(i), i == 0 ? 1 : 0) + h * part_stride(D);
-      st[j] = __ldcg(reinterpret_cast<const float4*>(row + D));
+      for (int j = 0; j < AHEAD; ++j) {
+        const int i = from + min(i0 + j, count - 1) * step;
+        const float* row = part_of<D, HEADS>(p, parts.warp(i), parts.slot(i)) + h * part_stride(D);
+        st[j] = __ldcg(reinterpret_cast<const float4*>(row + D));
 #pragma unroll
-      for (int k = 0; k < Sums<D>::V; k += 4) {
-        const float4 y = __ldcg(reinterpret_cast<const float4*>(row + Sums<D>::V * lane + k));
-        x[j][k] = y.x;
-        x[j][k + 1] = y.y;
-        x[j][k + 2] = y.z;
-        x[j][k + 3] = y.w;
+        for (int k = 0; k < Sums<D>::V; k += 4) {
+          const float4 y = __ldcg(reinterpret_cast<const float4*>(row + Sums<D>::V * column + k));
+          x[j][k] = y.x;
+          x[j][k + 1] = y.y;
+          x[j][k + 2] = y.z;
+          x[j][k + 3] = y.w;
+        }
+      }
+      float bm = sums.m, bo = sums.mo;
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        bm = fmaxf(bm, st[j].x);  // a part that is loaded twice changes no maximum
+        bo = fmaxf(bo, st[j].y);
+      }
+      sums.raise(bm, bo);
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        if (i0 + j < count) {
+          sums.l = fmaf(st[j].z, ex2_approx(st[j].x - bm), sums.l);
+          sums.add(x[j], ex2_approx(st[j].y - bo));
+        }
       }
     }
-    float bm = sums.m, bo = sums.mo;
-#pragma unroll
-    for (int j = 0; j < AHEAD; ++j) {
-      bm = fmaxf(bm, st[j].x);  // a part that is loaded twice changes no maximum
-      bo = fmaxf(bo, st[j].y);
-    }
-    sums.raise(bm, bo);
-#pragma unroll
-    for (int j = 0; j < AHEAD; ++j) {
-      if (i0 + j < parts.count) {
-        sums.l = fmaf(st[j].z, ex2_approx(st[j].x - bm), sums.l);
-        sums.add(x[j], ex2_approx(st[j].y - bo));
-      }
+    if (out) {
+      sums.write(p, static_cast<int64_t>(piece.row) + h, column);
+    } else {
+      sums.store(part_of<D, HEADS>(p, parts.warp(from), parts.slot(from)) + h * part_stride(D), column);
     }
   }
-  sums.write(p, out_row, lane);
 }
 
 template <typename C, int D, int NT>
@@ -955,6 +988,7 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attention8_kernel(Params p, 
   bool stands = false;
   uint64_t seen = 0;
   uint64_t* word = nullptr;
+  int all = 0;
   const Piece* piece = nullptr;
   if (warp == 0 && lane < 2 * WARPS) {
     const int w = lane >> 1, k = lane & 1;
@@ -964,7 +998,11 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attention8_kernel(Params p, 
     stands = piece == &s_ended[w] ||
              (first && piece->heads > 0 && piece->begins == k && !(piece->begins && s_last[end - 1].ends));
     if (stands) {
-      word = p.arrivals + piece->parts.begin;
+      const Parts& parts = piece->parts;
+      const bool grouped = parts.groups() > 1;
+      const int group = parts.group_of(blockIdx.x);
+      word = p.arrivals + (grouped ? gridDim.x * WARPS + parts.counter(group) : parts.begin);
+      all = grouped ? parts.parts_of(group) : parts.count;
       seen = *reinterpret_cast<volatile uint64_t*>(word);
     }
   }
@@ -1017,7 +1055,7 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attention8_kernel(Params p, 
     const uint32_t same = __match_any_sync(__activemask(), piece->place);  // this CTA's parts of one range
     if (lane == __ffs(same) - 1) {
       fence_gpu();  // the CTA's parts before their count
-      if (arrive(word, seen, p.tag, __popc(same), piece->parts.count)) {
+      if (arrive(word, seen, p.tag, __popc(same), all)) {
         fence_gpu();  // the count before the parts
         s_join[lane] = 1;
         last_here = true;
@@ -1029,10 +1067,27 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attention8_kernel(Params p, 
   for (int i = 0; i < 2 * WARPS; ++i) {
     if (s_join[i] == 0) continue;
     const Piece& whose = (i & 1) == 0 && s_ended[i >> 1].heads > 0 ? s_ended[i >> 1] : s_last[i >> 1];
-    const Parts parts = whose.parts;
-#pragma unroll 1
-    for (int h = threadIdx.x >> 4; h < whose.heads; h += THREADS / 16)
-      join_head<D, HEADS>(p, parts, static_cast<int64_t>(whose.row) + h, h, lane & 15);
+    const Parts& parts = whose.parts;
+    const int groups = parts.groups(), group = parts.group_of(blockIdx.x);
+    bool out = groups == 1;
+    int from = out ? 0 : group * JOIN_CTAS, step = 1, count = out ? parts.count : parts.parts_of(group);
+    for (;;) {
+      join<D, HEADS>(p, whose, from, step, count, out);
+      if (out) break;
+      __syncthreads();
+      bool last = false;
+      if (threadIdx.x == 0) {
+        fence_gpu();  // the joined part before its count
+        uint64_t* const counted = p.arrivals + parts.begin;
+        last = arrive(counted, *reinterpret_cast<volatile uint64_t*>(counted), p.tag, 1, groups);
+        if (last) fence_gpu();
+      }
+      if (!__syncthreads_or(last)) break;
+      out = true;
+      from = 0;
+      step = JOIN_CTAS;
+      count = groups;
+    }
   }
 }
 
@@ -1105,7 +1160,7 @@ rk_status launch_d(const Params& p, int64_t head_dim, int nt, const KernelCtl& c
 size_t paged_attention8_workspace_bytes(int64_t hq, int64_t hkv, int64_t head_dim) {
   const pa8::Plan pl = pa8::plan(hq, hkv, head_dim);
   const size_t warps = static_cast<size_t>(device_sm_count()) * pa8::ctas_per_sm(static_cast<int>(head_dim)) * pa8::WARPS;
-  return warps * (sizeof(uint64_t) + 2 * 8 * pl.nt * pa8::part_stride(static_cast<int>(head_dim)) * sizeof(float));
+  return warps * (2 * sizeof(uint64_t) + 2 * 8 * pl.nt * pa8::part_stride(static_cast<int>(head_dim)) * sizeof(float));
 }
 
 rk_status paged_attention8_launch(const PagedAttention8Args& a, void* workspace, size_t workspace_bytes, cudaStream_t s) {
@@ -1126,7 +1181,7 @@ rk_status paged_attention8_launch(const PagedAttention8Args& a, void* workspace,
   p.lens = a.context_lengths;
   p.out = a.out;
   p.arrivals = static_cast<uint64_t*>(workspace);
-  p.part = reinterpret_cast<float*>(p.arrivals + device_sm_count() * pa8::ctas_per_sm(static_cast<int>(a.head_dim)) * pa8::WARPS);
+  p.part = reinterpret_cast<float*>(p.arrivals + 2 * device_sm_count() * pa8::ctas_per_sm(static_cast<int>(a.head_dim)) * pa8::WARPS);
   p.tag = pa8::next_tag();
   p.batch = static_cast<int>(a.batch);
   p.hq = static_cast<int>(a.hq);

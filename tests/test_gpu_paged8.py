@@ -339,6 +339,27 @@ def test_attention_matches_its_definition(lengths, query_heads, kv_heads, dim, s
     assert torch.equal(out.view(torch.int16), p.run().view(torch.int16))  # the same bits every time
 
 
+@pytest.mark.parametrize(
+    "lengths,query_heads,kv_heads,dim,size",
+    [([20000], 4, 1, 128, 16), ([12000], 8, 1, 256, 64), ([9000, 3, 14000], 6, 2, 64, 24), ([40000, 40000], 1, 1, 64, 128),
+     ([30001], 17, 1, 64, 32), ([6000, 6000, 6000], 16, 1, 128, 8)])
+def test_sequences_that_fill_the_gpu(lengths, query_heads, kv_heads, dim, size):
+    """A head of a sequence is spread over all SMs; whichever comes last, the result is the same."""
+    import torch
+
+    p = Problem(lengths, query_heads, kv_heads, dim, size, "bf16", "int8", seed=sum(lengths))
+    out = p.run()
+    p.check(out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = [p.run() for _ in range(3)]
+    for _ in range(5):
+        for c in captured:
+            c.zero_()
+        graph.replay()
+        assert all(torch.equal(c, out) for c in captured)
+
+
 @pytest.mark.parametrize("scale", [1e-4, 0.5, 3])
 def test_attention_scale(scale):
     p = Problem([100, 700], 8, 2, 128, 16, seed=3)
