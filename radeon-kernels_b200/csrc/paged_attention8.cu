@@ -24,7 +24,7 @@
 // 16 x 2048 positions, and a device-wide fence at each CTA's end 2 us: hence one count
 // and one fence.)
 //
-// A warp feeds itself: a ring of STAGES units of K and V with their scales in shared memory,
+// A warp feeds itself: a ring of two units of K and V with their scales in shared memory,
 // filled by cp.async and running on across the ends of ranges; block-table entries 32 at a time
 // and queries are loaded a range ahead.  No barrier until the warp's stretch is done.
 //
@@ -46,9 +46,9 @@
 // only when a weight passes them by SLACK; in between p and w may reach that, far inside the
 // range of both types, and the sums need no rescaling.
 //
-// What bounds it: the bytes of K and V, 1.07 GB in 205 us at 4 x 131072 positions of 8 heads of
-// 128 (5.2 TB/s; the same kernel without the products streams them in 187 us, and some SMs
-// finish their equal share 20 % before others).  At 16 x 2048 positions (67 MB, 21.5 us) the
+// What bounds it: the bytes of K and V, 1.07 GB in 203 to 211 us at 4 x 131072 positions of 8 heads of
+// 128 (5.1 TB/s; without the products it streamed them in 187 us, and some SMs finish
+// their equal share 20 % before others).  At 16 x 2048 positions (67 MB, 21.5 us) the
 // start and the end: 2.2 us until the first loads leave (lengths, then table, then rows: each
 // waits for the one before), 4 us from the last tile to the last join.
 #include <cuda_runtime.h>
@@ -65,7 +65,10 @@ namespace pa8 {
 
 constexpr int WARPS = 4;
 constexpr int THREADS = WARPS * 32;
-constexpr int STAGES = 3;
+// Units of a warp's ring.  Three kept more bytes under way and cost more (8 x 15317 positions of 3 heads
+// of 256: 51.9 us, and 46.5 with two; 61 sequences of 1 to 16 Ki, 4 heads of 128: 26.4, 25.3; 4 x 128
+// Ki the same).
+constexpr int STAGES = 2;
 constexpr int RANGE_COST = 2;        // what starting and ending a range costs, in units
 // Ranges over more CTAs than JOIN_ONCE are joined in two steps, JOIN_CTAS at a time first (one
 // sequence of 20000 positions, one KV head of 128 with 4 query heads, 40 CTAs: 32 us at once, 15 in
@@ -74,9 +77,9 @@ constexpr int JOIN_ONCE = 24, JOIN_CTAS = 16;
 constexpr float SLACK = 256.0f;      // a running maximum is raised when a weight is this much above it
 constexpr float NONE = -3.402823466e38f;  // a maximum before any score: finite, so that -inf - NONE = -inf
 
-// CTAs of an SM that are launched (and that the workspace has room for): 3 fit at head_dim 64, 2
-// otherwise.
-__host__ __device__ constexpr int ctas_per_sm(int head_dim) { return head_dim == 64 ? 3 : 2; }
+// CTAs of an SM, which the registers allow (held to 168 for three: 4 x 128 Ki positions 209 -> 215
+// us, 16 x 2048 21.5 -> 23.9).
+constexpr int CTAS_PER_SM = 2;
 
 // Positions of a unit, which is one tile of a warp.
 __host__ __device__ constexpr int unit_of(int head_dim) { return head_dim == 256 ? 16 : 32; }
@@ -470,7 +473,7 @@ __device__ __forceinline__ void join(const Params& p, const Piece& piece, int fr
 }
 
 template <typename C, int D, int NT>
-__global__ void __launch_bounds__(THREADS, 2) paged_attention8_kernel(Params p, KernelCtl ctl) {
+__global__ void __launch_bounds__(THREADS, CTAS_PER_SM) paged_attention8_kernel(Params p, KernelCtl ctl) {
   using L = Layout<D>;
   constexpr int TILE = L::TILE, SUB = TILE / 16;  // MMA tiles of 16 positions
   constexpr int KC = D / 64;   // 16-byte chunks of a K row per lane
@@ -631,7 +634,7 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attention8_kernel(Params p, 
         }
       }
     } else {
-#pragma unroll 1
+#pragma unroll 4
       for (int i = 0; i < TILE / PER; ++i) {
         const int r = i * PER + r0;
         const uint8_t* from = p.k + __shfl_sync(0xffffffffu, row_bytes, r) + head_bytes + ch * 16;
@@ -1137,7 +1140,7 @@ rk_status launch(const Params& p, const KernelCtl& ctl, cudaStream_t s) {
     note_error("the block tables hold too many positions for one call");
     return RK_ERR_UNSUPPORTED;
   }
-  int64_t ctas = static_cast<int64_t>(device_sm_count()) * (resident < ctas_per_sm(D) ? resident : ctas_per_sm(D));
+  int64_t ctas = static_cast<int64_t>(device_sm_count()) * (resident < CTAS_PER_SM ? resident : CTAS_PER_SM);
   // Not more warps than units; RANGE_COST places of a range hold none.
   if (ranges <= ctas * WARPS && ranges * (per_range + RANGE_COST) < ctas * WARPS)
     ctas = (ranges * (per_range + RANGE_COST) + WARPS - 1) / WARPS;
@@ -1159,7 +1162,7 @@ rk_status launch_d(const Params& p, int64_t head_dim, int nt, const KernelCtl& c
 
 size_t paged_attention8_workspace_bytes(int64_t hq, int64_t hkv, int64_t head_dim) {
   const pa8::Plan pl = pa8::plan(hq, hkv, head_dim);
-  const size_t warps = static_cast<size_t>(device_sm_count()) * pa8::ctas_per_sm(static_cast<int>(head_dim)) * pa8::WARPS;
+  const size_t warps = static_cast<size_t>(device_sm_count()) * pa8::CTAS_PER_SM * pa8::WARPS;
   return warps * (2 * sizeof(uint64_t) + 2 * 8 * pl.nt * pa8::part_stride(static_cast<int>(head_dim)) * sizeof(float));
 }
 
@@ -1181,7 +1184,7 @@ rk_status paged_attention8_launch(const PagedAttention8Args& a, void* workspace,
   p.lens = a.context_lengths;
   p.out = a.out;
   p.arrivals = static_cast<uint64_t*>(workspace);
-  p.part = reinterpret_cast<float*>(p.arrivals + 2 * device_sm_count() * pa8::ctas_per_sm(static_cast<int>(a.head_dim)) * pa8::WARPS);
+  p.part = reinterpret_cast<float*>(p.arrivals + 2 * device_sm_count() * pa8::CTAS_PER_SM * pa8::WARPS);
   p.tag = pa8::next_tag();
   p.batch = static_cast<int>(a.batch);
   p.hq = static_cast<int>(a.hq);
