@@ -14,7 +14,9 @@
 // they are used.
 //
 // What bounds it: the bytes of the queries and keys, read and written once (8192 tokens of 32 + 8
-// heads of 128 in bf16: 168 MB in 29.1 us, 5.8 TB/s; 16 tokens: 2.4 us, the launch).
+// heads of 128 in bf16: 168 MB in 29.2 us, 5.7 TB/s; 16 tokens: 2.4 us, the launch).  Heads whose
+// sizes allow only 8- or 4-byte vectors: 5000 tokens of 28 + 2 heads of 80, 40 or 20 of them turned,
+// 48 MB in 13.9 us (50.8 an element at a time).
 #include <cuda_runtime.h>
 
 #include "rk_device.cuh"
@@ -24,7 +26,9 @@ namespace rk {
 namespace {
 
 constexpr int THREADS = 256;
-constexpr int ROWS_AHEAD = 2;  // rows of a thread in flight, of two vectors each
+constexpr int MOST_TOKENS = 8;  // of a CTA: a table of 32 KB at most
+// Rows of a thread in flight, of two vectors each.
+constexpr int rows_ahead(int width) { return width == 8 ? 2 : 4; }
 
 struct RotaryParams {
   const void* in[2];    // queries, keys
@@ -47,31 +51,77 @@ struct RotaryParams {
 // tokens of 32 + 8 heads of 128: 32.8 us instead of 29.2), so the unit's number exchanges its four.
 __device__ __forceinline__ int table_at(int pair) { return pair ^ ((pair >> 3) & 6); }
 
-// Two vectors of 8 elements that a lane turns: the first and second elements of 8 pairs, which are
-// those of `unit` in the table's row.
-template <typename T>
-__device__ __forceinline__ void turn_halves(uint4& a, uint4& b, const float2* row, int unit) {
-  uint32_t* pa = reinterpret_cast<uint32_t*>(&a);
-  uint32_t* pb = reinterpret_cast<uint32_t*>(&b);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float2 x = Pack2<T>::to_floats(pa[j]), y = Pack2<T>::to_floats(pb[j]);
-    const float4 t = *reinterpret_cast<const float4*>(row + unit * 8 + ((2 * j) ^ (unit & 6)));  // cos, sin, cos, sin
-    pa[j] = Pack2<T>::from_floats(x.x * t.x - y.x * t.y, x.y * t.z - y.y * t.w);
-    pb[j] = Pack2<T>::from_floats(y.x * t.x + x.x * t.y, y.y * t.z + x.y * t.w);
+// W elements of 16 bits, loaded and stored at once.
+template <int W>
+struct Vector {
+  uint32_t w[W / 2];
+};
+template <>
+struct Vector<1> {};
+template <int W>
+__device__ __forceinline__ Vector<W> load_vector(const void* from) {
+  Vector<W> v;
+  if constexpr (W == 8) {
+    const uint4 x = ld_stream_v4(from);
+    v.w[0] = x.x;
+    v.w[1] = x.y;
+    v.w[2] = x.z;
+    v.w[3] = x.w;
+  } else if constexpr (W == 4) {
+    const uint2 x = __ldcs(static_cast<const uint2*>(from));
+    v.w[0] = x.x;
+    v.w[1] = x.y;
+  } else {
+    v.w[0] = __ldcs(static_cast<const uint32_t*>(from));
+  }
+  return v;
+}
+template <int W>
+__device__ __forceinline__ void store_vector(void* to, const Vector<W>& v) {
+  if constexpr (W == 8) {
+    *static_cast<uint4*>(to) = make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]);
+  } else if constexpr (W == 4) {
+    *static_cast<uint2*>(to) = make_uint2(v.w[0], v.w[1]);
+  } else {
+    *static_cast<uint32_t*>(to) = v.w[0];
   }
 }
 
-// A vector of 4 neighbouring pairs: the first (from = 0) or second (4) four of `unit`.
-template <typename T>
-__device__ __forceinline__ void turn_pairs(uint4& a, const float2* row, int unit, int from) {
-  uint32_t* pa = reinterpret_cast<uint32_t*>(&a);
+// Cosine and sine of two neighbouring pairs, the j-th (even) of those that begin at `at` =
+// table_at(a multiple of their number).
+__device__ __forceinline__ float4 turns_of(const float2* row, int at, int j) {
+  return *reinterpret_cast<const float4*>(row + (at ^ j));
+}
+
+// Two vectors that a lane turns: the first and second elements of W pairs from `pair` on.
+template <typename T, int W>
+__device__ __forceinline__ void turn_halves(Vector<W>& a, Vector<W>& b, const float2* row, int pair) {
+  const int at = table_at(pair);
 #pragma unroll
-  for (int j = 0; j < 4; j += 2) {
-    const float4 t = *reinterpret_cast<const float4*>(row + unit * 8 + ((from + j) ^ (unit & 6)));
-    const float2 x = Pack2<T>::to_floats(pa[j]), y = Pack2<T>::to_floats(pa[j + 1]);
-    pa[j] = Pack2<T>::from_floats(x.x * t.x - x.y * t.y, x.y * t.x + x.x * t.y);
-    pa[j + 1] = Pack2<T>::from_floats(y.x * t.z - y.y * t.w, y.y * t.z + y.x * t.w);
+  for (int j = 0; j < W / 2; ++j) {
+    const float2 x = Pack2<T>::to_floats(a.w[j]), y = Pack2<T>::to_floats(b.w[j]);
+    const float4 t = turns_of(row, at, 2 * j);  // cos, sin, cos, sin
+    a.w[j] = Pack2<T>::from_floats(x.x * t.x - y.x * t.y, x.y * t.z - y.y * t.w);
+    b.w[j] = Pack2<T>::from_floats(y.x * t.x + x.x * t.y, y.y * t.z + x.y * t.w);
+  }
+}
+
+// A vector of W / 2 neighbouring pairs from `pair` on.
+template <typename T, int W>
+__device__ __forceinline__ void turn_pairs(Vector<W>& a, const float2* row, int pair) {
+  if constexpr (W == 2) {
+    const float2 t = row[table_at(pair)];
+    const float2 x = Pack2<T>::to_floats(a.w[0]);
+    a.w[0] = Pack2<T>::from_floats(x.x * t.x - x.y * t.y, x.y * t.x + x.x * t.y);
+  } else {
+    const int at = table_at(pair);
+#pragma unroll
+    for (int j = 0; j < W / 2; j += 2) {
+      const float4 t = turns_of(row, at, j);
+      const float2 x = Pack2<T>::to_floats(a.w[j]), y = Pack2<T>::to_floats(a.w[j + 1]);
+      a.w[j] = Pack2<T>::from_floats(x.x * t.x - x.y * t.y, x.y * t.x + x.x * t.y);
+      a.w[j + 1] = Pack2<T>::from_floats(y.x * t.z - y.y * t.w, y.y * t.z + y.x * t.w);
+    }
   }
 }
 
@@ -80,11 +130,12 @@ __host__ __device__ constexpr int table_stride(int half) { return (half + 7) & ~
 
 // A CTA takes some tokens.  Each thread keeps one unit of a head (no division in the loop) and
 // walks over the heads of the tokens, ROWS of them in flight; the first are on their way while
-// the threads fill the table of the tokens' cosines and sines.  VEC: 16-byte vectors (head
-// sizes, strides and pointers allow them); otherwise a pair or an element at a time.
-template <typename T, bool INTERLEAVED, bool VEC>
-__global__ void __launch_bounds__(THREADS, VEC ? 6 : 1) rotary_kernel(RotaryParams p, int tokens_per_cta) {
-  constexpr int ROWS = VEC ? ROWS_AHEAD : 1;
+// the threads fill the table of the tokens' cosines and sines.  W: elements of a vector, the most
+// that head sizes, strides and pointers allow; 1: a pair or an element at a time.
+template <typename T, bool INTERLEAVED, int W>
+__global__ void __launch_bounds__(THREADS, W == 8 ? 6 : 5) rotary_kernel(RotaryParams p, int tokens_per_cta) {
+  constexpr bool VEC = W > 1;
+  constexpr int ROWS = VEC ? rows_ahead(W) : 1;
   extern __shared__ __align__(16) float2 table[];  // [tokens_per_cta][stride]
   const int stride = table_stride(p.half);
   pdl_begin();
@@ -106,11 +157,11 @@ __global__ void __launch_bounds__(THREADS, VEC ? 6 : 1) rotary_kernel(RotaryPara
       second = INTERLEAVED ? first + 1 : first + p.half;
       both = turns;
     } else if (INTERLEAVED || !turns) {
-      first = INTERLEAVED ? unit * 16 : 2 * p.half + (unit - p.turn_units) * 16;
-      second = first + 8;
+      first = INTERLEAVED ? unit * 2 * W : 2 * p.half + (unit - p.turn_units) * 2 * W;
+      second = first + W;
       both = second < p.head_dim;
     } else {
-      first = unit * 8;
+      first = unit * W;
       second = first + p.half;
       both = true;
     }
@@ -127,17 +178,17 @@ __global__ void __launch_bounds__(THREADS, VEC ? 6 : 1) rotary_kernel(RotaryPara
       }
     }
   };
-  uint4 a[ROWS], b[ROWS];
+  Vector<W> a[ROWS], b[ROWS];
   const auto source = [&](int t, int h) {
     const bool key = h >= p.query_heads;
     return static_cast<const T*>(key ? p.in[1] : p.in[0]) + (t0 + t) * (key ? p.token_stride[1] : p.token_stride[0]) +
            (key ? h - p.query_heads : h) * (key ? p.head_stride[1] : p.head_stride[0]);
   };
   const auto load = [&](int k, int t, int h) {
-    if (VEC) {
+    if constexpr (VEC) {
       const T* in = source(t, h);
-      a[k] = ld_stream_v4(in + first);
-      if (both) b[k] = ld_stream_v4(in + second);
+      a[k] = load_vector<W>(in + first);
+      if (both) b[k] = load_vector<W>(in + second);
     }
   };
   const auto turn_and_store = [&](int k, int t, int h) {
@@ -145,16 +196,16 @@ __global__ void __launch_bounds__(THREADS, VEC ? 6 : 1) rotary_kernel(RotaryPara
     const int head = key ? h - p.query_heads : h, nheads = key ? p.heads - p.query_heads : p.query_heads;
     T* out = static_cast<T*>(key ? p.out[1] : p.out[0]) + ((t0 + t) * nheads + head) * p.head_dim;
     const float2* cs = table + t * stride;
-    if (VEC) {
+    if constexpr (VEC) {
       if (INTERLEAVED) {
         // The border between turned and copied elements lies on a vector's.
-        if (first < 2 * p.half) turn_pairs<T>(a[k], cs, unit, 0);
-        if (second < 2 * p.half) turn_pairs<T>(b[k], cs, unit, 4);
+        if (first < 2 * p.half) turn_pairs<T, W>(a[k], cs, unit * W);
+        if (second < 2 * p.half) turn_pairs<T, W>(b[k], cs, unit * W + W / 2);
       } else if (turns) {
-        turn_halves<T>(a[k], b[k], cs, unit);
+        turn_halves<T, W>(a[k], b[k], cs, first);
       }
-      *reinterpret_cast<uint4*>(out + first) = a[k];
-      if (both) *reinterpret_cast<uint4*>(out + second) = b[k];
+      store_vector<W>(out + first, a[k]);
+      if (both) store_vector<W>(out + second, b[k]);
     } else {
       const T* in = source(t, h);
       if (turns) {
@@ -205,15 +256,16 @@ __global__ void __launch_bounds__(THREADS, VEC ? 6 : 1) rotary_kernel(RotaryPara
   }
 }
 
-template <typename T>
-cudaError_t launch(const RotaryParams& p, bool interleaved, bool vec, int per_cta, cudaStream_t s) {
+template <typename T, bool INTERLEAVED>
+cudaError_t launch(const RotaryParams& p, int width, int per_cta, cudaStream_t s) {
   const dim3 grid(static_cast<unsigned>((p.tokens + per_cta - 1) / per_cta));
   const size_t smem = static_cast<size_t>(per_cta) * table_stride(p.half) * sizeof(float2);
-  if (interleaved)
-    return vec ? launch_kernel(rotary_kernel<T, true, true>, grid, dim3(THREADS), smem, s, 0, p, per_cta)
-               : launch_kernel(rotary_kernel<T, true, false>, grid, dim3(THREADS), smem, s, 0, p, per_cta);
-  return vec ? launch_kernel(rotary_kernel<T, false, true>, grid, dim3(THREADS), smem, s, 0, p, per_cta)
-             : launch_kernel(rotary_kernel<T, false, false>, grid, dim3(THREADS), smem, s, 0, p, per_cta);
+  switch (width) {
+    case 8: return launch_kernel(rotary_kernel<T, INTERLEAVED, 8>, grid, dim3(THREADS), smem, s, 0, p, per_cta);
+    case 4: return launch_kernel(rotary_kernel<T, INTERLEAVED, 4>, grid, dim3(THREADS), smem, s, 0, p, per_cta);
+    case 2: return launch_kernel(rotary_kernel<T, INTERLEAVED, 2>, grid, dim3(THREADS), smem, s, 0, p, per_cta);
+    default: return launch_kernel(rotary_kernel<T, INTERLEAVED, 1>, grid, dim3(THREADS), smem, s, 0, p, per_cta);
+  }
 }
 
 }  // namespace
@@ -239,23 +291,33 @@ rk_status rotary_launch(const RotaryArgs& a, cudaStream_t s) {
   p.index_bits = a.index_bits;
   p.amplitude = a.amplitude;
   p.inverse = a.inverse ? 1 : 0;
-  bool vec = a.head_dim % 8 == 0 && (a.interleaved ? p.half % 4 == 0 : p.half % 8 == 0);
+  // The most elements that every vector's place and size allow.
+  int64_t places = a.head_dim | (a.interleaved ? 2 * p.half : p.half);
   for (int w = 0; w < 2; ++w)
-    vec = vec && aligned16(p.in[w]) && aligned16(p.out[w]) && p.token_stride[w] % 8 == 0 && p.head_stride[w] % 8 == 0;
-  if (vec) {
+    places |= p.token_stride[w] | p.head_stride[w] |
+              static_cast<int64_t>((reinterpret_cast<uintptr_t>(p.in[w]) | reinterpret_cast<uintptr_t>(p.out[w])) / sizeof(uint16_t));
+  const int width = places % 8 == 0 ? 8 : places % 4 == 0 ? 4 : places % 2 == 0 ? 2 : 1;
+  if (width > 1) {
     // Two vectors to a unit: neighbours, or the two halves of the pairs.
-    p.turn_units = p.half / 8;  // interleaved units look at their elements
-    p.units = a.interleaved ? (p.head_dim + 15) / 16 : p.turn_units + (p.head_dim - 2 * p.half + 15) / 16;
+    p.turn_units = p.half / width;  // interleaved units look at their elements
+    const int two = 2 * width;
+    p.units = a.interleaved ? (p.head_dim + two - 1) / two : p.turn_units + (p.head_dim - 2 * p.half + two - 1) / two;
   } else {
     p.turn_units = p.half;
     p.units = p.half + p.head_dim - 2 * p.half;
   }
-  // Few tokens: one CTA each, so that they spread over the SMs.  Many: two to a CTA (8192 tokens of
-  // 32 + 8 heads of 128: 29.1 us with two, 33.9 with one, 30.0 with four; 1000 tokens: 7.4, 5.9,
-  // 10.5).
-  const int per_cta = p.tokens >= 16 * static_cast<int64_t>(device_sm_count()) ? 2 : 1;
-  const cudaError_t e = a.dt == RK_DTYPE_BF16 ? launch<__nv_bfloat16>(p, a.interleaved, vec, per_cta, s)
-                                              : launch<__half>(p, a.interleaved, vec, per_cta, s);
+  // Few tokens: one CTA each, so that they spread over the SMs.  Many: as many to a CTA as keep its
+  // threads busy, but 4 CTAs for each SM (8192 tokens of 32 + 8 heads of 128: 29.1 us with two,
+  // 33.9 with one, 30.0 with four; 1000 tokens: 7.4, 5.9, 10.5).
+  const int64_t fill = (rows_ahead(width) * THREADS + p.heads * p.units - 1) / (p.heads * p.units);
+  const int64_t spread = p.tokens / (4 * static_cast<int64_t>(device_sm_count()));
+  const int64_t most = fill < spread ? fill : spread;
+  const int per_cta = static_cast<int>(most < 1 ? 1 : most > MOST_TOKENS ? MOST_TOKENS : most);
+  cudaError_t e;
+  if (a.dt == RK_DTYPE_BF16)
+    e = a.interleaved ? launch<__nv_bfloat16, true>(p, width, per_cta, s) : launch<__nv_bfloat16, false>(p, width, per_cta, s);
+  else
+    e = a.interleaved ? launch<__half, true>(p, width, per_cta, s) : launch<__half, false>(p, width, per_cta, s);
   note_launch("rotary_kernel");
   return cuda_status(e);
 }

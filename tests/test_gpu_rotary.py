@@ -68,6 +68,25 @@ def test_matches_the_rotation(tokens, query_heads, kv_heads, dim, rotary_dim, dt
     assert rk.get_last_dispatch()["selected"] == "native/rotary_embedding"
 
 
+@pytest.mark.parametrize("interleaved", [False, True], ids=["halves", "interleaved"])
+@pytest.mark.parametrize("offset", [1, 2, 4, 8])
+@pytest.mark.parametrize("tokens, heads, dim, rotary_dim", [(3, 3, 96, 24), (700, 2, 80, 20), (2500, 1, 72, 40), (5000, 3, 12, 4)])
+def test_vectors_of_every_width(tokens, heads, dim, rotary_dim, offset, interleaved):
+    """Rows that start 2, 4, 8 and 16 bytes off, with sizes that allow 2, 4, 8 and 16 bytes at a time; many tokens of few heads."""
+    import torch
+
+    import radeon_kernels as rk
+
+    gen = torch.Generator().manual_seed(tokens)
+    flat = torch.randn(offset + tokens * (heads + 1) * dim, generator=gen).half().cuda()[offset:].view(tokens, heads + 1, dim)
+    query, key = flat[:, :heads], flat[:, heads:]
+    positions = torch.arange(tokens, dtype=torch.int32, device="cuda") * 11
+    frequencies = rk.rotary_frequencies(rotary_dim)
+    out_q, out_k = rk.rotary_embedding(query, key, positions, frequencies, interleaved=interleaved)
+    _check(out_q, query, positions, frequencies, interleaved, 1.0, "fp16")
+    _check(out_k, key, positions, frequencies, interleaved, 1.0, "fp16")
+
+
 @pytest.mark.parametrize("positions", [[0], [2**30 + 7, -3], [131071, 1048575, -(2**31)], [2**40, -(2**40) + 1]])
 def test_far_and_negative_positions(positions):
     import torch
