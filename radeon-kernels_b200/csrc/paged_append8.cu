@@ -17,9 +17,10 @@
 // slot.  A run is one block's tokens, so a warp that owns (run, head, K or V) owns
 // (block, head, K or V) alone: it takes the largest magnitude over the run's rows, holds them
 // in registers (8 x 16 bytes a lane: 16 rows at head_dim 128), and stores them with the
-// new scale.  No atomics on data, no second pass over it.  A block whose tokens are not
-// adjacent would have two owners: only the first run is stored, the others are skipped and
-// reported.
+// new scale.  Where blocks are larger than that, teams of 2 to 8 warps do, and agree on the
+// magnitude in shared memory.  No atomics on data, no second pass over it.  A block whose
+// tokens are not adjacent would have two owners: only the first run is stored, the others are
+// skipped and reported.
 //
 // Up to SCAN_TOKENS tokens a CTA per token looks for its run and through the earlier slots by
 // itself, in one launch.  Beyond that those looks would be quadratic: in a launch before, each
@@ -49,6 +50,7 @@ constexpr int WARPS = THREADS / 32;
 constexpr int SCAN_TOKENS = 2048;  // more tokens than this: a list of runs and claims
 constexpr int HELD = 8;            // 16-byte vectors a lane keeps
 constexpr int APPEND_CTAS = 3;      // resident on an SM
+constexpr int HELPERS = 8;          // tokens of a long run whose CTAs store it
 
 // The tokens of one block: `len` from `token` on, ascending from `offset` to `last` in `block`.
 struct Run {
@@ -65,6 +67,7 @@ struct AppendParams {
   int32_t* claims;  // per block: a token that starts a run of it; or anything
   uint8_t* rivals;  // per token that starts a run: whether another run of its block is known
   int parts;        // CTAs that share THREADS tokens
+  int team;         // warps that hold a full block of a head
   int64_t capacity;  // num_blocks * block_size
   int32_t tokens;
   int heads, block_size, index_bits;
@@ -234,27 +237,57 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t w, float was, float inv) {
   return C::pack4((a.x * was) * inv, (a.y * was) * inv, (b.x * was) * inv, (b.y * was) * inv);
 }
 
-// One run of one head of K or V (`pair` < heads: K), by a warp.  `is_first` says whether the run
+// Warps that store a run's head together: one, or `size`, a power of two.
+struct Alone {
+  static constexpr int size = 1, rank = 0, UNROLL = 1;
+  __device__ __forceinline__ float largest(float x, int) { return x; }
+};
+struct Team {
+  static constexpr int UNROLL = 4;  // of the rows that are not held
+  int size, rank, barrier;
+  float* most;  // [2][size] in shared memory
+  int turn;
+  __device__ __forceinline__ Team(int warps, int warp, float* places)
+      : size(warps), rank(warp % warps), barrier(1 + warp / warps), most(places + warp / warps * warps), turn(0) {}
+  // The largest of all warps' values.  A warp can be one call ahead of another at most, so two sets of
+  // places are enough.
+  __device__ __forceinline__ float largest(float x, int lane) {
+    if (size == 1) return x;
+    float* const at = most + turn * WARPS;
+    turn ^= 1;
+    if (lane == 0) at[rank] = x;
+    asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(size * 32) : "memory");
+    for (int i = 0; i < size; ++i) x = fmaxf(x, at[i]);
+    return x;
+  }
+};
+
+// Rows of a head that a warp keeps in registers.
+__host__ __device__ constexpr int held_rows(int head_dim) { return HELD * (256 / head_dim); }
+
+// One run of one head of K or V (`pair` < heads: K), by a team.  `is_first` says whether the run
 // is the first of its block; it is asked when the rows are there, before anything is stored.
-template <typename T, typename C, int D, typename First>
-__device__ __forceinline__ void append_run(const AppendParams& p, const Run& run, int pair, int lane, const First& is_first) {
+template <typename T, typename C, int D, typename Warps, typename First>
+__device__ __forceinline__ void append_run(const AppendParams& p, const Run& run, int pair, int lane, Warps& team,
+                                           const First& is_first) {
   constexpr int LANES = D / 8;      // lanes of a row, 8 elements each
-  constexpr int ROWS = 32 / LANES;  // rows side by side
-  const int row = lane / LANES, at = (lane - row * LANES) * 8;
+  constexpr int ROWS = 32 / LANES;  // rows of a warp side by side
+  const int side = ROWS * team.size;
+  const int row = lane / LANES + ROWS * team.rank, at = (lane % LANES) * 8;
   const bool which = pair >= p.heads;
   const int head = which ? pair - p.heads : pair;
   const int64_t stride = which ? p.token_stride[1] : p.token_stride[0];
   const T* src = static_cast<const T*>(which ? p.rows[1] : p.rows[0]) + run.token * stride +
                  head * (which ? p.head_stride[1] : p.head_stride[0]) + at;
-  const int rows = run.len - row;  // from this lane's first on, ROWS apart
+  const int rows = run.len - row;  // from this lane's first on, `side` apart
   uint4 held[HELD];
   {
     const T* from = src + row * stride;
 #pragma unroll
     for (int k = 0; k < HELD; ++k) {
       held[k] = make_uint4(0, 0, 0, 0);
-      if (k * ROWS < rows) held[k] = ld_stream_v4(from);
-      from += ROWS * stride;
+      if (k * side < rows) held[k] = ld_stream_v4(from);
+      from += side * stride;
     }
   }
   const int64_t slot_bytes = static_cast<int64_t>(p.heads) * D;
@@ -278,11 +311,12 @@ __device__ __forceinline__ void append_run(const AppendParams& p, const Run& run
   // registers of the rows themselves.
 #pragma unroll
   for (int k = 0; k < HELD; ++k) asm volatile("" : "+r"(held[k].x), "+r"(held[k].y), "+r"(held[k].z), "+r"(held[k].w));
-#pragma unroll 1
-  for (int r = row + HELD * ROWS; r < run.len; r += ROWS)
+#pragma unroll Warps::UNROLL
+  for (int r = row + HELD * side; r < run.len; r += side)
     amax = fmaxf(amax, amax8<T>(*reinterpret_cast<const uint4*>(src + r * stride)));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  amax = team.largest(amax, lane);  // and every warp has read the old scale
   const float now = fmaxf(was, C::scale_for(amax));
   const float inv = 1.0f / now;
 
@@ -291,7 +325,7 @@ __device__ __forceinline__ void append_run(const AppendParams& p, const Run& run
   if (run.offset > 0 && now != was) {
     // Rows that stay: those below the last new one that the run does not write.
 #pragma unroll 1
-    for (int r = row; r < run.last; r += ROWS) {
+    for (int r = row; r < run.last; r += side) {
       bool stays = r < run.offset;
       if (!stays && !dense) {
         int lo = 0, hi = run.len - 1;  // the run's slots ascend
@@ -315,64 +349,92 @@ __device__ __forceinline__ void append_run(const AppendParams& p, const Run& run
     uint8_t* to = dst + (run.offset + row) * slot_bytes;
 #pragma unroll
     for (int k = 0; k < HELD; ++k) {
-      if (k * ROWS < rows) *reinterpret_cast<uint2*>(to) = store8<T, C>(held[k], inv);
-      to += ROWS * slot_bytes;
+      if (k * side < rows) *reinterpret_cast<uint2*>(to) = store8<T, C>(held[k], inv);
+      to += side * slot_bytes;
     }
   }
-#pragma unroll 1
-  for (int r = row + (dense ? HELD * ROWS : 0); r < run.len; r += ROWS) {
+#pragma unroll Warps::UNROLL
+  for (int r = row + (dense ? HELD * side : 0); r < run.len; r += side) {
     const int64_t o = dense ? run.offset + r : slot_of(p, run.token + r) - slot0;
     *reinterpret_cast<uint2*>(dst + o * slot_bytes) = store8<T, C>(*reinterpret_cast<const uint4*>(src + r * stride), inv);
   }
   __syncwarp();  // every lane has read the old scale
-  if (lane == 0) *scale = now;
+  if (lane == 0 && team.rank == 0) *scale = now;
 }
 
-// Few tokens: a CTA (of each 8 heads of K and V) per token, which goes on if a run starts there.
-template <typename T, typename C, int D>
+// Few tokens: a CTA (of each 8 heads of K and V) per token, which goes on if a run starts there.  The CTAs
+// of the next tokens of a run help if it is longer than a warp holds: teams of p.team warps store it.
+template <typename T, typename C, int D, bool TEAMS>
 __global__ void __launch_bounds__(THREADS) paged_append8_kernel(AppendParams p, KernelCtl ctl) {
+  __shared__ float s_most[2 * WARPS];
   pdl_begin();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int pair = static_cast<int>(blockIdx.y) * WARPS + warp;
-  const int64_t t = blockIdx.x;
+  int64_t t = blockIdx.x;
   const int64_t slot = slot_of(p, t);
   const int64_t before = t > 0 ? slot_of(p, t - 1) : -1;
   if (slot >= p.capacity && threadIdx.x == 0 && blockIdx.y == 0) atomicOr(ctl.status, RK_DEV_ERR_BAD_INDEX);
   if (slot < 0 || slot >= p.capacity) return;
   const int block = block_of(p, slot);
-  if (goes_on(p, before, slot, block)) return;
-  // A block that an earlier token went to has been stored by that run.
   const int64_t slot0 = static_cast<int64_t>(block) * p.block_size;
+  int helps = 0;  // the token's number in its run
+  int64_t first = slot;
+  if (goes_on(p, before, slot, block)) {
+    if (!TEAMS) return;
+    // The run's first token, if it is one of the last few.
+    const int64_t u = t - lane;
+    int64_t here = -1;
+    bool on = false;
+    if (u > 0 && lane < HELPERS) {
+      here = slot_of(p, u);
+      on = here < slot0 + p.block_size && goes_on(p, slot_of(p, u - 1), here, block);
+    } else if (u == 0) {
+      here = slot_of(p, u);
+    }
+    helps = __ffs(~__ballot_sync(0xffffffffu, on)) - 1;
+    if (helps >= HELPERS) return;
+    t -= helps;
+    first = __shfl_sync(0xffffffffu, here, helps);
+  }
+  const int len = 1 + more_tokens(p, t, block, lane);
+  if (helps > 0 && len <= held_rows(D)) return;
+  // A block that an earlier token went to has been stored by that run.
   bool seen = false;
   for (int64_t i = threadIdx.x; i < t; i += THREADS) {
     const int64_t other = slot_of(p, i);
     seen = seen || (other >= slot0 && other < slot0 + p.block_size);
   }
   if (__syncthreads_or(seen)) {
-    if (threadIdx.x == 0 && blockIdx.y == 0) atomicOr(ctl.status, RK_DEV_ERR_BAD_INDEX);
+    if (threadIdx.x == 0 && blockIdx.y == 0 && helps == 0) atomicOr(ctl.status, RK_DEV_ERR_BAD_INDEX);
     return;
   }
-  if (pair >= 2 * p.heads) return;
-  const int len = 1 + more_tokens(p, t, block, lane);
-  const Run run{static_cast<int32_t>(t), block, static_cast<int16_t>(slot - slot0), static_cast<int16_t>(len),
-                static_cast<int16_t>((len == 1 ? slot : slot_of(p, t + len - 1)) - slot0), 0};
-  append_run<T, C, D>(p, run, pair, lane, [] { return true; });
+  const Run run{static_cast<int32_t>(t), block, static_cast<int16_t>(first - slot0), static_cast<int16_t>(len),
+                static_cast<int16_t>((len == 1 ? first : slot_of(p, t + len - 1)) - slot0), 0};
+  const auto is_first = [] { return true; };
+  if (TEAMS && len > held_rows(D)) {
+    Team team(p.team, warp, s_most);
+    const int pair = (helps * static_cast<int>(gridDim.y) + static_cast<int>(blockIdx.y)) * (WARPS / team.size) + warp / team.size;
+    if (pair < 2 * p.heads) append_run<T, C, D>(p, run, pair, lane, team, is_first);
+  } else {
+    Alone team;
+    const int pair = static_cast<int>(blockIdx.y) * WARPS + warp;
+    if (pair < 2 * p.heads) append_run<T, C, D>(p, run, pair, lane, team, is_first);
+  }
 }
 
-// Many tokens: `parts` CTAs for each THREADS of them, whose warps take the runs' heads of K and V in
-// turn.  Each CTA lists the runs for itself and loads its warps' first rows while the claims
-// are still being made.
-template <typename T, typename C, int D>
+// Many tokens: `parts` CTAs for each THREADS of them, whose warps or teams take the runs' heads of K and
+// V in turn.  Each CTA lists the runs for itself and loads its first rows while the claims are still
+// being made.
+template <typename T, typename C, int D, bool TEAMS>
 __global__ void __launch_bounds__(THREADS, APPEND_CTAS) paged_append8_runs_kernel(AppendParams p, KernelCtl ctl) {
   __shared__ __align__(16) Run s_runs[THREADS];
+  __shared__ float s_most[2 * WARPS];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int list = static_cast<int>(blockIdx.x) / p.parts, part = static_cast<int>(blockIdx.x) - list * p.parts;
   const int pairs = 2 * p.heads;
   const int items = list_runs(p, static_cast<int64_t>(list) * THREADS, s_runs) * pairs;
   bool waited = false;
-#pragma unroll 1
-  for (int item = part * WARPS + (threadIdx.x >> 5); item < items; item += p.parts * WARPS) {
+  const auto store = [&](auto& team, int item) {
     const int at = item / pairs, pair = item - at * pairs;
     const int4 raw = *reinterpret_cast<const int4*>(s_runs + at);
     const Run run{raw.x, raw.y, static_cast<int16_t>(raw.z & 0xFFFF), static_cast<int16_t>(raw.z >> 16),
@@ -384,7 +446,7 @@ __global__ void __launch_bounds__(THREADS, APPEND_CTAS) paged_append8_runs_kerne
       rival = __ldcg(p.rivals + run.token);
     };
     if (waited) look();
-    append_run<T, C, D>(p, run, pair, lane, [&] {
+    append_run<T, C, D>(p, run, pair, lane, team, [&] {
       if (!waited) {
         wait_for_earlier_kernels();
         waited = true;
@@ -398,26 +460,41 @@ __global__ void __launch_bounds__(THREADS, APPEND_CTAS) paged_append8_runs_kerne
         const int64_t slot = t0 + lane < run.token ? slot_of(p, t0 + lane) : -1;
         seen = __any_sync(0xffffffffu, slot >= slot0 && slot < slot0 + p.block_size) != 0;
       }
-      if (seen && lane == 0 && pair == 0) atomicOr(ctl.status, RK_DEV_ERR_BAD_INDEX);
+      if (seen && lane == 0 && pair == 0 && team.rank == 0) atomicOr(ctl.status, RK_DEV_ERR_BAD_INDEX);
       return !seen;
     });
+  };
+  if constexpr (TEAMS) {
+    const int teams = WARPS / p.team;
+    Team team(p.team, warp, s_most);
+#pragma unroll 1
+    for (int item = part * teams + warp / p.team; item < items; item += p.parts * teams) store(team, item);
+  } else {
+    Alone team;
+#pragma unroll 1
+    for (int item = part * WARPS + warp; item < items; item += p.parts * WARPS) store(team, item);
   }
   if (!waited) wait_for_earlier_kernels();
 }
 
 int64_t lists_of(int64_t tokens) { return (tokens + THREADS - 1) / THREADS; }
 
-template <typename T, typename C, int D>
+template <typename T, typename C, int D, bool TEAMS>
 cudaError_t launch(const AppendParams& p, const KernelCtl& ctl, cudaStream_t s) {
   if (p.claims == nullptr) {
     const dim3 grid(static_cast<unsigned>(p.tokens), static_cast<unsigned>((2 * p.heads + WARPS - 1) / WARPS));
     note_launch("paged_append8_kernel");
-    return launch_kernel(paged_append8_kernel<T, C, D>, grid, dim3(THREADS), 0, s, 0, p, ctl);
+    return launch_kernel(paged_append8_kernel<T, C, D, TEAMS>, grid, dim3(THREADS), 0, s, 0, p, ctl);
   }
   const int64_t lists = lists_of(p.tokens);
   note_launch("paged_append8_runs_kernel");
-  return launch_kernel(paged_append8_runs_kernel<T, C, D>, dim3(static_cast<unsigned>(lists * p.parts)), dim3(THREADS), 0,
-                       s, 0, p, ctl);
+  return launch_kernel(paged_append8_runs_kernel<T, C, D, TEAMS>, dim3(static_cast<unsigned>(lists * p.parts)),
+                       dim3(THREADS), 0, s, 0, p, ctl);
+}
+
+template <typename T, typename C, int D>
+cudaError_t launch(const AppendParams& p, const KernelCtl& ctl, cudaStream_t s) {
+  return p.team > 1 ? launch<T, C, D, true>(p, ctl, s) : launch<T, C, D, false>(p, ctl, s);
 }
 
 template <typename T, typename C>
@@ -461,6 +538,10 @@ rk_status paged_append8_launch(const PagedAppend8Args& a, void* workspace, size_
   p.capacity = a.num_blocks * a.block_size;
   p.heads = static_cast<int>(a.kv_heads);
   p.block_size = static_cast<int>(a.block_size);
+  // Warps that together hold a full block of a head: rows read once and a block's worth of loads at
+  // once (36k tokens of 8 heads of 256 in blocks of 128: 142 us with one warp, 57 with eight).
+  p.team = 1;
+  while (p.team < WARPS && p.team * held_rows(static_cast<int>(a.head_dim)) < p.block_size) p.team *= 2;
   if (need > 0) {
     const int64_t lists = lists_of(a.tokens);
     p.claims = static_cast<int32_t*>(workspace);
@@ -468,7 +549,7 @@ rk_status paged_append8_launch(const PagedAppend8Args& a, void* workspace, size_
     // CTAs that fill the GPU four times (43k tokens: the same from three to six; each lists its runs,
     // so not more), each with a run for every warp if blocks fill up.
     const int64_t fill = static_cast<int64_t>(device_sm_count()) * APPEND_CTAS * 4;
-    const int64_t most = (THREADS / p.block_size + 1) * 2 * static_cast<int64_t>(p.heads) / WARPS + 1;
+    const int64_t most = (THREADS / p.block_size + 1) * 2 * static_cast<int64_t>(p.heads) * p.team / WARPS + 1;
     const int64_t parts = (fill + lists - 1) / lists;
     p.parts = static_cast<int>(parts < most ? parts : most);
     const cudaError_t e = launch_kernel(append_claims_kernel, dim3(static_cast<unsigned>(lists)), dim3(THREADS), 0, s, 0, p, ctl);

@@ -106,6 +106,23 @@ def test_append_matches_its_definition(dim, heads, size, lengths, dtype, kind):
     _append(rng, _rows(rng, len(slots), heads, dim, dtype), slots, kind, blocks, size, "int32" if size % 3 else "int64")
 
 
+@pytest.mark.parametrize("tokens", [0, 2100], ids=["scan", "claims"])
+@pytest.mark.parametrize("dim, heads, size", [(256, 2, 16), (256, 9, 64), (128, 5, 128), (64, 1, 1000), (256, 1, 1024), (128, 3, 24)])
+def test_long_runs_of_large_blocks(dim, heads, size, tokens):
+    """Runs that one warp does not hold: new blocks, blocks that go on with larger values, gaps, runs that come again."""
+    rng = np.random.default_rng(dim + size)
+    blocks = 6
+    pad = lambda slots: slots + [-1] * max(0, tokens - len(slots))
+    whole = lambda block, first, last, step=1: list(range(block * size + first, block * size + last, step))
+    cache = scales = None
+    for i, slots in enumerate((whole(0, 0, size - 2) + whole(3, 0, size // 2) + whole(1, 1, 9),
+                               whole(3, size // 2, size) + whole(1, 9, size, 2) + whole(0, size - 2, size) + whole(4, 0, 1),
+                               whole(2, 0, size - 5) + whole(5, 3, size) + whole(2, size - 5, size) + whole(4, 1, 14),
+                               [-1] + whole(1, 10, size, 3) + [-1, -1] + whole(5, 0, size))):
+        rows = [r * 2.0**i for r in _rows(rng, max(len(slots), tokens), heads, dim, "bf16")]
+        cache, scales = _append(rng, rows, pad(slots), "int8" if size % 3 else "e4m3", blocks, size, scales=scales, cache=cache)
+
+
 @pytest.mark.parametrize("kind", ["e4m3", "int8"])
 def test_a_block_that_fills_token_by_token(kind):
     """Magnitudes grow and fall: the scale follows the largest, older rows are re-rounded."""
