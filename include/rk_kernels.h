@@ -441,7 +441,8 @@ RK_API rk_status rk_sdpa(const void* query, const void* key, const void* value, 
  * projection need no copy; query_out, key_out: dense, overlapping no input.  positions: [tokens] int32 or
  * int64 (index_bits), any sign; frequencies: [rotary_dim / 2] fp64, radians per position.
  * Angles are formed and reduced in fp64, so they are as exact at position 2^30 as at 1; the
- * turn is fp32 and each output is rounded once.  rotary_dim even, 2 <= rotary_dim <= head_dim
+ * turn is fp32 and each output is rounded once.  Pointers are aligned to their elements, here and
+ * in the three operators that follow (RK_ERR_UNSUPPORTED otherwise).  rotary_dim even, 2 <= rotary_dim <= head_dim
  * <= 1024; query_heads, kv_heads <= 32767.  tokens == 0: nothing to do.  No counterpart in
  * the reference.
  */

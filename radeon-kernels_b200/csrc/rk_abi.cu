@@ -5,6 +5,7 @@
 
 #include <atomic>
 #include <cstring>
+#include <initializer_list>
 #include <mutex>
 #include <string>
 
@@ -421,6 +422,13 @@ rk_status rk_sdpa(const void* query, const void* key, const void* value, void* o
                      is_causal != 0, scale, dt, reinterpret_cast<cudaStream_t>(stream));
 }
 
+// Whether all pointers are multiples of `bytes`: of the elements that kernels load through them.
+static bool aligned_to(size_t bytes, std::initializer_list<const void*> pointers) {
+  for (const void* p : pointers)
+    if (reinterpret_cast<uintptr_t>(p) % bytes != 0) return false;
+  return true;
+}
+
 rk_status rk_rotary_embedding(const void* query, const void* key, const void* positions,
                               const double* frequencies, void* query_out, void* key_out,
                               int64_t tokens, int64_t query_heads, int64_t kv_heads,
@@ -438,6 +446,9 @@ rk_status rk_rotary_embedding(const void* query, const void* key, const void* po
   if (query == nullptr || key == nullptr || positions == nullptr || frequencies == nullptr ||
       query_out == nullptr || key_out == nullptr)
     return RK_ERR_INVALID_ARGUMENT;
+  if (!aligned_to(2, {query, key, query_out, key_out}) || !aligned_to(index_bits / 8, {positions}) ||
+      !aligned_to(8, {frequencies}))
+    return RK_ERR_UNSUPPORTED;
   if (current_device_info() == nullptr) return RK_ERR_NO_DEVICE;
   RotaryArgs a{};
   a.query = query;
@@ -477,6 +488,9 @@ rk_status rk_paged_slots(void* block_tables, const void* context_lengths, const 
     return RK_ERR_INVALID_ARGUMENT;
   if (max_blocks > INT32_MAX || block_size > INT32_MAX || max_blocks * block_size > INT32_MAX ||
       batch > INT32_MAX || tokens > INT32_MAX)
+    return RK_ERR_UNSUPPORTED;
+  if (!aligned_to(index_bits / 8, {block_tables, context_lengths, new_lengths, free_blocks, positions, lengths_out, blocks_used}) ||
+      !aligned_to(8, {slot_mapping}))
     return RK_ERR_UNSUPPORTED;
   if (current_device_info() == nullptr) return RK_ERR_NO_DEVICE;
   PagedSlotsArgs a{};
@@ -528,7 +542,7 @@ rk_status rk_paged_cache_append_8bit(const void* key, const void* value, void* k
     return RK_ERR_INVALID_ARGUMENT;
   if (!aligned16(key) || !aligned16(value) || !aligned16(key_cache) || !aligned16(value_cache) ||
       key_token_stride % 8 != 0 || key_head_stride % 8 != 0 || value_token_stride % 8 != 0 ||
-      value_head_stride % 8 != 0)
+      value_head_stride % 8 != 0 || !aligned_to(4, {key_scales, value_scales}) || !aligned_to(index_bits / 8, {slot_mapping}))
     return RK_ERR_UNSUPPORTED;
   if (current_device_info() == nullptr) return RK_ERR_NO_DEVICE;
   PagedAppend8Args a{};
@@ -579,7 +593,8 @@ rk_status rk_paged_attention_decode_8bit(
   if (query == nullptr || key_cache == nullptr || value_cache == nullptr || key_scales == nullptr ||
       value_scales == nullptr || block_tables == nullptr || context_lengths == nullptr || out == nullptr)
     return RK_ERR_INVALID_ARGUMENT;
-  if ((reinterpret_cast<uintptr_t>(query) & 7u) != 0 || !aligned16(out) || !aligned16(key_cache) || !aligned16(value_cache))
+  if (!aligned_to(8, {query}) || !aligned16(out) || !aligned16(key_cache) || !aligned16(value_cache) ||
+      !aligned_to(4, {key_scales, value_scales}) || !aligned_to(index_bits / 8, {block_tables, context_lengths}))
     return RK_ERR_UNSUPPORTED;
   // Positions of a unit's last tile stay below 2^31.
   if (num_blocks > INT32_MAX || block_size > INT32_MAX || max_blocks > INT32_MAX ||

@@ -304,10 +304,19 @@ def test_c_entries_check_their_arguments():
         assert attention(**changes) == bad, changes
     for changes in (dict(width=2**21, size=2**10), dict(p=ctypes.c_void_p(264 + 4))):
         assert attention(**{"p": some, **changes}) == no, changes
-    for at, offset in ((0, 4), (1, 8), (2, 8), (7, 8)):  # query; caches; output
-        pointers = [some] * 8
+    def off(count, at, offset):
+        pointers = [some] * count
         pointers[at] = ctypes.c_void_p(256 + offset)
-        assert lib.rk_paged_attention_decode_8bit(*pointers, 1, 2, 1, 64, 1, 16, 1, 1.0, 1, 0, 32, null, 0, null) == no, at
+        return pointers
+
+    for at, offset in ((0, 4), (1, 8), (2, 8), (3, 2), (4, 1), (5, 4), (6, 4), (7, 8)):
+        assert lib.rk_paged_attention_decode_8bit(*off(8, at, offset), 1, 2, 1, 64, 1, 16, 1, 1.0, 1, 0, 64, null, 0, null) == no, at
+    for at, offset in ((0, 8), (1, 8), (2, 8), (3, 8), (4, 2), (5, 1), (6, 4)):
+        assert lib.rk_paged_cache_append_8bit(*off(7, at, offset), 1, 1, 64, 1, 16, 64, 64, 64, 64, 1, 0, 64, null, 0, null) == no, at
+    for at, offset in ((0, 1), (1, 1), (2, 4), (3, 4), (4, 1), (5, 1)):
+        assert lib.rk_rotary_embedding(*off(6, at, offset), 1, 2, 1, 64, 32, 128, 64, 64, 64, 0, 0, 1.0, 1, 64, null) == no, at
+    for at, offset in ((0, 4), (1, 4), (2, 4), (3, 4), (4, 4), (5, 4), (6, 4), (7, 4)):
+        assert lib.rk_paged_slots(*off(8, at, offset), 1, 1, 1, 1, 1, 64, null) == no, at
     assert lib.rk_paged_attention_decode_8bit_workspace_size(3, 2, 64, ctypes.byref(size)) == bad and size.value == 0
     assert lib.rk_paged_attention_decode_8bit_workspace_size(2, 2, 64, None) == bad
 
