@@ -47,7 +47,7 @@ namespace {
 
 constexpr int THREADS = 256;
 constexpr int WARPS = THREADS / 32;
-constexpr int SCAN_TOKENS = 2048;  // more tokens than this: a list of runs and claims
+constexpr int SCAN_TOKENS = 256;   // more tokens than this: a list of runs and claims
 constexpr int HELD = 8;            // 16-byte vectors a lane keeps
 constexpr int APPEND_CTAS = 3;      // resident on an SM
 constexpr int HELPERS = 8;          // tokens of a long run whose CTAs store it
@@ -133,8 +133,9 @@ __global__ void __launch_bounds__(THREADS) append_claims_kernel(AppendParams p, 
   p.rivals[t] = claimed != static_cast<int32_t>(t) && starts_run(p, claimed, block);
 }
 
-// The runs that start in THREADS tokens from t0 on, in their order; returns how many.
-__device__ __forceinline__ int list_runs(const AppendParams& p, int64_t t0, Run* runs) {
+// The runs that start in THREADS tokens from t0 on, in their order; returns how many, and whether one
+// is longer than `held`.
+__device__ __forceinline__ int list_runs(const AppendParams& p, int64_t t0, Run* runs, int held, bool* longer) {
   __shared__ int64_t s_slots[THREADS];
   __shared__ uint32_t s_breaks[WARPS];  // tokens that do not go on with the one before
   __shared__ uint32_t s_starts[WARPS];
@@ -187,7 +188,7 @@ __device__ __forceinline__ int list_runs(const AppendParams& p, int64_t t0, Run*
         Run{static_cast<int32_t>(t), block, static_cast<int16_t>(slot - first),
             static_cast<int16_t>(open ? len + more : len), static_cast<int16_t>(last - first), 0};
   }
-  __syncthreads();
+  *longer = __syncthreads_or((open ? len + more : len) > held) != 0;
   return all;
 }
 
@@ -421,8 +422,8 @@ __global__ void __launch_bounds__(THREADS) paged_append8_kernel(AppendParams p, 
   }
 }
 
-// Many tokens: `parts` CTAs for each THREADS of them, whose warps or teams take the runs' heads of K and
-// V in turn.  Each CTA lists the runs for itself and loads its first rows while the claims are still
+// Many tokens: `parts` CTAs for each THREADS of them, whose warps, or teams if a run is longer than a warp
+// holds, take the runs' heads of K and V in turn.  Each CTA lists the runs for itself and loads its first rows while the claims are still
 // being made.
 template <typename T, typename C, int D, bool TEAMS>
 __global__ void __launch_bounds__(THREADS, APPEND_CTAS) paged_append8_runs_kernel(AppendParams p, KernelCtl ctl) {
@@ -432,7 +433,8 @@ __global__ void __launch_bounds__(THREADS, APPEND_CTAS) paged_append8_runs_kerne
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int list = static_cast<int>(blockIdx.x) / p.parts, part = static_cast<int>(blockIdx.x) - list * p.parts;
   const int pairs = 2 * p.heads;
-  const int items = list_runs(p, static_cast<int64_t>(list) * THREADS, s_runs) * pairs;
+  bool longer;
+  const int items = list_runs(p, static_cast<int64_t>(list) * THREADS, s_runs, held_rows(D), &longer) * pairs;
   bool waited = false;
   const auto store = [&](auto& team, int item) {
     const int at = item / pairs, pair = item - at * pairs;
@@ -464,7 +466,7 @@ __global__ void __launch_bounds__(THREADS, APPEND_CTAS) paged_append8_runs_kerne
       return !seen;
     });
   };
-  if constexpr (TEAMS) {
+  if (TEAMS && longer) {
     const int teams = WARPS / p.team;
     Team team(p.team, warp, s_most);
 #pragma unroll 1
@@ -547,11 +549,12 @@ rk_status paged_append8_launch(const PagedAppend8Args& a, void* workspace, size_
     p.claims = static_cast<int32_t*>(workspace);
     p.rivals = reinterpret_cast<uint8_t*>(p.claims + a.num_blocks);
     // CTAs that fill the GPU four times (43k tokens: the same from three to six; each lists its runs,
-    // so not more), each with a run for every warp if blocks fill up.
-    const int64_t fill = static_cast<int64_t>(device_sm_count()) * APPEND_CTAS * 4;
+    // so not more), each with a run for every warp if blocks fill up -- but at least once, for
+    // blocks that get a token each (600 tokens of 8 heads: 20 us with a run for every warp).
+    const int64_t once = static_cast<int64_t>(device_sm_count()) * APPEND_CTAS, fill = 4 * once;
     const int64_t most = (THREADS / p.block_size + 1) * 2 * static_cast<int64_t>(p.heads) * p.team / WARPS + 1;
-    const int64_t parts = (fill + lists - 1) / lists;
-    p.parts = static_cast<int>(parts < most ? parts : most);
+    const int64_t parts = (fill + lists - 1) / lists, least = (once + lists - 1) / lists;
+    p.parts = static_cast<int>(parts < most ? parts : most < least ? least : most);
     const cudaError_t e = launch_kernel(append_claims_kernel, dim3(static_cast<unsigned>(lists)), dim3(THREADS), 0, s, 0, p, ctl);
     note_launch("append_claims_kernel");
     if (e != cudaSuccess) return cuda_status(e);
