@@ -12,8 +12,8 @@
 // those that need them; entries of blocks that a request had are only read.
 //
 // What bounds it: launch and latency -- lengths, scan, table or free list, slot -- at all sizes of
-// use (a token each of 256 requests 3.3 us on the device, 64k tokens of 61 requests 4.4 us for
-// 1 MB written).
+// use (a token each of 256 requests 3.3 us on the device, of 896 requests 5.1; 64k tokens of 61
+// requests 4.4 us for 1 MB written).
 #include <cuda_runtime.h>
 
 #include "rk_device.cuh"
@@ -22,8 +22,7 @@
 namespace rk {
 namespace {
 
-constexpr int THREADS = 256;
-constexpr int TOKENS_PER_CTA = 512;
+constexpr int FEW = 256, MANY = 1024;  // threads of a CTA, by the number of requests
 
 template <typename Index>
 struct SlotParams {
@@ -38,9 +37,8 @@ struct SlotParams {
   int64_t batch, max_blocks, block_size, free_count, tokens;
 };
 
-// Inclusive sums over the CTA of two values, in thread order.
-__device__ __forceinline__ void scan2(int64_t& a, int64_t& b, int64_t (*warp_sums)[2]) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// Inclusive sums over the lanes of two values.
+__device__ __forceinline__ void scan_lanes2(int64_t& a, int64_t& b, int lane) {
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int64_t x = __shfl_up_sync(0xffffffffu, a, o), y = __shfl_up_sync(0xffffffffu, b, o);
@@ -49,18 +47,37 @@ __device__ __forceinline__ void scan2(int64_t& a, int64_t& b, int64_t (*warp_sum
       b += y;
     }
   }
+}
+
+// Inclusive sums over the CTA of two values, in thread order.
+template <int WARPS>
+__device__ __forceinline__ void scan2(int64_t& a, int64_t& b, int64_t (*warp_sums)[2]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  scan_lanes2(a, b, lane);
   if (lane == 31) {
     warp_sums[warp][0] = a;
     warp_sums[warp][1] = b;
   }
   __syncthreads();
-  for (int w = 0; w < warp; ++w) {
-    a += warp_sums[w][0];
-    b += warp_sums[w][1];
+  if constexpr (WARPS <= 8) {
+    for (int w = 0; w < warp; ++w) {
+      a += warp_sums[w][0];
+      b += warp_sums[w][1];
+    }
+  } else {
+    static_assert(WARPS == 32, "a lane for each warp");
+    int64_t x = warp_sums[lane][0], y = warp_sums[lane][1];
+    scan_lanes2(x, y, lane);
+    x = __shfl_sync(0xffffffffu, x, (warp + 31) & 31);
+    y = __shfl_sync(0xffffffffu, y, (warp + 31) & 31);
+    if (warp > 0) {
+      a += x;
+      b += y;
+    }
   }
 }
 
-template <typename Index>
+template <typename Index, int THREADS>
 __global__ void __launch_bounds__(THREADS) paged_slots_kernel(SlotParams<Index> p, KernelCtl ctl) {
   __shared__ int64_t warp_sums[THREADS / 32][2];
   __shared__ int64_t s_end[THREADS];    // tokens of the requests up to and with this one
@@ -68,9 +85,11 @@ __global__ void __launch_bounds__(THREADS) paged_slots_kernel(SlotParams<Index> 
   __shared__ int64_t s_first[THREADS];  // its first entry of the free list
   __shared__ int64_t s_old[THREADS], s_want[THREADS];  // its blocks before and after
   pdl_begin();
-  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * TOKENS_PER_CTA;
-  const int64_t t1 = min(t0 + TOKENS_PER_CTA, p.tokens);
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * (2 * THREADS);
+  const int64_t t1 = min(t0 + 2 * THREADS, p.tokens);
   const int64_t room = p.max_blocks * p.block_size;
+  // Dividends below 2^32: lengths and block_size are below 2^31, and so is the number of tokens.
+  const auto blocks_of = [&](int64_t n) -> int64_t { return static_cast<uint32_t>(n) / static_cast<uint32_t>(p.block_size); };
   int64_t token_base = 0, free_base = 0;  // sums over the requests of earlier rounds
   bool bad = false;
   for (int64_t base = 0; base < p.batch; base += THREADS) {
@@ -85,10 +104,10 @@ __global__ void __launch_bounds__(THREADS) paged_slots_kernel(SlotParams<Index> 
     }
     const int64_t end = min(has + min(gets, room), room);
     gets = min(gets, p.tokens);  // a larger count overruns the token buffer in any case
-    const int64_t old = (has + p.block_size - 1) / p.block_size;
-    const int64_t want = (end + p.block_size - 1) / p.block_size;
+    const int64_t old = blocks_of(has + p.block_size - 1);
+    const int64_t want = blocks_of(end + p.block_size - 1);
     int64_t tokens = gets, blocks = want - old;
-    scan2(tokens, blocks, warp_sums);
+    scan2<THREADS / 32>(tokens, blocks, warp_sums);
     const int64_t first = free_base + blocks - (want - old);
     s_end[threadIdx.x] = token_base + tokens;
     s_has[threadIdx.x] = has;
@@ -121,7 +140,7 @@ __global__ void __launch_bounds__(THREADS) paged_slots_kernel(SlotParams<Index> 
       }
       const int64_t before = lo == 0 ? token_base : s_end[lo - 1];
       const int64_t position = s_has[lo] + t - before;
-      const int64_t j = position / p.block_size;
+      const int64_t j = blocks_of(position);
       int64_t block = -1;
       if (j < s_old[lo]) {
         block = static_cast<int64_t>(p.tables[(base + lo) * p.max_blocks + j]);
@@ -148,6 +167,13 @@ __global__ void __launch_bounds__(THREADS) paged_slots_kernel(SlotParams<Index> 
   if (bad) atomicOr(ctl.status, RK_DEV_ERR_BAD_INDEX);
 }
 
+template <typename Index, int THREADS>
+cudaError_t launch(const SlotParams<Index>& p, const KernelCtl& ctl, cudaStream_t s) {
+  const int64_t ctas = (p.tokens + 2 * THREADS - 1) / (2 * THREADS);
+  return launch_kernel(paged_slots_kernel<Index, THREADS>, dim3(static_cast<unsigned>(ctas < 1 ? 1 : ctas)), dim3(THREADS), 0,
+                       s, 0, p, ctl);
+}
+
 template <typename Index>
 cudaError_t launch(const PagedSlotsArgs& a, const KernelCtl& ctl, cudaStream_t s) {
   SlotParams<Index> p{};
@@ -164,9 +190,8 @@ cudaError_t launch(const PagedSlotsArgs& a, const KernelCtl& ctl, cudaStream_t s
   p.block_size = a.block_size;
   p.free_count = a.free_count;
   p.tokens = a.tokens;
-  const int64_t ctas = (a.tokens + TOKENS_PER_CTA - 1) / TOKENS_PER_CTA;
-  return launch_kernel(paged_slots_kernel<Index>, dim3(static_cast<unsigned>(ctas < 1 ? 1 : ctas)), dim3(THREADS), 0,
-                       s, 0, p, ctl);
+  // One round of the scan for up to 1024 requests.
+  return a.batch > FEW ? launch<Index, MANY>(p, ctl, s) : launch<Index, FEW>(p, ctl, s);
 }
 
 }  // namespace

@@ -57,9 +57,12 @@ def _case(seed, batch, longest, most, block_size, extra=0):
         (33, 100, 700, 24, 1000),   # several CTAs of tokens, padding across a CTA's edge
         (255, 50, 2, 8, 3),
         (256, 50, 3, 8, 0),
-        (257, 50, 3, 8, 0),         # a second round of requests
+        (257, 50, 3, 8, 0),         # larger CTAs
         (700, 20, 5, 4, 129),
         (2, 0, 40000, 64, 1),
+        (1024, 9, 30, 5, 0),
+        (1025, 40, 1, 16, 7),       # a second round of requests
+        (2500, 3, 4, 2, 5000),
     ],
 )
 def test_matches_a_loop(batch, longest, most, block_size, padding, index):
