@@ -27,8 +27,8 @@
 // run leaves its token in its block's claim (workspace), and only where a claim shows a second
 // run of the block are the earlier slots read.  The claims need no clearing: whatever they
 // held is checked against the slots.  The storing launch starts beside it and waits for it only
-// when its first rows are there (13k tokens of 4 heads of 64: 9.7 us, and 10.5 with the runs listed
-// by the first launch).
+// when its first rows are there (13k tokens of 4 heads of 64: 9.0 us, 0.8 more with the runs listed by
+// the first launch).
 //
 // What bounds it.  A decode step: launch and latency (a token each of 128 requests, 8 heads of
 // 128: 3.6 us on the device).  A prefill: the bytes, 2 in and 1 out per element (43k
