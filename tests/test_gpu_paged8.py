@@ -450,6 +450,21 @@ def test_scales_far_apart(kind):
         p.check(p.run())
 
 
+@pytest.mark.parametrize("batch, kv_heads, dim", [(33, 3, 256), (1000, 2, 64), (5000, 1, 128)])
+def test_thousands_of_short_sequences(batch, kv_heads, dim):
+    p = Problem([(7 * b) % 4 if b % 11 else 40 for b in range(batch)], 2 * kv_heads, kv_heads, dim, 8, "fp16", "int8", seed=batch)
+    p.check(p.run())
+
+
+@pytest.mark.parametrize("tokens", [255, 256, 257, 512, 513])
+def test_append_at_the_edges_of_its_forms(tokens):
+    rng = np.random.default_rng(tokens)
+    for lengths in ([tokens], [1] * tokens, [tokens - 200, 90, 110]):
+        blocks = sum(-(-n // 16) + 1 for n in lengths) + 1
+        slots = _prefill_slots(rng, blocks, 16, lengths)
+        _append(rng, _rows(rng, tokens, 1, 64, "fp16"), slots, "e4m3", blocks, 16)
+
+
 @pytest.mark.parametrize("exponent", [-126, -120, 120, 127])
 def test_value_scales_at_the_ends_of_fp32(exponent):
     p = Problem([1, 45, 300], 8, 2, 128, 16, "bf16", "int8", seed=31)
