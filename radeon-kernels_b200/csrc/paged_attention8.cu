@@ -59,19 +59,16 @@
 #include "rk_cache8.cuh"
 #include "rk_device.cuh"
 #include "rk_internal.h"
+#include "rk_paged8_shares.h"
 
 namespace rk {
 namespace pa8 {
 
-constexpr int WARPS = 4;
 constexpr int THREADS = WARPS * 32;
 // Units of a warp's ring.  Three kept more bytes under way and cost more (8 x 15317 positions of 3 heads
 // of 256: 51.9 us, and 46.5 with two; 61 sequences of 1 to 16 Ki, 4 heads of 128: 26.4, 25.3; 4 x 128
 // Ki the same).
 constexpr int STAGES = 2;
-// What starting and ending a range costs, in units (1 to 6 measured the same within 3 %: ragged batch 25.5
-// to 25.8 us, 64 x 512 positions 23.1 to 24.0).
-constexpr int RANGE_COST = 2;
 // Ranges over more CTAs than JOIN_ONCE are joined in two steps, JOIN_CTAS at a time first (one
 // sequence of 20000 positions, one KV head of 128 with 4 query heads, 40 CTAs: 32 us at once, 15 in
 // two steps; 17 CTAs of head_dim 256 with 8 query heads: 18.6 and 21.4).
@@ -82,9 +79,6 @@ constexpr float NONE = -3.402823466e38f;  // a maximum before any score: finite,
 // CTAs of an SM, which the registers allow (held to 168 for three: 4 x 128 Ki positions 209 -> 215
 // us, 16 x 2048 21.5 -> 23.9).
 constexpr int CTAS_PER_SM = 2;
-
-// Positions of a unit, which is one tile of a warp.
-__host__ __device__ constexpr int unit_of(int head_dim) { return head_dim == 256 ? 16 : 32; }
 
 // Shared memory of a tile.  The 16-byte chunks of a row are exchanged by its number (chunk ^
 // row % 8), so that the 128-bit reads of the MMA operands touch every bank once; at D 64,
@@ -174,12 +168,6 @@ __device__ __forceinline__ int block_of(const Params& p, int t) {
   return static_cast<int>(static_cast<uint64_t>(static_cast<uint32_t>(t)) * p.block_multiplier >> p.block_shift);
 }
 
-// Units of one (sequence, head tile); an empty sequence has one, which writes its NaN.
-template <int D>
-__device__ __forceinline__ int units_of(int context) {
-  return context <= unit_of(D) ? 1 : (context + unit_of(D) - 1) / unit_of(D);
-}
-
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
@@ -215,34 +203,6 @@ __device__ __forceinline__ float lg2_approx(float x) {
   asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-
-// a / b for quotients below 2^21, where fp32 is off by one at most.
-__device__ __forceinline__ uint32_t quotient(uint32_t a, uint32_t b) {
-  uint32_t q = static_cast<uint32_t>(__fdividef(static_cast<float>(a), static_cast<float>(b)));
-  const int rest = static_cast<int>(a - q * b);
-  if (rest < 0) --q;
-  if (rest >= static_cast<int>(b)) ++q;
-  return q;
-}
-
-// The shares of all warps: `extra` of them hold base + 1 places, the others base.  The host has
-// checked that the places of the largest lengths fit 32 bits.
-struct Shares {
-  uint32_t total, warps, base, extra;
-  __device__ __forceinline__ void set(uint32_t places, uint32_t most_warps) {
-    total = places;
-    warps = min(most_warps, places);
-    base = quotient(places, warps);
-    extra = places - base * warps;
-  }
-  __device__ __forceinline__ uint32_t start(uint32_t w) const { return w * base + min(w, extra); }
-  // The warp that holds a place.
-  __device__ __forceinline__ uint32_t owner(uint32_t place) const {
-    const uint32_t wide = extra * (base + 1);
-    const bool in = place < wide;
-    return (in ? 0u : extra) + quotient(in ? place : place - wide, in ? base + 1 : base);
-  }
-};
 
 // The parts in the workspace of a range that starts at `place`: that of the warp that begins it,
 // one of each later CTA (of its first warp), and one of the warp that ends it where that
@@ -314,13 +274,9 @@ __device__ __forceinline__ int k_chunk(int c, int i) {
   return D == 64 ? c : 2 * c + (i & 1) + 8 * (i >> 1);
 }
 
-// A place in the row of all units: sequence b, KV head h and its group hg of query heads (a
-// head tile), unit c of its `units`; `left` units
-// of this warp's share from here on.  Every range is followed by RANGE_COST places that hold
-// no unit, so that shares with many short ranges hold fewer units.  The next sequence's
-// length is loaded a sequence ahead.
-struct Walk {
-  int b, h, hg, c, units, left, context;
+// A place with its sequence's length; the next sequence's is loaded a sequence ahead.
+struct Walk : Place {
+  int context;
   Raw next;
 };
 
@@ -328,13 +284,7 @@ struct Walk {
 // some valid length and is not used (left <= 0).
 template <int D>
 __device__ __forceinline__ void next_range(const Params& p, Walk& w) {
-  w.left -= w.units + RANGE_COST - w.c;
-  w.c = 0;
-  if (++w.hg < p.head_groups) return;
-  w.hg = 0;
-  if (++w.h < p.hkv) return;
-  w.h = 0;
-  ++w.b;
+  if (!next_tile(w, p.hkv, p.head_groups)) return;
   w.context = context_of(p, w.next);
   w.units = units_of<D>(w.context);
   w.next = load_raw(p.lens, p.index_bits, min(w.b + 1, p.batch - 1));
@@ -647,9 +597,9 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) paged_attention8_kernel(
     }
   };
 
-  load_pages(load.b, block_of(p, load.c * TILE), load.context);
+  if (has_units(load)) load_pages(load.b, block_of(p, load.c * TILE), load.context);
   auto load_next = [&](int stage) {  // always a group, so that the groups count the tiles
-    if (load.left > 0) {
+    if (has_units(load)) {
       if (load.c >= until) turn_page(load);
       issue(load, stage);
       const int c = load.c;
@@ -675,7 +625,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) paged_attention8_kernel(
       }
     }
   };
-  if (run.left > 0) load_queries(run.b, run.h, run.hg);
+  if (has_units(run)) load_queries(run.b, run.h, run.hg);
   const uint32_t place_first = place0;
 
 #pragma unroll 1
@@ -692,7 +642,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) paged_attention8_kernel(
   Piece mine{}, ended{};
   bool alone = false;
   float* const sums = reinterpret_cast<float*>(smem + ring);  // for the last range's part: no tile is left then
-  while (run.left > 0) {
+  while (has_units(run)) {
     const int length = min(run.units - run.c, run.left);  // units of the range that this warp holds
     const int head0 = run.h * p.group + run.hg * HEADS;
     const int nheads = min(HEADS, p.group - run.hg * HEADS);
@@ -1142,10 +1092,8 @@ rk_status launch(const Params& p, const KernelCtl& ctl, cudaStream_t s) {
     note_error("the block tables hold too many positions for one call");
     return RK_ERR_UNSUPPORTED;
   }
-  int64_t ctas = static_cast<int64_t>(device_sm_count()) * (resident < CTAS_PER_SM ? resident : CTAS_PER_SM);
-  // Not more warps than units; RANGE_COST places of a range hold none.
-  if (ranges <= ctas * WARPS && ranges * (per_range + RANGE_COST) < ctas * WARPS)
-    ctas = (ranges * (per_range + RANGE_COST) + WARPS - 1) / WARPS;
+  const int64_t ctas =
+      ctas_of(ranges, per_range, static_cast<int64_t>(device_sm_count()) * (resident < CTAS_PER_SM ? resident : CTAS_PER_SM));
   e = launch_kernel(kernel, dim3(static_cast<unsigned>(ctas)), dim3(THREADS), SMEM, s, 0, p, ctl);
   note_launch("paged_attention8_kernel");
   return cuda_status(e);
