@@ -103,7 +103,9 @@ __global__ void __launch_bounds__(THREADS) paged_slots_kernel(SlotParams<Index> 
       gets = max(gets, int64_t{0});
     }
     const int64_t end = min(has + min(gets, room), room);
-    gets = min(gets, p.tokens);  // a larger count overruns the token buffer in any case
+    // A larger count overruns the token buffer by itself: said here, for the sum no longer shows it.
+    bad = bad || gets > p.tokens;
+    gets = min(gets, p.tokens);
     const int64_t old = blocks_of(has + p.block_size - 1);
     const int64_t want = blocks_of(end + p.block_size - 1);
     int64_t tokens = gets, blocks = want - old;

@@ -132,3 +132,21 @@ def test_replayed_graph_follows_its_inputs():
         for got, expected in zip((*out, t[0]), want[:3] + (np.array([want[3]]), want[4])):
             np.testing.assert_array_equal(got.cpu().numpy(), expected)
     device_status()
+
+
+@pytest.mark.parametrize("index", ["int32", "int64"])
+@pytest.mark.parametrize("batch", [1, 5, 300, 1100])
+def test_a_single_request_overruns_the_buffer(batch, index):
+    """More tokens than the buffer holds are reported, whichever request has them all."""
+    for at in {0, batch // 2, batch - 1}:
+        gets = np.zeros(batch, int)
+        gets[at] = 100
+        tables = np.full((batch, 8), -1)
+        for tokens in (99, 50, 1, 0):
+            _run(tables, np.zeros(batch, int), gets, list(range(20)), tokens, 16, index)
+        _run(tables, np.zeros(batch, int), gets, list(range(20)), 100, 16, index)  # just enough
+
+
+def test_no_buffer_and_tokens_to_place():
+    _run(np.full((3, 4), -1), [0, 5, 0], [1, 0, 2], [7, 8, 9], 0, 8, "int32")
+    _run(np.full((2, 4), -1), [0, 0], [1, 1], [7, 8, 9], 0, 8, "int64")
