@@ -527,8 +527,8 @@ RK_API rk_status rk_paged_cache_append_8bit_workspace_size(int64_t tokens, int64
  * sequences (NaN), clamped lengths and block-table entries out of range (skipped and
  * reported) as there; any query_heads / kv_heads and any block_size.  Scales are finite and
  * >= 0.  The caches and out are 16-byte aligned, the query 8-byte.  fp32 scores, softmax and sums;
- * the weights of V are rounded to fp16 (relative to the largest of the head), the output
- * once.  The value scales of one head lie within 2^100 of one another, zeros aside.  out does not
+ * the weights of V are rounded to fp16 -- half a step, or 2^-36 of the head's largest
+ * where that is more --, the output once.  The value scales of one head lie within 2^100 of one another, zeros aside.  out does not
  * overlap an input.  workspace: rk_paged_attention_decode_8bit_workspace_size() bytes, 16-byte
  * aligned, uninitialised, its size independent of batch and lengths; calls that may overlap
  * need one each.  max_blocks_per_sequence * block_size < 2^31 - 64, and batch * kv_heads *

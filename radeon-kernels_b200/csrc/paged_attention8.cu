@@ -40,10 +40,14 @@
 // Numbers.  Queries are brought to f16 by a power of two per head (exact unless a component is
 // below 2^-14 of the head's largest: then it keeps 2^-25 of that).  Scores, maxima, sums and
 // accumulators are fp32.  The weights of V carry its scales, w_t = p_t * vs(t) * c with c =
-// 2^(m - mo) for m the running maximum of the scores s (in powers of two) and mo that of s +
-// log2 vs, and are rounded to f16 for the product: half a step, 2^-11, of each, however the
-// scales differ from block to block, since the largest are near 1.  The maxima are raised
-// only when a weight passes them by SLACK; in between p and w may reach that, far inside the
+// 2^(m - mo) for m the reference of the scores s (in powers of two) and mo that of s + log2 vs, each
+// HEADROOM below the running maximum, and are rounded to f16 for the product: half a step, 2^-11, of
+// each that is at least 2^-25 of the largest, however the scales differ from block to block,
+// and 2^-36 of the largest for smaller ones, which vanish below that.  (With the largest near 1, 11 powers
+// of two less, a first position that takes the weight and has no value left what lies 2^-25
+// below it nothing.)  The denominator sums the p in fp32, unrounded, so n positions lose n * 2^-36 of
+// the largest weight at most.  The maxima are raised
+// only when a weight passes SLACK; in between p and w may reach that, inside the
 // range of both types, and the sums need no rescaling.
 //
 // What bounds it: the bytes of K and V, 1.07 GB in 203 to 211 us at 4 x 131072 positions of 8 heads of
@@ -73,7 +77,12 @@ constexpr int STAGES = 2;
 // sequence of 20000 positions, one KV head of 128 with 4 query heads, 40 CTAs: 32 us at once, 15 in
 // two steps; 17 CTAs of head_dim 256 with 8 query heads: 18.6 and 21.4).
 constexpr int JOIN_ONCE = 24, JOIN_CTAS = 16;
-constexpr float SLACK = 256.0f;      // a running maximum is raised when a weight is this much above it
+// The largest weight lies HEADROOM powers of two above the reference that its maximum is, so that the f16
+// weights of V reach far below it; the maxima are raised when a weight passes SLACK, inside f16's range.
+// The less lies between the two, the more often (32 x 3000 positions of 4 KV heads with 16 query
+// heads each: 35.9 us with 8 powers of two, 36.7 with these 4, 38.0 with 2; up to 8 query heads
+// the same within 1 %).
+constexpr float HEADROOM = 11.0f, SLACK = 32768.0f;
 constexpr float NONE = -3.402823466e38f;  // a maximum before any score: finite, so that -inf - NONE = -inf
 
 // CTAs of an SM, which the registers allow (held to 168 for three: 4 x 128 Ki positions 209 -> 215
@@ -761,7 +770,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) paged_attention8_kernel(
           for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              float bm = m[nt][i], bo = mo[nt][i];
+              float bm = NONE, bo = NONE;
 #pragma unroll
               for (int t = 0; t < SUB; ++t) {
 #pragma unroll
@@ -778,6 +787,8 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) paged_attention8_kernel(
                 bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, x));
                 bo = fmaxf(bo, __shfl_xor_sync(0xffffffffu, bo, x));
               }
+              bm = fmaxf(m[nt][i], bm - HEADROOM);
+              bo = fmaxf(mo[nt][i], bo - HEADROOM);
               // c = 2^(m - mo) and its inverse are kept normal numbers, for ex2.approx flushes the others
               // (scales of 2^127 or 2^-126, or none but zeros).
               bo = bm - fminf(fmaxf(bm - bo, -125.f), 125.f);

@@ -794,3 +794,84 @@ def test_refusals_after_calls_of_the_same_kind():
     with pytest.raises(TypeError, match="interleaved"):
         rk.rotary_embedding(rows, rows, positions, frequencies, interleaved=0)
     device_status()
+
+
+# ------------------------------------------------------------- weights far below the largest
+def _alike(codes, unit, heads, dim, kind, dtype, seed):
+    """1184 sequences over the same blocks, one KV head: a range for every warp of the GPU, so that a warp
+    holds all positions of a range.  Position t's score is codes[t] * unit exactly; value codes are
+    whole numbers from 1 to 15.  Returns the problem of one sequence and a call for all of them."""
+    import torch
+
+    length = len(codes)
+    p = Problem([length], heads, 1, dim, 32, dtype, kind, seed=seed)
+    pool = p.caches[0].shape[0]
+    order = p.tables[0, : -(-length // 32)].long().cpu()
+    keys, values = torch.zeros((len(order) * 32, dim)), torch.zeros((len(order) * 32, dim))
+    keys[:length, 0] = torch.tensor(codes).float()
+    values[:length] = torch.from_numpy(p.rng.integers(1, 16, (length, dim))).float()
+
+    def placed(x):
+        out = torch.zeros((pool, 32, 1, dim))
+        out[order] = x.view(-1, 32, 1, dim)
+        stored = out.to(_torch_dtype(kind))
+        assert torch.equal(stored.float(), out)  # the codes are values of the type
+        return stored.cuda()
+
+    p.caches = [placed(keys), placed(values)]
+    p.scales = [torch.ones((pool, 1), device="cuda") for _ in range(2)]
+    p.query.zero_()
+    p.query[:, :, 0] = unit
+
+    def run():
+        import radeon_kernels as rk
+
+        query, tables, lengths = (x.expand(1184, *x.shape[1:]).contiguous() for x in (p.query, p.tables, p.lengths))
+        out = rk.paged_attention_decode_8bit(query, *p.caches, *p.scales, tables, lengths, 1.0)
+        assert torch.equal(out.view(torch.int16), out[:1].expand_as(out).contiguous().view(torch.int16))
+        return out[:1].double().cpu().numpy()
+
+    return p, run
+
+
+def _definition(p):
+    return ref.attention(p.query.double().cpu().numpy(), *[_values(c) for c in p.caches],
+                         *[s.double().cpu().numpy() for s in p.scales], p.tables.cpu().numpy(), p.lengths.cpu().numpy(),
+                         1.0, p.dtype)
+
+
+def _tight(codes, unit, p):
+    """The attention's bound for `_alike`: the terms of ref.attention, but each weight of V is off by half
+    a step of fp16 (2^-11 of itself) or by 2^-36 of the largest, whichever is more; a score is one
+    product, off by 2^-24 of itself, and so is its distance to the maximum."""
+    import torch
+
+    n = len(codes)
+    blocks = p.tables[0, : -(-n // 32)].long()
+    v = p.caches[1].view(torch.uint8)[blocks].view(p.caches[1].dtype).float().reshape(-1, p.query.shape[2])[:n].double().cpu().numpy()
+    s = np.array(codes) * unit
+    w = np.exp(s - s.max())
+    w /= w.sum()
+    out = w @ v
+    bound = out * (2.0**-11 * (1 + 2.0**-10) + 2 * (3 * np.abs(s).max() * 2.0**-24 + 2.0**-18))
+    return out, bound + n * 2.0**-36 * w.max() * 15 + ref.rounding(out, p.dtype)
+
+
+@pytest.mark.parametrize("kind", ["e4m3", "int8"])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("dim, heads", [(64, 4), (128, 8), (128, 16), (256, 3)])
+@pytest.mark.parametrize("sink", [0, 5000, 8191])
+def test_weights_far_below_one_whose_value_is_zero(dim, heads, sink, dtype, kind):
+    """A position that takes nearly all the weight and has no value: the others, 2^-25 to 2^-29 of it
+    each, are the output."""
+    import torch
+
+    codes = np.random.default_rng(sink).integers(0, 10, 8192)
+    codes[sink] = 80
+    p, run = _alike(codes, 0.25, heads, dim, kind, dtype, seed=sink)
+    p.caches[1].view(torch.uint8)[int(p.tables[0, sink // 32]), sink % 32] = 0
+    out, bound = _tight(codes, 0.25, p)
+    np.testing.assert_allclose(out, _definition(p)[0][0, 0], rtol=1e-12)
+    assert (bound < out * 2.0**-6).all()  # it says something
+    got = run()
+    assert (np.abs(got - out) <= bound).all(), np.max(np.abs(got - out) / bound)
