@@ -758,7 +758,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) paged_attention8_kernel(
                 if (mask != FULL && !((mask >> row) & 1u)) x = -INFINITY;
                 const float pw = ex2_approx(x);
                 s2[nt][t][e] = pw;
-                weight[nt][t][e] = pw * (vs * c[nt][i]);
+                weight[nt][t][e] = (pw * c[nt][i]) * vs;  // in this order: see below
                 most = fmax3(most, pw, weight[nt][t][e]);
               }
             }
@@ -790,8 +790,10 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) paged_attention8_kernel(
               bm = fmaxf(m[nt][i], bm - HEADROOM);
               bo = fmaxf(mo[nt][i], bo - HEADROOM);
               // c = 2^(m - mo) and its inverse are kept normal numbers, for ex2.approx flushes the others
-              // (scales of 2^127 or 2^-126, or none but zeros).
-              bo = bm - fminf(fmaxf(bm - bo, -125.f), 125.f);
+              // (scales of 2^127 or 2^-126, or none but zeros), and c at most 2^110: then p * c is finite
+              // up to SLACK, and 0 where p is, so that a weight is NaN only where p or vs is -- whatever
+              // scales follow blocks of smaller ones or of zeros.
+              bo = bm - fminf(fmaxf(bm - bo, -125.f), 110.f);
               l[nt][i] *= ex2_approx(m[nt][i] - bm);
               const float down = ex2_approx(mo[nt][i] - bo);
               c[nt][i] = ex2_approx(bm - bo);
@@ -811,7 +813,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) paged_attention8_kernel(
                   float x = fmaf(s[nt][t][2 * r + i], ks * factor[nt][i], -bm);
                   if (!((mask >> row) & 1u)) x = -INFINITY;
                   s2[nt][t][2 * r + i] = ex2_approx(x);
-                  weight[nt][t][2 * r + i] = s2[nt][t][2 * r + i] * (vs * c[nt][i]);
+                  weight[nt][t][2 * r + i] = (s2[nt][t][2 * r + i] * c[nt][i]) * vs;
                 }
               }
             }

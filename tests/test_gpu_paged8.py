@@ -875,3 +875,22 @@ def test_weights_far_below_one_whose_value_is_zero(dim, heads, sink, dtype, kind
     assert (bound < out * 2.0**-6).all()  # it says something
     got = run()
     assert (np.abs(got - out) <= bound).all(), np.max(np.abs(got - out) / bound)
+
+
+@pytest.mark.parametrize("kind", ["e4m3", "int8"])
+@pytest.mark.parametrize("dim, heads", [(64, 4), (128, 8), (128, 16), (256, 3)])
+@pytest.mark.parametrize("rise", [0, 4, 28])
+def test_value_scales_of_zero_before_larger_ones(dim, heads, rise, kind):
+    """Blocks whose value scale is 0 hold the largest scores, the blocks behind them have large value
+    scales: weights that vanish leave a 0, those that do not count as ever."""
+    for low in (-60, -30, 0):
+        codes = [60] * 64 + [60 + rise] * 64 + [low] * 128
+        p, run = _alike(codes, 1.0, heads, dim, kind, "bf16", seed=-low)
+        p.scales[1][p.tables[0, :4].long()] = 0.0
+        for scale in (2.0**4, 2.0**60, 2.0**100):
+            p.scales[1][p.tables[0, 4:8].long()] = scale
+            got = run()
+            want, bound = _definition(p)
+            assert np.isfinite(got).all(), (low, scale)
+            # Exponentials below 2^-126 of the largest are 0.
+            assert (np.abs(got - want) <= bound + 256 * 2.0**-126 * scale * 15).all(), (low, scale)
