@@ -428,6 +428,7 @@ __device__ __forceinline__ void join(const Params& p, const Piece& piece, int fr
     if (out) {
       sums.write(p, static_cast<int64_t>(piece.row) + h, column);
     } else {
+      __syncwarp(0xFFFFu << (threadIdx.x & 16));  // all lanes of the head have read the statistics that lane 0 replaces
       sums.store(part_of<D, HEADS>(p, parts.warp(from), parts.slot(from)) + h * part_stride(D), column);
     }
   }

@@ -894,3 +894,17 @@ def test_value_scales_of_zero_before_larger_ones(dim, heads, rise, kind):
             assert np.isfinite(got).all(), (low, scale)
             # Exponentials below 2^-126 of the largest are 0.
             assert (np.abs(got - want) <= bound + 256 * 2.0**-126 * scale * 15).all(), (low, scale)
+
+
+@pytest.mark.parametrize("query_heads, dim", [(1, 64), (3, 128), (5, 256), (13, 128), (16, 64)])
+def test_joins_in_two_steps_of_every_number_of_heads(query_heads, dim):
+    """One sequence over all SMs, whose parts are joined a group of CTAs at a time into the first one's:
+    odd numbers of heads leave half of a warp idle; the same bits every time."""
+    import torch
+
+    p = Problem([40000 if dim < 256 else 20000], query_heads, 1, dim, 64, "fp16", "e4m3", seed=query_heads)
+    out = p.run()
+    want, bound = _plain64(p)
+    assert ((out.double() - want).abs() <= bound).all()
+    for _ in range(50):
+        assert torch.equal(p.run(), out)
