@@ -38,14 +38,14 @@ POSITIONAL_CALLS = 8192  # kinds of call that a runtime keeps ready
 WINNER_FAILURES = (PackResolutionError, ArtifactError, native.NativeProviderError, RuntimeError, TypeError, ValueError)
 
 
-# Every runtime's loaders, for loaded_modules(); a loader that is gone takes its entry along.
-_LOADERS: weakref.WeakSet[Any] = weakref.WeakSet()
+# Every runtime, for loaded_modules(); one that is gone takes its entry along.
+_RUNTIMES: weakref.WeakSet[Any] = weakref.WeakSet()
 
 
 def loaded_modules() -> list[Any]:
     """The pack modules that a runtime of this process has loaded and that keep a status word."""
 
-    modules = {id(m): m for loader in list(_LOADERS) for m in getattr(loader, "modules", ())}
+    modules = {id(m): m for runtime in list(_RUNTIMES) for loader in runtime.loaders() for m in getattr(loader, "modules", ())}
     return [m for m in modules.values() if hasattr(m, "device_status")]
 
 
@@ -99,6 +99,7 @@ class DispatchingRuntime:
         # lifetime of a runtime, so the decision cannot change; reset_*runtime() drops it.
         self._fast: dict[tuple, tuple[Any, Any, dict[str, Any]]] = {}
         self._fast_positional: dict[tuple, tuple[Any, Any, dict[str, Any]]] = {}
+        _RUNTIMES.add(self)
 
     @property
     def pack_registry(self) -> KernelPackRegistry:
@@ -115,8 +116,11 @@ class DispatchingRuntime:
         with self._lock:
             if root not in self._loaders:
                 self._loaders[root] = self._loader_factory(root)
-                _LOADERS.add(self._loaders[root])
             return self._loaders[root]
+
+    def loaders(self) -> list[PrecompiledArtifactLoader]:
+        with self._lock:
+            return list(self._loaders.values())
 
     @staticmethod
     def fast_key(operator: str, device_index: int, signature: Mapping[str, Any]) -> tuple:

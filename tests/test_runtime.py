@@ -273,3 +273,32 @@ def test_operator_runtime_passes_launch_parameters_to_the_winner(tmp_path):
     assert _run(runtime) == "native:input:{'variant': 2}"
     assert packs.calls == 1
     assert get_last_dispatch()["selected"] == "native/run"
+
+
+def test_a_loader_of_any_kind_serves_the_winner(tmp_path):
+    """Loaders need not be hashable or weakly referenced; what they loaded is found for the device status."""
+    from radeon_kernels.ops._runtime import loaded_modules
+
+    module = SimpleNamespace(device_status=lambda: 0)
+
+    class Slotted:
+        __slots__ = ("modules", "load_entrypoint")
+        __hash__ = None
+
+    def make(_root):
+        loader = Slotted()
+        loader.modules = (module,)
+        loader.load_entrypoint = _Loader(_root).load_entrypoint
+        return loader
+
+    runtime, _ = _operator_runtime(tmp_path, winner=True)
+    runtime._loader_factory = make
+    clear_last_dispatch()
+    assert _run(runtime) == "native:input:{'variant': 2}"
+    assert get_last_dispatch()["selected"] == "native/run"
+    assert any(m is module for m in loaded_modules())
+    del runtime
+    import gc
+
+    gc.collect()
+    assert not any(m is module for m in loaded_modules())
