@@ -443,6 +443,12 @@ at::Tensor vector_rows(const at::Tensor& t, const char* name) {
   return rows.clone(at::MemoryFormat::Contiguous);
 }
 
+// No kernel carries forward-mode tangents: refused, where they would be lost.
+void check_no_tangents(std::initializer_list<const at::Tensor*> tensors) {
+  for (const at::Tensor* t : tensors)
+    TORCH_CHECK(!t->_fw_grad(/*level=*/0).defined(), "forward-mode gradients are not supported");
+}
+
 // Rotary positions (rk_rotary_embedding): new dense [query_out, key_out].
 std::vector<at::Tensor> rotary_forward(const at::Tensor& query_in, const at::Tensor& key_in,
                                        const at::Tensor& positions_in, const at::Tensor& frequencies_in,
@@ -504,6 +510,7 @@ struct RotaryFunction : public torch::autograd::Function<RotaryFunction> {
 
 std::vector<at::Tensor> rotary_embedding(const at::Tensor& query, const at::Tensor& key, const at::Tensor& positions,
                                          const at::Tensor& frequencies, bool interleaved, double amplitude, bool inverse) {
+  check_no_tangents({&query, &key, &frequencies});
   if (at::GradMode::is_enabled() && (query.requires_grad() || key.requires_grad()))
     return RotaryFunction::apply(query, key, positions, frequencies, interleaved, amplitude, inverse);
   return rotary_forward(query, key, positions, frequencies, interleaved, amplitude, inverse);
@@ -560,6 +567,7 @@ class Scratch {
 
 void check_no_grad(std::initializer_list<const at::Tensor*> tensors) {
   for (const at::Tensor* t : tensors) TORCH_CHECK(!t->requires_grad(), "inference only: no input may require gradients");
+  check_no_tangents(tensors);
 }
 
 rk_cache_dtype cache_dtype_of(const at::Tensor& t, const char* name) {

@@ -7,7 +7,8 @@ block_tables, context_lengths, scale=None)``.
 ``block_slot_head_dim``, as the 16-bit cache of ``rk.paged_attention_decode``) hold
 ``torch.float8_e4m3fn`` or ``torch.int8``; ``key_scales`` / ``value_scales`` ``[num_blocks,
 kv_heads]`` float32 hold one scale per block and head, and a stored value stands for itself
-times its scale.  head_dim 64, 128 or 256; inference only.
+times its scale.  head_dim 64, 128 or 256; inference only: inputs that require gradients or carry
+forward-mode tangents are refused.
 
 The append stores ``key`` / ``value`` ``[tokens, kv_heads, head_dim]`` (fp16/bf16, slices of a
 projection are read in place) at ``slot_mapping [tokens]`` (int32/int64, ``block * block_size +

@@ -8,7 +8,7 @@ len(frequencies)`` elements of each head are pairs ``(i, i + n)``, or ``(2i, 2i 
 a sin)`` at the angle ``p * frequencies[i]``; the rest of the head is copied.  The result is a
 new dense pair ``(query, key)``.  Queries and keys that are slices of one projection are read
 in place (any stride between tokens and heads); inputs that require gradients get the inverse
-rotation of theirs.
+rotation of theirs.  Forward-mode tangents are refused.
 
 ``frequencies`` (float64, radians per position) is computed once by
 :func:`rotary_frequencies`, which also knows the usual rules for stretching a model's context.

@@ -301,3 +301,36 @@ def test_on_a_side_stream():
     torch.cuda.current_stream().wait_stream(side)
     torch.cuda.synchronize()
     _check(out, query, positions, frequencies, False, 1.0, "bf16")
+
+
+@pytest.mark.parametrize("requires_grad", [False, True])
+def test_forward_mode_tangents_are_refused(requires_grad):
+    """Refused by first calls and by calls of a kind that has been served."""
+    import torch
+    from torch.autograd import forward_ad
+
+    import radeon_kernels as rk
+
+    rows = torch.randn((3, 2, 64), device="cuda").bfloat16()
+    frequencies, positions = rk.rotary_frequencies(64), torch.arange(3, device="cuda")
+    caches = [torch.zeros((1, 16, 2, 64), dtype=torch.int8, device="cuda") for _ in range(2)]
+    scales = [torch.ones((1, 2), device="cuda") for _ in range(2)]
+    tables = torch.zeros((3, 1), dtype=torch.int64, device="cuda")
+    for served in (False, True):
+        if served:
+            rk.rotary_embedding(rows, rows, positions, frequencies)
+            rk.paged_cache_append_8bit(rows, rows, *caches, *scales, positions)
+            rk.paged_attention_decode_8bit(rows, *caches, *scales, tables, positions)
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(rows.clone().requires_grad_(requires_grad), torch.ones_like(rows))
+            for query, key in ((dual, rows), (rows, dual)):
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    rk.rotary_embedding(query, key, positions, frequencies)
+            if requires_grad:
+                continue  # the others refuse that in any case
+            for key, value in ((dual, rows), (rows, dual)):
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    rk.paged_cache_append_8bit(key, value, *caches, *scales, positions)
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                rk.paged_attention_decode_8bit(dual, *caches, *scales, tables, positions)
+            assert not caches[0].any() or served
