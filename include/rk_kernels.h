@@ -469,7 +469,8 @@ RK_API rk_status rk_rotary_embedding(const void* query, const void* key, const v
  *   blocks_used     [1]: entries of free_blocks that the step needs.
  * All index arrays but slot_mapping are int32 or int64 (index_bits).  Where free_blocks is too
  * short, entries and slots that miss a block are -1; tokens past the end of their table row
- * and those of an entry below 0 have slot -1; a negative length counts as 0.  Each of these,
+ * and those of an entry below 0, or of one whose slots exceed 64 bits, have slot -1; a negative
+ * length counts as 0.  Each of these,
  * and more tokens than `tokens`, makes the next rk_device_status() report
  * RK_ERR_INVALID_ARGUMENT (blocks_used > free_count says that the list was too short).
  * batch, max_blocks, block_size >= 1; tokens, free_count >= 0; max_blocks * block_size <

@@ -35,6 +35,7 @@ struct SlotParams {
   Index* lengths;
   Index* used;
   int64_t batch, max_blocks, block_size, free_count, tokens;
+  int64_t most_block;  // whose slots fit 64 bits
 };
 
 // Inclusive sums over the lanes of two values.
@@ -150,6 +151,7 @@ __global__ void __launch_bounds__(THREADS) paged_slots_kernel(SlotParams<Index> 
         const int64_t at = s_first[lo] + j - s_old[lo];
         if (at < p.free_count) block = static_cast<int64_t>(p.free_blocks[at]);
       }
+      if (block > p.most_block) block = -1;
       bad = bad || block < 0;
       p.slots[t] = block < 0 ? -1 : block * p.block_size + position - j * p.block_size;
       p.positions[t] = static_cast<Index>(position);
@@ -192,6 +194,7 @@ cudaError_t launch(const PagedSlotsArgs& a, const KernelCtl& ctl, cudaStream_t s
   p.block_size = a.block_size;
   p.free_count = a.free_count;
   p.tokens = a.tokens;
+  p.most_block = (INT64_MAX - (a.block_size - 1)) / a.block_size;
   // One round of the scan for up to 1024 requests.
   return a.batch > FEW ? launch<Index, MANY>(p, ctl, s) : launch<Index, FEW>(p, ctl, s);
 }

@@ -150,3 +150,24 @@ def test_a_single_request_overruns_the_buffer(batch, index):
 def test_no_buffer_and_tokens_to_place():
     _run(np.full((3, 4), -1), [0, 5, 0], [1, 0, 2], [7, 8, 9], 0, 8, "int32")
     _run(np.full((2, 4), -1), [0, 0], [1, 1], [7, 8, 9], 0, 8, "int64")
+
+
+@pytest.mark.parametrize("block_size", [2, 5, 16, 2**20])
+def test_entries_whose_slots_exceed_64_bits(block_size):
+    """They have no slot and are reported, in a table as in the free list; the largest that fit are mapped."""
+    import torch
+
+    import radeon_kernels as rk
+
+    most = (2**63 - 1 - (block_size - 1)) // block_size
+    for held, free, well in ((most, most - 1, True), (most, 2**63 - 1, False), (2**63 - 1, most, False), (2**62, 2**62, None)):
+        fits = [b <= most for b in (held, free)]
+        tables = torch.tensor([[held, -1]], device="cuda")
+        slots, *_ = rk.paged_slots(tables, torch.tensor([1], device="cuda"), torch.tensor([block_size], device="cuda"),
+                                   torch.tensor([free], device="cuda"), num_tokens=block_size, block_size=block_size)
+        want = [held * block_size + i if fits[0] else -1 for i in range(1, block_size)]
+        want.append(free * block_size if fits[1] else -1)
+        assert slots.tolist() == want
+        assert device_status() == (_native.RK_OK if all(fits) else _native.RK_ERR_INVALID_ARGUMENT)
+        if well is not None:
+            assert all(fits) == well
